@@ -32,7 +32,6 @@ import sys
 
 EVERY = int(os.environ.get("S2L_CONV_EVERY", "12"))   # one group of memory instructions behind every EVERY-th MFMA of a chunk
 EVERY_FIRST = int(os.environ.get("S2L_CONV_EVERY_FIRST", "10"))   # ... of a tile's first chunk (DMA and the stores of the tile before)
-TRACE = os.environ.get("S2L_CONV_TRACE") == "1"      # experiment builds only (tools/trace_conv_asm.py): per-tile timestamps
 HALO_BYTES, W_BYTES = 18 * 18 * 64, 9 * 4 * 64 * 16
 BUF = HALO_BYTES + W_BYTES           # 57 600
 
@@ -76,12 +75,10 @@ S = _scalar_map(8,
                 singles="LDSB CA CB COUT H W TILESX TILESY NCT TILE TEND NCH CC WAVE TX TY CT FRAME NTX NTY NCTN NFR X0 Y0 BORDER "
                         "CHB T0 T1 T2 T3 FO OB1 OB2".split(),
                 pairs=("P0", "INA", "INB", "WB", "BIAS", "OUT", "POOL", "M0_", "M1_", "M2_", "M3_", "M4_", "M5_", "VALID2", "VALID3",
-                       "COLOK", "SRC", "WCH", "OUTF", "POOLF", "TOFF", "SM0", "SM1", "SM2", "SM3", "PM0", "PM1")
-                      + (("TRACE",) if TRACE else ()))
+                       "COLOK", "SRC", "WCH", "OUTF", "POOLF", "TOFF", "SM0", "SM1", "SM2", "SM3", "PM0", "PM1"))
 S["GATE"], S["GATE1"], S["GATEF"], S["GATEF1"], S["LASTF"], S["LASTF1"] = S["POOL"], S["POOL1"], S["POOLF"], S["POOLF1"], S["PM0"], S["PM01"]   # (lin)
 S["OB0"] = S["CB"]                                  # (fwd_out: the output bias; CB is dead once NCH is known)
 S["KARG"], S["KARG1"] = S["P0"], S["P01"]          # the kernel-argument pointer is dead once the arguments are loaded
-S["TS"], S["TS1"], S["TA"], S["TA1"] = S["COLOK"], S["COLOK1"], S["P0"], S["P01"]   # (trace builds: both are dead at the trace points)
 S_LAST = max(S.values())
 assert S_LAST <= 101, S_LAST
 
@@ -117,29 +114,6 @@ class Body:
         assert newer <= 15
         self.e(f"s_waitcnt lgkmcnt({newer})")
         self.lds = self.lds[len(self.lds) - newer:] if newer else []
-
-    def trace(self, slot, plus_cc=False):
-        """experiment builds: wave 0 stores s_memtime to trace[TILE][slot (+ CC)] (24 slots of 8 bytes per tile)"""
-        if not TRACE:
-            return
-        e = self.e
-        skip = self.label("notrace")
-        e(f"s_memtime {s2('TS')}")
-        e(f"s_cmp_eq_u64 {s2('TRACE')}, 0")
-        e(f"s_cbranch_scc1 {skip}")
-        e(f"s_cmp_eq_u32 {s('WAVE')}, 0")
-        e(f"s_cbranch_scc0 {skip}")
-        e(f"s_mul_i32 {s('TA')}, {s('TILE')}, 192")
-        e(f"s_add_u32 {s('TA')}, {s('TA')}, {8 * slot}")
-        if plus_cc:
-            e(f"s_lshl_b32 {s('TA1')}, {s('CC')}, 3")
-            e(f"s_add_u32 {s('TA')}, {s('TA')}, {s('TA1')}")
-        e(f"s_add_u32 {s('TA')}, {s('TRACE')}, {s('TA')}")
-        e(f"s_addc_u32 {s('TA1')}, {s('TRACE1')}, 0")
-        e("s_waitcnt lgkmcnt(0)")
-        e(f"s_store_dwordx2 {s2('TS')}, {s2('TA')}, 0")
-        e("s_waitcnt lgkmcnt(0)")
-        e(f"{skip}:")
 
     @staticmethod
     def acc(mb, g):
@@ -325,7 +299,6 @@ class Body:
                 assert not self.lds
                 e("s_waitcnt vmcnt(0)")
                 e("s_barrier")
-                self.trace(2, plus_cc=True)
                 if read_next:
                     late = self.tap_reads(1 - b, 0, 1 - b, "entry")
             base = V_OPS[(t + b) % 2]
@@ -517,8 +490,6 @@ class Body:
         for dst, off in (("CA", "oCA"), ("CB", "oCB"), ("COUT", "ocout"), ("H", "oH"), ("W", "oW"), ("TILESX", "otx"), ("TILESY", "oty"),
                          ("NCT", "onct")):
             e(f"s_load_dword {s(dst)}, {s2('KARG')}, %[{off}]")
-        if TRACE:
-            e(f"s_load_dwordx2 {s2('TRACE')}, {s2('KARG')}, %[otrace]")
         if self.lin:
             e(f"s_load_dwordx2 {s2('GATE')}, {s2('KARG')}, %[ogate]")
         if self.fuse:      # POOL <- out3; output weights and bias through PM0 / PM1 (zeroed below)
@@ -616,7 +587,6 @@ class Body:
         self.first_tap_reads(0)
 
         e("S2LC_TILE:")
-        self.trace(0)
         # accumulators = bias of this channel tile (the C++ kernel's initial value; loaded when the tile's fetch was set up)
         for mb in range(4):
             for g in range(4):
@@ -626,7 +596,6 @@ class Body:
                     else:
                         e(f"v_accvgpr_read_b32 v{V_ACC + (mb * 4 + g) * 4 + r}, a{A_BIAS + 4 * mb + r}")
         e(f"s_mov_b32 {s('CC')}, 0")
-        self.trace(1)
         # ---- chunk 0 (buffer 0): fetches chunk 1 of the same tile, and issues the stores of the tile before
         self.advance_in_tile()
         self.zero_fill(1)
@@ -703,7 +672,6 @@ class Body:
         e("s_cbranch_scc1 S2LC_EVEN")
         # ---- the tile is complete
         self.tile_end()
-        self.trace(20)
         e(f"s_add_u32 {s('TILE')}, {s('TILE')}, 1")
         e(f"s_mov_b32 {s('TX')}, {s('NTX')}")
         e(f"s_mov_b32 {s('TY')}, {s('NTY')}")
@@ -716,8 +684,6 @@ class Body:
             for x in grp:
                 e(x)
         e("s_waitcnt vmcnt(0)")
-        if TRACE:
-            e("s_dcache_wb")
         return self.L
 
 
@@ -744,7 +710,7 @@ def main(outdir):
                 + [f"s{r}" for r in range(8, S_LAST + 1) if r not in (32, 33)] + ["vcc", "scc", "memory"])
         out = ["// GENERATED by csrc/gen_conv_body.py -- do not edit; the generator is the source.", "asm volatile("]
         out += [f'    "{x}\\n\\t"' for x in lines]
-        out.append(OPERANDS.rstrip("\n") + (',\n        [otrace] "n"(offsetof(ConvArgs, trace))' if TRACE else ""))
+        out.append(OPERANDS.rstrip("\n"))
         out.append("      : " + ", ".join(f'"{c}"' for c in clob) + ");")
         with open(os.path.join(outdir, f"conv_body_{variant}.inc"), "w") as f:
             f.write("\n".join(out) + "\n")

@@ -23,14 +23,13 @@ fwd_bf16_kernel: activation images, mask dwords and rgb are bit-identical.
     different instructions, meeting only in L2 -- the same modifier had cost a factor of two).
 
 State: bit-identical; 3.04 ms against the C++ kernel's 3.3-3.4 ms.  S2L_FWD_EXP builds ablate stores / epilogue /
-MFMAs / DMA / barrier, S2L_FWD_TRACE=1 builds time the phases of every stage (tools/trace_fwd16.py).
+MFMAs / DMA / barrier.
 
 Layer bodies: A (layer 0: x only, -> P), B (h from P -> Q: layers 1, 3, 7), C (h from Q -> P: 2, 4, 6), D (layer 5: x + h from P ->
 Q); four stages each, sequenced by a scalar layer counter."""
 import os
 import sys
 
-TRACE = os.environ.get("S2L_FWD_TRACE") == "1"      # experiment builds (tools/trace_fwd16.py): per-stage phase timestamps of wave 0
 BX_MODE = os.environ.get("S2L_FWD_BX", "kloop")      # embedded rows of the next tile: "start" = loaded at its start (exposed), "epilogue" / "kloop" = prefetched in layer 6
 BX_AT_TILE_START = BX_MODE == "start"   # embedded rows of a tile: loaded at its start (exposed) or prefetched in layer 6
 EXP = int(os.environ.get("S2L_FWD_EXP", "0"))      # timing experiments (results wrong): 1 no image stores, 2 no epilogue VALU, 4 no MFMAs, 8 no stage DMA, 16 no barrier
@@ -78,7 +77,7 @@ def _scalar_map(first, singles, pairs, skip=(32, 33)):
 
 S = _scalar_map(8,
                 singles="LDSB WAVE TILE NTILES GRID L ST T0 T1 T2 T3 NX NH ONE PENDOK BXF MDST G0 NROWS".split(),
-                pairs=("KARG", "WB", "XT", "HT", "MASKS", "RGB", "LSTR", "MSTR", "WP", "HTL", "MKL", "PEND", "XTN", "XTA", "EX", "WQ") + (("TRACE", "TS", "TA") if TRACE else ()))
+                pairs=("KARG", "WB", "XT", "HT", "MASKS", "RGB", "LSTR", "MSTR", "WP", "HTL", "MKL", "PEND", "XTN", "XTA", "EX", "WQ"))
 S_LAST = max(S.values())
 assert S_LAST <= 101, S_LAST
 
@@ -125,28 +124,6 @@ class Body:
         if self.lds:
             self.e("s_waitcnt lgkmcnt(0)")
             self.lds = []
-
-    def trace(self, slot):
-        """experiment builds: wave 0 stores s_memtime to trace[(TILE * 32 + ST) * 8 + slot]"""
-        if not TRACE:
-            return
-        e = self.e
-        skip = self.label("notrace")
-        e(f"s_memtime {s2('TS')}")
-        e(f"s_cmp_eq_u64 {s2('TRACE')}, 0")
-        e(f"s_cbranch_scc1 {skip}")
-        e(f"s_cmp_eq_u32 {s('WAVE')}, 0")
-        e(f"s_cbranch_scc0 {skip}")
-        e(f"s_lshl_b32 {s('TA')}, {s('TILE')}, 5")
-        e(f"s_add_u32 {s('TA')}, {s('TA')}, {s('ST')}")
-        e(f"s_lshl_b32 {s('TA')}, {s('TA')}, 6")
-        e(f"s_add_u32 {s('TA')}, {s('TA')}, {8 * slot}")
-        e(f"s_add_u32 {s('TA')}, {s('TRACE')}, {s('TA')}")
-        e(f"s_addc_u32 {s('TA1')}, {s('TRACE1')}, 0")
-        e("s_waitcnt lgkmcnt(0)")
-        e(f"s_store_dwordx2 {s2('TS')}, {s2('TA')}, 0")
-        e("s_waitcnt lgkmcnt(0)")
-        e(f"{skip}:")
 
     # ------------------------------------------------------------------ registers
     @staticmethod
@@ -396,7 +373,7 @@ class Body:
             self.xt_pointer("T2")
         for q in range(4):
             st = self.store_items(inset, 3, guarded=(kind == "A")) if q == 0 else self.store_items(outset, q - 1, guarded=False)
-            # tools/trace_fwd16.py: the next stage's set-up and DMA ride behind the first MFMAs, at most four scalar / memory
+            # (measured per stage:) the next stage's set-up and DMA ride behind the first MFMAs, at most four scalar / memory
             # instructions per MFMA (a longer run lets the matrix pipe drain), so that the DMA is old when the wait right behind the
             # k-loop asks for it; the eight stores ride between the batches of the epilogue (behind the wait: they have a whole
             # stage until the next one; the texture path takes 40 cycles per contiguous 1-KiB store)
@@ -415,18 +392,13 @@ class Body:
             if kind == "C" and q < 2 and BX_MODE == "kloop":      # behind the DMA groups: nothing else asks for the texture path for a while
                 mixed = mixed + [(len(mixed) + 2 + 2 * k, g) for k, g in enumerate(self.bx_items(q))]
             # the next stage's bias quads are read once this stage's first MFMAs (which take V_BIAS as C) have been issued
-            self.trace(0)
             self.kloop(q & 1, parts, mixed, 1, lds_after=(8, self.bias_reads((q + 1) & 3)))
-            self.trace(1)
             e("s_waitcnt vmcnt(0) lgkmcnt(0)")      # the next stage has landed (this wave's part); nobody reads this buffer any more
-            self.trace(2)
             if not EXP & 16:
                 e("s_barrier")
-            self.trace(3)
             if q < 3:      # the next stage is the next quarter of this layer: its first A quads fly during the epilogue
                 self.first_reads((q + 1) & 1, parts[0][0])
             self.epilogue(q, outset, late)
-            self.trace(4)
             e(f"s_add_u32 {s('ST')}, {s('ST')}, 1")
             e(f"s_and_b32 {s('ST')}, {s('ST')}, 31")
             if kind == "B" and q == 3:
@@ -493,8 +465,6 @@ class Body:
         e = self.e
         for dst, src in (("LDSB", "ldsbase"), ("WAVE", "wave"), ("TILE", "tile0"), ("GRID", "grid")):
             e(f"s_mov_b32 {s(dst)}, %[{src}]")
-        if TRACE:
-            e(f"s_mov_b64 {s2('TRACE')}, %[trace]")
         e(f"s_mov_b64 {s2('KARG')}, %[karg]")
         for dst, off in (("WB", "owb"), ("XT", "oxt"), ("HT", "oht"), ("MASKS", "omasks"), ("RGB", "orgb"), ("LSTR", "olstr"),
                          ("MSTR", "omstr")):
@@ -598,8 +568,6 @@ class Body:
             for x in it:
                 e(x)
         e("s_waitcnt vmcnt(0)")
-        if TRACE:
-            e("s_dcache_wb")
         e(f"{done}:")
         return [x for x in self.L if x is not None]
 
@@ -627,7 +595,7 @@ def main(outdir):
             + [f"s{r}" for r in range(8, S_LAST + 1) if r not in (32, 33)] + ["vcc", "scc", "memory"])
     out = ["// GENERATED by csrc/gen_fwd16_body.py -- do not edit; the generator is the source.", "asm volatile("]
     out += [f'    "{x}\\n\\t"' for x in lines]
-    out.append(OPERANDS.rstrip("\n") + (', [trace] "s"(g_ftrace)' if TRACE else ""))
+    out.append(OPERANDS.rstrip("\n"))
     out.append("      : " + ", ".join(f'"{c}"' for c in clob) + ");")
     with open(os.path.join(outdir, "fwd16_body.inc"), "w") as f:
         f.write("\n".join(out) + "\n")

@@ -332,14 +332,10 @@ __global__ __launch_bounds__(512, 1) void fwd_bf16_kernel(FwdArgs a) {
 // per SIMD, stages by LDS-DMA, every memory instruction behind an MFMA.  Same arithmetic in the same order as fwd_bf16_kernel:
 // images, mask dwords and rgb are bit-identical (tests/test_gpu_parity.py switches between the two with
 // s2l_set_bf16_forward_kernel).  3.04 ms against the C++ kernel's 3.3-3.4 ms for 64 frames of 96x96 (tools/bench_bf16_kernels.py);
-// tools/trace_fwd16.py (experiment build) gives the phases of a stage: k-loop 2 250 cycles (64 MFMAs = 2 048), wait 110, barrier
+// timestamps of an experiment build gave the phases of a stage: k-loop 2 250 cycles (64 MFMAs = 2 048), wait 110, barrier
 // 120, epilogue 1 180 (its eight image stores keep the texture path busy for 1 280), 110 to the next k-loop.
 #ifndef S2L_FWD_ASM
 #define S2L_FWD_ASM 1
-#endif
-#ifdef S2L_EXP_TRACE   // experiment builds (generator run with S2L_FWD_TRACE=1, tools/trace_fwd16.py): per-stage timestamps
-__device__ unsigned long long* g_ftrace = nullptr;
-extern "C" int s2l_debug_set_fwd_trace(void* p) { return (int)hipMemcpyToSymbol(HIP_SYMBOL(g_ftrace), &p, sizeof(p)); }
 #endif
 __global__ __launch_bounds__(256, 1) void fwd_asm_bf16_kernel(FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
