@@ -237,6 +237,29 @@ int s2l_audio_backward(const float* packed, const float* windows, const float* d
 int s2l_mse(const float* pred, const float* target, float weight, float* dpred, float* work,
             float* loss, int64_t n_elems, s2l_stream_t stream);
 
+/* ---- a dense layer of any size (csrc/linear.hip) ----------------------------------------------------------------------------------
+ * z = x W^T + bias,  out = act(z) + residual:  x [rows, in], weight [out, in] (nn.Linear's layout), bias [out] or NULL, residual [rows, out]
+ * or NULL, all of one type (S2L_DTYPE_*).  ld*: row strides in elements; columns are dense; pointers need only their element's alignment.
+ * rows >= 0 (0: nothing to do), in_features, out_features >= 1.  Sums, activation and residual in fp32, one rounding at the store.
+ * `slope`: leaky_relu's factor below zero.  The layers of the reference's networks are this with act = ReLU / LeakyReLU
+ * (tf_nerf.py:105-109, :149-172, :265-283).
+ * saved: NULL, or s2l_linear_saved_bytes(...) bytes that the backward pass reads (relu / leaky_relu: one bit per element, the sign of the fp32
+ * z; gelu (erf form) / silu: z in the call's type; none: nothing).  work: s2l_linear_forward_work_bytes(...) bytes, 16-byte aligned (may be 0
+ * bytes: NULL).
+ * s2l_linear_backward: dy [rows, out] -> dx [rows, in], dweight [out, in] dense, dbias [out]; dx may be NULL, dweight and dbias may be NULL
+ * (dbias only with dweight).  The residual's gradient is dy itself.  rows = 0: dweight = dbias = 0.  Sums are joined in a fixed order. */
+enum { S2L_DTYPE_F32 = 0, S2L_DTYPE_BF16 = 1, S2L_DTYPE_F16 = 2 };
+enum { S2L_ACT_NONE = 0, S2L_ACT_RELU = 1, S2L_ACT_LEAKY_RELU = 2, S2L_ACT_GELU = 3, S2L_ACT_SILU = 4 };
+int64_t s2l_linear_saved_bytes(int dtype, int act, int64_t rows, int64_t out_features);
+int64_t s2l_linear_forward_work_bytes(int dtype, int64_t rows, int64_t in_features, int64_t out_features);
+int64_t s2l_linear_backward_work_bytes(int dtype, int act, int64_t rows, int64_t in_features, int64_t out_features);
+int s2l_linear_forward(int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual,
+                       int64_t ldr, void* out, int64_t ldo, void* saved, void* work, int64_t rows, int64_t in_features,
+                       int64_t out_features, int act, float slope, s2l_stream_t stream);
+int s2l_linear_backward(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                        const void* saved, void* dx, int64_t lddx, void* dweight, void* dbias, void* work, int64_t rows,
+                        int64_t in_features, int64_t out_features, int act, float slope, s2l_stream_t stream);
+
 /* optimizer.step() of the reference's training loop (train.py:173-199 builds torch.optim.Adam; training.py:559-574 steps it after
  * check_weights) for EVERY tensor of a parameter group in ONE launch: torch's _single_tensor_adam arithmetic, operation for operation in
  * fp32 (no amsgrad, no maximize).  table: n_tensors records of four device pointers {param, grad, exp_avg, exp_avg_sq} (32 bytes each, fp32

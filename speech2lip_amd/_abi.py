@@ -14,6 +14,8 @@ S2L_NUM_TENSORS = 42
 S2L_PAD_MAY, S2L_PAD_DEFAULT = 0, 1
 S2L_POSE_OBS2CAN, S2L_POSE_CAN2OBS, S2L_POSE_CAN2OBS_INV = 0, 1, 2
 S2L_SAMPLE_ZEROS, S2L_SAMPLE_BORDER = 0, 1
+S2L_DTYPE_F32, S2L_DTYPE_BF16, S2L_DTYPE_F16 = 0, 1, 2
+S2L_ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "gelu": 3, "silu": 4}
 
 # order of the pointer table of s2l_pack_weights == enum S2L_T_* in include/s2l_hip.h
 TENSOR_ORDER = [
@@ -33,7 +35,7 @@ assert len(TENSOR_ORDER) == S2L_NUM_TENSORS
 
 _ERRORS = {-1: "S2L_E_NULL (null pointer)", -2: "S2L_E_SIZE (bad size)", -3: "S2L_E_ALIGN (pointer not 16-byte aligned)",
            -4: "S2L_E_GEOMETRY (geometry the reference cannot evaluate either, e.g. a lip box entirely outside the face frame)",
-           -5: "S2L_E_UNSUPPORTED (a kernel form only libs2l_hip_ref.so holds)"}
+           -5: "S2L_E_UNSUPPORTED (a kernel form only libs2l_hip_ref.so holds, or an unknown type / activation)"}
 
 EXPORTS = {
     "s2l_version": (c_char_p, []),
@@ -192,6 +194,13 @@ EXPORTS = {
     "s2l_wgrad_bf16": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "s2l_rows_to_tiles_bf16": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "s2l_out_grad_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "s2l_linear_saved_bytes": (c_int64, [c_int, c_int, c_int64, c_int64]),
+    "s2l_linear_forward_work_bytes": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "s2l_linear_backward_work_bytes": (c_int64, [c_int, c_int, c_int64, c_int64, c_int64]),
+    "s2l_linear_forward": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                   c_int64, c_int64, c_int64, c_int, c_float, c_void_p]),
+    "s2l_linear_backward": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                    c_void_p, c_int64, c_int64, c_int64, c_int, c_float, c_void_p]),
     "s2l_to8b": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "s2l_from8b": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }

@@ -15,8 +15,9 @@ The parameters are passed to `apply` as inputs so that the engine delivers their
     unet_train            post_fusion_unet (train mode)     SimpleUnetLight.py:99-111   backward: s2l_unet_train_backward (d input + 32 tensors)
     crop_resize           crop + transforms.Resize          training.py:541-544   backward: s2l_crop_resize_backward
     sync_contrastive_loss get_sync_contrastive_loss         training.py:581-603   backward: s2l_syncnet_face_backward (d window)
+    linear                nn.Linear + activation (any size) tf_nerf.py:105-109, :149-172  backward: s2l_linear_backward
     mse                   add_photometric_loss              training.py:605-619   backward: the gradient s2l_mse returns
-Gradients flow to: the 42 hot-path parameters, the audio columns of `rgb_forward`'s rows, the lip image, the U-Net input, the
+Gradients flow to: the 42 hot-path parameters, everything that `linear` takes, the audio columns of `rgb_forward`'s rows, the lip image, the U-Net input, the
 generated sync window, the prediction of the MSE.  Inputs the reference treats as data (audio windows, pixel coordinates,
 observed frames, warp grids) get none.
 """
@@ -339,3 +340,103 @@ def lpips_distance(module, in0_nhwc, in1_nhwc, from01: bool = False, precision: 
     """lpips.LPIPS(net='alex')(in0, in1) for NHWC images -> [N]; differentiable in in0 (csrc/lpips.hip).  precision: None (the
     module's `conv_precision`), "fp32" or "split" (conv2..conv5 on hi + lo bf16 operands)."""
     return _LpipsDistance.apply(module, in0_nhwc, in1_nhwc, bool(from01), precision)
+
+
+_LINEAR_DTYPES = {torch.float32: _abi.S2L_DTYPE_F32, torch.bfloat16: _abi.S2L_DTYPE_BF16, torch.float16: _abi.S2L_DTYPE_F16}
+
+
+def _dense_rows(t):
+    """`t` [..., n] as rows of dense columns: (tensor [rows, n], row stride).  A view wherever the strides allow it."""
+    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
+    rows, n = t.shape
+    if (n > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < n):
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else n)
+
+
+def _linear_forward(x, weight, bias, residual, act, slope, keep):
+    lib = _abi.load()
+    dt = _LINEAR_DTYPES[x.dtype]
+    dev = x.device
+    out = torch.empty(*x.shape[:-1], weight.shape[0], dtype=x.dtype, device=dev)
+    x2, ldx = _dense_rows(x)
+    w2, ldw = _dense_rows(weight)
+    rows, k, n = x2.shape[0], x2.shape[1], w2.shape[0]
+    res, ldr = _dense_rows(residual) if residual is not None else (None, n)
+    b = bias.contiguous() if bias is not None else None
+    saved = torch.empty(lib.s2l_linear_saved_bytes(dt, act, rows, n), dtype=torch.uint8, device=dev) if keep and act else None
+    need = lib.s2l_linear_forward_work_bytes(dt, rows, k, n)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with torch.cuda.device(dev):
+        _abi.check(lib.s2l_linear_forward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(),
+                                          0 if res is None else res.data_ptr(), ldr, out.data_ptr(), n,
+                                          0 if saved is None else saved.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, act, slope,
+                                          torch.cuda.current_stream().cuda_stream), "s2l_linear_forward")
+    return out, x2, w2, saved
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, slope):
+        keep = any(ctx.needs_input_grad[:3])
+        out, x2, w2, saved = _linear_forward(x, weight, bias, residual, act, slope, keep)
+        need_w = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]      # the bias gradient is a by-product of dW
+        ctx.save_for_backward(x2 if need_w else None, w2 if ctx.needs_input_grad[0] else None, saved)
+        ctx.meta = (act, slope, x.shape, weight.shape)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        act, slope, x_shape, w_shape = ctx.meta
+        x2, w2, saved = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            lib = _abi.load()
+            dt = _LINEAR_DTYPES[dy.dtype]
+            dev = dy.device
+            d2, ldd = _dense_rows(dy)
+            rows, n = d2.shape
+            k = w_shape[1]
+            dx = torch.empty(x_shape, dtype=dy.dtype, device=dev) if need_x else None
+            dw = torch.empty(w_shape, dtype=dy.dtype, device=dev) if need_w or need_b else None
+            db = torch.empty(n, dtype=dy.dtype, device=dev) if need_b else None
+            need = lib.s2l_linear_backward_work_bytes(dt, act, rows, k, n)
+            work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            with torch.cuda.device(dev):
+                _abi.check(lib.s2l_linear_backward(dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(), k if x2 is None or rows < 2 else x2.stride(0),
+                                                   0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
+                                                   0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k,
+                                                   0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
+                                                   0 if work is None else work.data_ptr(), rows, k, n, act, slope,
+                                                   torch.cuda.current_stream().cuda_stream), "s2l_linear_backward")
+        return dx, dw if need_w else None, db, dy if need_r else None, None, None
+
+
+def linear(x, weight, bias=None, residual=None, activation: str = "none", negative_slope: float = 0.02):
+    """act(x W^T + bias) + residual: a dense layer of any size in one launch (csrc/linear.hip), differentiable in x, weight, bias and residual.
+
+    x [..., in], weight [out, in] (nn.Linear's layout), bias [out], residual [..., out] -> [..., out]; all fp32, all bf16 or all fp16, on one GPU.
+    activation: "none", "relu", "leaky_relu" (`negative_slope`; 0.02 is the audio encoder's), "gelu" (erf form) or "silu".  Sums, activation and
+    residual are evaluated in fp32 and rounded once.  The backward pass keeps one bit per output for the kinked activations and the pre-activation
+    for the smooth ones; it can run once (no double backward).  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
+    if activation not in _abi.S2L_ACT:
+        raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")
+    given = [t for t in (x, weight, bias, residual) if t is not None]
+    if not all(isinstance(t, torch.Tensor) for t in given) or x is None or weight is None:
+        raise TypeError("linear: x, weight, bias and residual are tensors")
+    if x.dtype not in _LINEAR_DTYPES or any(t.dtype != x.dtype for t in given):
+        raise ValueError(f"linear: all float32, all bfloat16 or all float16: got {', '.join(str(t.dtype) for t in given)}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear: x [..., in] and weight [out, in] with in, out >= 1: got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"linear: bias must be [{weight.shape[0]}]: got {tuple(bias.shape)}")
+    if residual is not None and (residual.shape[:-1] != x.shape[:-1] or residual.shape[-1:] != weight.shape[:1]):
+        raise ValueError(f"linear: residual must be {tuple(x.shape[:-1]) + (weight.shape[0],)} (it is not broadcast): got {tuple(residual.shape)}")
+    if any(t.device != x.device for t in given) or x.device.type != "cuda":
+        raise _abi.S2LError("linear: every tensor must be on one GPU (no CPU fallback)")
+    act, slope = _abi.S2L_ACT[activation], float(negative_slope)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return _Linear.apply(x, weight, bias, residual, act, slope)
+    return _linear_forward(x, weight, bias, residual, act, slope, False)[0]

@@ -1,0 +1,328 @@
+"""autograd.linear (csrc/linear.hip) against the formula in 64 bits.
+
+Tolerances, derived: u = finfo(type).eps / 2 is one rounding.  A sum of n products in fp32 is within (n + 8) 2^-24 of the sum of their magnitudes
+(8: bias, residual, and a few units in the last place of erf / exp).  A smooth activation's dz is computed from z rounded once (|z act''| <= 0.5
+for gelu and silu) and is itself rounded once; leaky_relu's is rounded once; relu's and none's are exact."""
+import math
+
+import pytest
+import torch
+
+import speech2lip_amd as s2l
+from speech2lip_amd import _abi, autograd
+
+U32 = 2.0 ** -24
+TYPES = (torch.float32, torch.bfloat16, torch.float16)
+SHAPES = [(1, 1, 1), (1, 256, 256), (2, 7, 3), (8, 333, 5), (9, 333, 201), (64, 64, 64), (65, 63, 66), (130, 129, 257), (300, 512, 256), (5000, 40, 24),
+          (33, 5000, 17), (257, 1030, 130), (20000, 129, 8), (4099, 200, 321)]
+ACTS = ("none", "relu", "leaky_relu", "gelu", "silu")
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+def make(rows, k, n, dtype, act, dev, residual=True, bias=True, seed=0):
+    """The kinked activations get multiples of 1/8 up to 1: every z is then exact in fp32 (multiples of 1/64 below 2^18), zeros among them, and so
+    is the side of the kink."""
+    g = torch.Generator(device=dev).manual_seed(seed + rows * 7 + k * 3 + n)
+    if act in ("relu", "leaky_relu"):
+        r = lambda *s: torch.randint(-8, 9, s, generator=g, device=dev).float() / 8  # noqa: E731
+        w = r(n, k)
+    else:
+        r = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+        w = r(n, k) / math.sqrt(k)
+    t = {"x": r(rows, k), "weight": w, "bias": r(n) if bias else None, "residual": torch.randn(rows, n, generator=g, device=dev) if residual else None}
+    t = {a: None if b is None else b.to(dtype).requires_grad_() for a, b in t.items()}
+    return t, torch.randn(rows, n, generator=g, device=dev).to(dtype)
+
+
+def formula(t, dy, act):
+    """(y, dx, dW, db) in 64 bits and, for each, the bound of what the kernels' roundings can add up to."""
+    d = {a: None if b is None else b.detach().double() for a, b in t.items()}
+    x, w, dy = d["x"], d["weight"], dy.double()
+    dtype = t["x"].dtype
+    u = torch.finfo(dtype).eps / 2
+    b = d["bias"] if d["bias"] is not None else torch.zeros(w.shape[0], dtype=torch.float64, device=x.device)
+    r = d["residual"] if d["residual"] is not None else torch.zeros_like(dy)
+    z = x @ w.t() + b
+    phi = 0.5 * (1 + torch.erf(z * math.sqrt(0.5)))
+    sig = torch.sigmoid(z)
+    y, slope = {"none": (z, torch.ones_like(z)), "relu": (z.clamp(min=0), (z > 0).double()),
+                "leaky_relu": (torch.where(z > 0, z, 0.02 * z), torch.where(z > 0, 1.0, 0.02)),
+                "gelu": (z * phi, phi + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)), "silu": (z * sig, sig * (1 + z * (1 - sig)))}[act]
+    y = y + r
+    dz = dy * slope
+    n, k, rows = w.shape[0], w.shape[1], x.shape[0]
+    size = x.abs() @ w.abs().t() + b.abs() + r.abs()
+    out = {"y": (y, u * y.abs() + 1.2 * (k + 8) * U32 * size)}
+    off = torch.zeros_like(dz)
+    if act in ("gelu", "silu"):      # z: its own sum's error too, times |act''| <= 0.8
+        off = (0.5 * u + 8 * U32) * dy.abs() + u * dz.abs() + 0.8 * dy.abs() * (k + 8) * U32 * size
+    elif act == "leaky_relu":
+        off = u * dz.abs()
+    tiny = torch.finfo(dtype).tiny * (0 if dtype == torch.float32 else 2 * u)      # a 16-bit result below the normal range is rounded to its grid
+    for name, v, e, mag, terms in (("x", dz @ w, off @ w.abs(), dz.abs() @ w.abs(), n), ("weight", dz.t() @ x, off.t() @ x.abs(), dz.abs().t() @ x.abs(), rows),
+                                   ("bias", dz.sum(0), off.sum(0), dz.abs().sum(0), rows)):
+        out["d" + name] = (v, u * v.abs() + (1 + u) * (e + (terms + 8) * U32 * mag) + tiny)
+    out["y"] = (out["y"][0], out["y"][1] + tiny)
+    out["dresidual"] = (dy, torch.zeros_like(dy))
+    return out
+
+
+def hold(got, want, what):
+    value, bound = want
+    assert got.shape == value.shape, (what, got.shape, value.shape)
+    far = (got.double() - value).abs() - bound
+    assert bool((far <= 0).all()), (what, float(far.max()), float(((got.double() - value).abs() / bound.clamp_min(1e-300)).max()))
+
+
+def call(t, dy, act, **more):
+    y = autograd.linear(t["x"], t["weight"], t["bias"], residual=t["residual"], activation=act, **more)
+    names = [a for a in ("x", "weight", "bias", "residual") if t[a] is not None]
+    return {"y": y.detach(), **dict(zip(["d" + a for a in names], torch.autograd.grad(y, [t[a] for a in names], dy)))}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_forward_and_gradients_against_the_formula(rows, k, n, dtype, act, dev):
+    full = (rows + k + n) % 2 == 0
+    t, dy = make(rows, k, n, dtype, act, dev, residual=full, bias=full or n % 3 != 0)
+    want = formula(t, dy, act)
+    got = call(t, dy, act)
+    for name, v in got.items():
+        hold(v, want[name], (name, rows, k, n))
+        assert v.dtype == dtype
+    again = call(t, dy, act)      # the same call gives the same bits: sums are joined in a fixed order
+    assert all(torch.equal(got[a], again[a]) for a in got)
+    with torch.no_grad():         # the inference form (few rows: another kernel) keeps nothing and stays within the same bounds
+        hold(autograd.linear(t["x"], t["weight"], t["bias"], residual=t["residual"], activation=act), want["y"], "no_grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_strides_shapes_and_alignment(dev, dtype):
+    """Leading dimensions, rows that are slices of wider rows at odd offsets, transposed and expanded inputs, an expanded output gradient."""
+    for act in ("relu", "silu"):
+        t, _ = make(2 * 3 * 50, 133, 70, dtype, act, dev)
+        base = torch.zeros(300, 140, dtype=dtype, device=dev)
+        base[:, 3:136] = t["x"].detach()
+        wide = torch.zeros(133, 75, dtype=dtype, device=dev)
+        wide[:, 1:71] = t["weight"].detach().t()
+        resw = torch.zeros(300, 81, dtype=dtype, device=dev)
+        resw[:, 7:77] = t["residual"].detach()
+        x = base[:, 3:136].view(2, 3, 50, 133).requires_grad_()
+        w = wide[:, 1:71].t().requires_grad_()          # columns not dense: copied
+        r = resw[:, 7:77].unflatten(0, (2, 3, 50)).requires_grad_()
+        y = autograd.linear(x, w, t["bias"], residual=r, activation=act)
+        assert y.shape == (2, 3, 50, 70) and y.is_contiguous()
+        dy = torch.ones((), dtype=dtype, device=dev).expand(y.shape)
+        want = formula(t, dy.reshape(300, 70), act)
+        gx, gw, gb, gr = torch.autograd.grad(y, (x, w, t["bias"], r), dy)
+        hold(y.detach().reshape(300, 70), want["y"], "y")
+        for got, name in ((gx.reshape(300, 133), "dx"), (gw, "dweight"), (gb, "dbias"), (gr.reshape(300, 70), "dresidual")):
+            hold(got, want[name], name)
+    # weight rows that are slices of wider rows; one vector; a row expanded over the batch (its gradient is the sum over the rows)
+    t, dy = make(40, 64, 48, dtype, "none", dev)
+    wide = torch.zeros(48, 77, dtype=dtype, device=dev)
+    wide[:, 5:69] = t["weight"].detach()
+    w = wide[:, 5:69]
+    want = formula(t, dy, "none")
+    with torch.no_grad():
+        hold(autograd.linear(t["x"], w, t["bias"], residual=t["residual"]), want["y"], "sliced weight")
+        one = autograd.linear(t["x"][0], w, t["bias"], residual=t["residual"][0])
+        assert one.shape == (48,)
+        hold(one, (want["y"][0][0], want["y"][1][0]), "vector")
+    row = t["x"].detach()[:1].clone().requires_grad_()
+    t2 = {**t, "x": row.expand(40, 64)}
+    want = formula(t2, dy, "none")
+    y = autograd.linear(t2["x"], t["weight"], t["bias"], residual=t["residual"])
+    hold(y.detach(), want["y"], "expanded rows")
+    (gx,) = torch.autograd.grad(y, row, dy)
+    value, bound = want["dx"]
+    u = torch.finfo(dtype).eps / 2
+    s = value.sum(0, keepdim=True)
+    hold(gx, (s, bound.sum(0, keepdim=True) + 41 * max(U32, u) * value.abs().sum(0, keepdim=True) + u * s.abs()), "expanded row's gradient")
+
+
+@pytest.mark.gpu
+def test_only_what_is_asked_for(dev):
+    for act in ("none", "relu", "gelu"):
+        t, dy = make(77, 50, 30, torch.float32, act, dev)
+        want = formula(t, dy, act)
+        for names in (("x",), ("weight",), ("bias",), ("residual",), ("x", "bias"), ("weight", "residual")):
+            u = {a: v.detach().requires_grad_(a in names) for a, v in t.items()}
+            y = autograd.linear(u["x"], u["weight"], u["bias"], residual=u["residual"], activation=act)
+            y.backward(dy)
+            for a in u:
+                assert (u[a].grad is not None) == (a in names)
+                if a in names:
+                    hold(u[a].grad, want["d" + a], (a, names, act))
+        with pytest.raises(RuntimeError):      # the backward pass runs once and is not differentiated again
+            y = autograd.linear(t["x"], t["weight"], t["bias"], activation=act)
+            (gx,) = torch.autograd.grad(y.sum(), t["x"], create_graph=True)
+            gx.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_no_rows(dev, dtype):
+    for act in ACTS:
+        t, dy = make(0, 20, 12, dtype, act, dev)
+        got = call(t, dy, act)
+        assert got["y"].shape == (0, 12) and got["dx"].shape == (0, 20)
+        assert bool((got["dweight"] == 0).all()) and bool((got["dbias"] == 0).all())
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(dev):
+    """d loss / d input along a direction, in fp32, against (loss(+h) - loss(-h)) / 2h of the formula in 64 bits: the difference's own error is
+    h^2 / 6 of a third derivative of order one, 1e-8 of the scale at h = 1e-4."""
+    for act in ("none", "gelu", "silu"):
+        t, dy = make(50, 40, 30, torch.float32, act, dev)
+        got = call(t, dy, act)
+        for name in ("x", "weight", "bias", "residual"):
+            g = torch.Generator(device=dev).manual_seed(3)
+            v = torch.randn(t[name].shape, generator=g, device=dev, dtype=torch.float64)
+            loss = []
+            for h in (1e-4, -1e-4):
+                moved = {a: b.detach().double() for a, b in t.items()}
+                moved[name] = moved[name] + h * v
+                z = moved["x"] @ moved["weight"].t() + moved["bias"]
+                y = {"none": z, "gelu": 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5))), "silu": z * torch.sigmoid(z)}[act] + moved["residual"]
+                loss.append((y * dy.double()).sum())
+            slope = float(loss[0] - loss[1]) / 2e-4
+            mine = float((got["d" + name].double() * v).sum())
+            scale = float((got["d" + name].double().abs() * v.abs()).sum())
+            assert abs(mine - slope) <= (1e-6 + 80 * U32) * scale, (act, name, mine, slope)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_values_that_are_not_numbers_stay_in_their_place(dev, dtype):
+    """A NaN or an infinity of one row reaches that row's outputs only, whatever tile it shares; large z saturate the smooth activations cleanly."""
+    for rows in (3, 200):
+        t, _ = make(rows, 70, 40, dtype, "none", dev)
+        x = t["x"].detach().clone()
+        clean = {a: None if b is None else b.detach() for a, b in t.items()}
+        y0 = autograd.linear(clean["x"], clean["weight"], clean["bias"], activation="relu")
+        x[1, 7], x[2, 69] = float("nan"), float("inf")
+        y = autograd.linear(x, clean["weight"], clean["bias"], activation="relu")
+        assert bool(torch.isnan(y[1]).all())
+        assert bool(((y[2] == float("inf")) == (clean["weight"][:, 69] > 0)).all()) and bool((y[2][clean["weight"][:, 69] < 0] == 0).all())
+        keep = [i for i in range(rows) if i not in (1, 2)]
+        assert torch.equal(y[keep], y0[keep])
+    big = torch.tensor([[-3e4, 3e4], [-200.0, 200.0]], device=dev).to(dtype).requires_grad_()
+    w = torch.tensor([[8.0, 0.0], [0.0, 8.0]], device=dev).to(dtype).requires_grad_()      # z = -+2.4e5: beyond float16
+    for act in ("gelu", "silu"):
+        y = autograd.linear(big, w, activation=act)
+        gx, gw = torch.autograd.grad(y, (big, w), torch.ones_like(y))
+        assert bool((gx[:, 0] == 0).all()) and bool((gx[:, 1] == 8).all()) and bool(torch.isfinite(gw).all())
+        assert bool((y[:, 0].abs() == 0).all())
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_one_are_left_alone(dev):
+    """Through the C entry: a guard band around every output keeps its bytes."""
+    lib = _abi.load()
+    for dt, dtype in ((0, torch.float32), (1, torch.bfloat16), (2, torch.float16)):
+        for rows, k, n in ((5, 33, 17), (130, 129, 257), (700, 64, 65)):
+            t, dy = make(rows, k, n, dtype, "silu", dev)
+            d = {a: b.detach() for a, b in t.items()}
+            size = d["x"].element_size()
+            ldo = n + 5
+            out = torch.full((rows + 2, ldo), 7.0, dtype=dtype, device=dev)
+            saved = torch.full((lib.s2l_linear_saved_bytes(dt, 4, rows, n) + 64,), 85, dtype=torch.uint8, device=dev)
+            work = torch.full((lib.s2l_linear_forward_work_bytes(dt, rows, k, n) + 64,), 85, dtype=torch.uint8, device=dev)
+            s = torch.cuda.current_stream().cuda_stream
+            _abi.check(lib.s2l_linear_forward(dt, d["x"].data_ptr(), k, d["weight"].data_ptr(), k, d["bias"].data_ptr(), d["residual"].data_ptr(), n,
+                                              out.data_ptr() + (ldo + 2) * size, ldo, saved.data_ptr(), work.data_ptr(), rows, k, n, 4, 0.0, s), "forward")
+            dx = torch.full((rows + 2, k + 3), 7.0, dtype=dtype, device=dev)
+            dw = torch.full((n + 2, k), 7.0, dtype=dtype, device=dev)
+            db = torch.full((n + 2,), 7.0, dtype=dtype, device=dev)
+            bwork = torch.full((lib.s2l_linear_backward_work_bytes(dt, 4, rows, k, n) + 64,), 85, dtype=torch.uint8, device=dev)
+            _abi.check(lib.s2l_linear_backward(dt, dy.data_ptr(), n, d["x"].data_ptr(), k, d["weight"].data_ptr(), k, saved.data_ptr(),
+                                               dx.data_ptr() + (k + 3) * size, k + 3, dw.data_ptr() + k * size, db.data_ptr() + size, bwork.data_ptr(),
+                                               rows, k, n, 4, 0.0, s), "backward")
+            torch.cuda.synchronize()
+            want = formula(t, dy, "silu")
+            hold(out[1:-1, 2:2 + n], want["y"], "y")
+            hold(dx[1:-1, :k], want["dx"], "dx")
+            hold(dw[1:-1], want["dweight"], "dw")
+            hold(db[1:-1], want["dbias"], "db")
+            out[1:-1, 2:2 + n], dx[1:-1, :k], dw[1:-1], db[1:-1] = 7, 7, 7, 7
+            assert all(bool((v == 7).all()) for v in (out, dx, dw, db))
+            assert all(bool((v[-64:] == 85).all()) for v in (saved, work, bwork))
+
+
+@pytest.mark.gpu
+def test_another_stream_and_a_captured_graph(dev):
+    """On a side stream, and captured with its backward pass and replayed on new values: the bits of the eager call."""
+    for dtype, act, shape in ((torch.bfloat16, "relu", (5000, 96, 72)), (torch.float32, "gelu", (3, 256, 256)), (torch.float16, "silu", (33, 5000, 17))):
+        t, dy = make(*shape, dtype, act, dev)
+        want = call(t, dy, act)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = call(t, dy, act)
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(want[a], got[a]) for a in want)
+        static = {a: b.detach().clone().requires_grad_() for a, b in t.items()}
+        sdy = dy.clone()
+        with torch.cuda.stream(side):
+            call(static, sdy, act)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(static, sdy, act)
+        for seed in (1, 2, 3):
+            fresh, fdy = make(*shape, dtype, act, dev, seed=seed)
+            with torch.no_grad():
+                for a in static:
+                    static[a].copy_(fresh[a])
+                sdy.copy_(fdy)
+            graph.replay()
+            torch.cuda.synchronize()
+            eager = call(fresh, fdy, act)
+            assert all(torch.equal(eager[a], out[a]) for a in eager), (dtype, act, seed)
+
+
+def test_refusals_need_no_gpu():
+    z = torch.zeros
+    with pytest.raises(_abi.S2LError):
+        autograd.linear(z(2, 3), z(4, 3))                                  # no CPU path
+    for bad in (dict(x=z(2, 3), weight=z(4, 2)), dict(x=z(2, 3), weight=z(4, 3, 1)), dict(x=z(()), weight=z(4, 3)), dict(x=z(2, 3), weight=z(0, 3)),
+                dict(x=z(2, 0), weight=z(4, 0)), dict(x=z(2, 3), weight=z(4, 3), bias=z(3)), dict(x=z(2, 3), weight=z(4, 3), bias=z(1, 4)),
+                dict(x=z(2, 3), weight=z(4, 3), residual=z(4)), dict(x=z(2, 3), weight=z(4, 3), residual=z(1, 4)),
+                dict(x=z(2, 3), weight=z(4, 3).bfloat16()), dict(x=z(2, 3).double(), weight=z(4, 3).double()), dict(x=z(2, 3), weight=z(4, 3), activation="tanh")):
+        with pytest.raises(ValueError):
+            autograd.linear(**bad)
+    with pytest.raises(TypeError):
+        autograd.linear([1.0], z(4, 1))
+
+
+def test_c_entry_refusals_need_no_gpu():
+    lib = _abi.load()
+    p, odd = 4096, 4097
+    fwd = lambda dt=0, x=p, ldx=8, w=p, ldw=8, b=p, r=p, ldr=6, o=p, ldo=6, saved=0, work=p, rows=3, k=8, n=6, act=1: lib.s2l_linear_forward(  # noqa: E731
+        dt, x, ldx, w, ldw, b, r, ldr, o, ldo, saved, work, rows, k, n, act, 0.0, 0)
+    assert fwd(rows=0, x=0, w=0, o=0) == 0                                 # nothing to do
+    assert fwd(dt=3) == -5 and fwd(act=5) == -5 and fwd(act=-1) == -5
+    assert fwd(rows=-1) == -2 and fwd(k=0) == -2 and fwd(n=0) == -2 and fwd(rows=1 << 31) == -2
+    assert fwd(x=0) == -1 and fwd(w=0) == -1 and fwd(o=0) == -1
+    assert fwd(ldx=7) == -2 and fwd(ldw=7) == -2 and fwd(ldo=5) == -2 and fwd(ldr=5) == -2
+    assert fwd(x=odd) == -3 and fwd(dt=1, w=odd) == -3 and fwd(b=p + 2) == -3 and fwd(work=p + 8) == -3
+    assert lib.s2l_linear_forward_work_bytes(0, 33, 5000, 17) > 0 and fwd(rows=33, k=5000, n=17, ldx=5000, ldw=5000, ldr=17, ldo=17, work=0) == -1
+    bwd = lambda dt=0, dy=p, lddy=6, x=p, ldx=8, w=p, ldw=8, saved=p, dx=p, lddx=8, dw=p, db=p, work=p, rows=3, k=8, n=6, act=1: lib.s2l_linear_backward(  # noqa: E731
+        dt, dy, lddy, x, ldx, w, ldw, saved, dx, lddx, dw, db, work, rows, k, n, act, 0.0, 0)
+    assert bwd(dx=0, dw=0, db=0) == 0
+    assert bwd(dw=0) == -1 and bwd(dy=0) == -1 and bwd(saved=0) == -1 and bwd(x=0) == -1 and bwd(w=0) == -1 and bwd(work=0) == -1
+    assert bwd(dt=7) == -5 and bwd(act=9) == -5 and bwd(rows=-1) == -2 and bwd(lddy=5) == -2 and bwd(lddx=7) == -2 and bwd(ldx=7) == -2 and bwd(ldw=7) == -2
+    assert bwd(dy=odd) == -3 and bwd(work=p + 4) == -3 and bwd(act=3, saved=p + 1) == -3
+    for act in range(5):      # no rows: sizes are asked for all the same
+        assert lib.s2l_linear_forward_work_bytes(0, 0, 20, 12) == 0 and lib.s2l_linear_backward_work_bytes(0, act, 0, 20, 12) == 256
+    assert lib.s2l_linear_saved_bytes(0, 1, 10, 17) == 30 and lib.s2l_linear_saved_bytes(1, 4, 10, 17) == 340 and lib.s2l_linear_saved_bytes(1, 0, 10, 17) == 0
