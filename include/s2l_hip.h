@@ -237,6 +237,28 @@ int s2l_audio_backward(const float* packed, const float* windows, const float* d
 int s2l_mse(const float* pred, const float* target, float weight, float* dpred, float* work,
             float* loss, int64_t n_elems, s2l_stream_t stream);
 
+/* ---- Newton-Schulz orthogonalisation and the Muon step (csrc/orthogonalize.hip) --------------------------------------------------
+ * X0 = G / max(||G||_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T of the shorter side: every matrix of the set in the
+ * same launches.  matrices_host: HOST array of `count` records, read before the call returns; in / out [rows, cols] dense, element-aligned,
+ * rows, cols in 1 .. 131072.  out may be in.  A matrix that holds a NaN or an infinity comes out all NaN; a zero matrix zero.  The iteration's
+ * values are scaled halves (fp32: hi + lo pairs): coefficients whose polynomial would let a singular value grow past 4 before the last step are
+ * refused (S2L_E_SIZE).  work: s2l_orthogonalize_work_bytes(...) bytes, 16-byte aligned, clean or not; a size depends on rows and cols alone.
+ * s2l_muon_step, fp32: in = gradient, momentum = its running mean m, out = the parameter p, step = its learning rate:
+ *   m <- m + (1 - momentum) (g - m),  u = nesterov ? g + momentum (m - g) : m,  p <- shrink p - step X_steps(u).
+ * nan_flags: NULL or count ints, set to 1 (never cleared) where the parameter as read holds a NaN. */
+typedef struct {
+  const void* in;
+  void* out;
+  float* momentum;
+  int rows, cols;
+  float step;
+} s2l_matrix;
+int64_t s2l_orthogonalize_work_bytes(const s2l_matrix* matrices_host, int64_t count);
+int s2l_orthogonalize(int dtype, const s2l_matrix* matrices_host, int64_t count, double a, double b, double c, float eps, int steps,
+                      void* work, s2l_stream_t stream);
+int s2l_muon_step(const s2l_matrix* matrices_host, int64_t count, float momentum, int nesterov, float shrink, double a, double b, double c,
+                  float eps, int steps, int* nan_flags, void* work, s2l_stream_t stream);
+
 /* ---- a dense layer of any size (csrc/linear.hip) ----------------------------------------------------------------------------------
  * z = x W^T + bias,  out = act(z) + residual:  x [rows, in], weight [out, in] (nn.Linear's layout), bias [out] or NULL, residual [rows, out]
  * or NULL, all of one type (S2L_DTYPE_*).  ld*: row strides in elements; columns are dense; pointers need only their element's alignment.
@@ -244,14 +266,14 @@ int s2l_mse(const float* pred, const float* target, float weight, float* dpred, 
  * `slope`: leaky_relu's factor below zero.  The layers of the reference's networks are this with act = ReLU / LeakyReLU
  * (tf_nerf.py:105-109, :149-172, :265-283).
  * saved: NULL, or s2l_linear_saved_bytes(...) bytes that the backward pass reads (relu / leaky_relu: one bit per element, the sign of the fp32
- * z; gelu (erf form) / silu: z in the call's type; none: nothing).  work: s2l_linear_forward_work_bytes(...) bytes, 16-byte aligned (may be 0
- * bytes: NULL).
+ * z; gelu (erf form) / silu: z in the call's type; none: nothing).  work: s2l_linear_forward_work_bytes(..., keep = whether saved is given, ...)
+ * bytes, 16-byte aligned (may be 0 bytes: NULL).
  * s2l_linear_backward: dy [rows, out] -> dx [rows, in], dweight [out, in] dense, dbias [out]; dx may be NULL, dweight and dbias may be NULL
  * (dbias only with dweight).  The residual's gradient is dy itself.  rows = 0: dweight = dbias = 0.  Sums are joined in a fixed order. */
 enum { S2L_DTYPE_F32 = 0, S2L_DTYPE_BF16 = 1, S2L_DTYPE_F16 = 2 };
 enum { S2L_ACT_NONE = 0, S2L_ACT_RELU = 1, S2L_ACT_LEAKY_RELU = 2, S2L_ACT_GELU = 3, S2L_ACT_SILU = 4 };
 int64_t s2l_linear_saved_bytes(int dtype, int act, int64_t rows, int64_t out_features);
-int64_t s2l_linear_forward_work_bytes(int dtype, int64_t rows, int64_t in_features, int64_t out_features);
+int64_t s2l_linear_forward_work_bytes(int dtype, int act, int keep, int64_t rows, int64_t in_features, int64_t out_features);
 int64_t s2l_linear_backward_work_bytes(int dtype, int act, int64_t rows, int64_t in_features, int64_t out_features);
 int s2l_linear_forward(int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual,
                        int64_t ldr, void* out, int64_t ldo, void* saved, void* work, int64_t rows, int64_t in_features,

@@ -15,6 +15,7 @@ S2L_PAD_MAY, S2L_PAD_DEFAULT = 0, 1
 S2L_POSE_OBS2CAN, S2L_POSE_CAN2OBS, S2L_POSE_CAN2OBS_INV = 0, 1, 2
 S2L_SAMPLE_ZEROS, S2L_SAMPLE_BORDER = 0, 1
 S2L_DTYPE_F32, S2L_DTYPE_BF16, S2L_DTYPE_F16 = 0, 1, 2
+S2L_MATRIX_WORDS = 5      # int64 words of an s2l_matrix record: in, out, momentum, rows | cols << 32, step (float bits)
 S2L_ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "gelu": 3, "silu": 4}
 
 # order of the pointer table of s2l_pack_weights == enum S2L_T_* in include/s2l_hip.h
@@ -194,8 +195,11 @@ EXPORTS = {
     "s2l_wgrad_bf16": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "s2l_rows_to_tiles_bf16": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "s2l_out_grad_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "s2l_orthogonalize_work_bytes": (c_int64, [c_void_p, c_int64]),
+    "s2l_orthogonalize": (c_int, [c_int, c_void_p, c_int64, c_double, c_double, c_double, c_float, c_int, c_void_p, c_void_p]),
+    "s2l_muon_step": (c_int, [c_void_p, c_int64, c_float, c_int, c_float, c_double, c_double, c_double, c_float, c_int, c_void_p, c_void_p, c_void_p]),
     "s2l_linear_saved_bytes": (c_int64, [c_int, c_int, c_int64, c_int64]),
-    "s2l_linear_forward_work_bytes": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "s2l_linear_forward_work_bytes": (c_int64, [c_int, c_int, c_int, c_int64, c_int64, c_int64]),
     "s2l_linear_backward_work_bytes": (c_int64, [c_int, c_int, c_int64, c_int64, c_int64]),
     "s2l_linear_forward": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                    c_int64, c_int64, c_int64, c_int, c_float, c_void_p]),

@@ -354,24 +354,31 @@ def _dense_rows(t):
     return t, (t.stride(0) if rows > 1 else n)
 
 
+def _on_device(index, fn, *args):
+    """fn(*args, raw current stream of device `index`), with that device current.  (The context manager and the stream object cost 4 us a call;
+    one layer of one sample is 10.)"""
+    if torch.cuda.current_device() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def _linear_forward(x, weight, bias, residual, act, slope, keep):
     lib = _abi.load()
     dt = _LINEAR_DTYPES[x.dtype]
-    dev = x.device
-    out = torch.empty(*x.shape[:-1], weight.shape[0], dtype=x.dtype, device=dev)
     x2, ldx = _dense_rows(x)
     w2, ldw = _dense_rows(weight)
-    rows, k, n = x2.shape[0], x2.shape[1], w2.shape[0]
+    (rows, k), n = x2.shape, w2.shape[0]
+    out = x.new_empty((*x.shape[:-1], n))
     res, ldr = _dense_rows(residual) if residual is not None else (None, n)
     b = bias.contiguous() if bias is not None else None
-    saved = torch.empty(lib.s2l_linear_saved_bytes(dt, act, rows, n), dtype=torch.uint8, device=dev) if keep and act else None
-    need = lib.s2l_linear_forward_work_bytes(dt, rows, k, n)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
-        _abi.check(lib.s2l_linear_forward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(),
-                                          0 if res is None else res.data_ptr(), ldr, out.data_ptr(), n,
-                                          0 if saved is None else saved.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, act, slope,
-                                          torch.cuda.current_stream().cuda_stream), "s2l_linear_forward")
+    saved = torch.empty(lib.s2l_linear_saved_bytes(dt, act, rows, n), dtype=torch.uint8, device=x.device) if keep and act else None
+    need = lib.s2l_linear_forward_work_bytes(dt, act, saved is not None, rows, k, n)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    rc = _on_device(x.get_device(), lib.s2l_linear_forward, dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(),
+                    0 if res is None else res.data_ptr(), ldr, out.data_ptr(), n, 0 if saved is None else saved.data_ptr(),
+                    0 if work is None else work.data_ptr(), rows, k, n, act, slope)
+    _abi.check(rc, "s2l_linear_forward")
     return out, x2, w2, saved
 
 
@@ -395,22 +402,19 @@ class _Linear(torch.autograd.Function):
         if need_x or need_w or need_b:
             lib = _abi.load()
             dt = _LINEAR_DTYPES[dy.dtype]
-            dev = dy.device
             d2, ldd = _dense_rows(dy)
             rows, n = d2.shape
             k = w_shape[1]
-            dx = torch.empty(x_shape, dtype=dy.dtype, device=dev) if need_x else None
-            dw = torch.empty(w_shape, dtype=dy.dtype, device=dev) if need_w or need_b else None
-            db = torch.empty(n, dtype=dy.dtype, device=dev) if need_b else None
+            dx = dy.new_empty(x_shape) if need_x else None
+            dw = dy.new_empty(w_shape) if need_w or need_b else None
+            db = dy.new_empty(n) if need_b else None
             need = lib.s2l_linear_backward_work_bytes(dt, act, rows, k, n)
-            work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            with torch.cuda.device(dev):
-                _abi.check(lib.s2l_linear_backward(dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(), k if x2 is None or rows < 2 else x2.stride(0),
-                                                   0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
-                                                   0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k,
-                                                   0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
-                                                   0 if work is None else work.data_ptr(), rows, k, n, act, slope,
-                                                   torch.cuda.current_stream().cuda_stream), "s2l_linear_backward")
+            work = torch.empty(need, dtype=torch.uint8, device=dy.device)
+            rc = _on_device(dy.get_device(), lib.s2l_linear_backward, dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(),
+                            k if x2 is None or rows < 2 else x2.stride(0), 0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
+                            0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k, 0 if dw is None else dw.data_ptr(),
+                            0 if db is None else db.data_ptr(), work.data_ptr(), rows, k, n, act, slope)
+            _abi.check(rc, "s2l_linear_backward")
         return dx, dw if need_w else None, db, dy if need_r else None, None, None
 
 
@@ -424,18 +428,23 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     if activation not in _abi.S2L_ACT:
         raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")
     given = [t for t in (x, weight, bias, residual) if t is not None]
-    if not all(isinstance(t, torch.Tensor) for t in given) or x is None or weight is None:
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor) or not all(isinstance(t, torch.Tensor) for t in given):
         raise TypeError("linear: x, weight, bias and residual are tensors")
-    if x.dtype not in _LINEAR_DTYPES or any(t.dtype != x.dtype for t in given):
-        raise ValueError(f"linear: all float32, all bfloat16 or all float16: got {', '.join(str(t.dtype) for t in given)}")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"linear: x [..., in] and weight [out, in] with in, out >= 1: got {tuple(x.shape)} and {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"linear: bias must be [{weight.shape[0]}]: got {tuple(bias.shape)}")
-    if residual is not None and (residual.shape[:-1] != x.shape[:-1] or residual.shape[-1:] != weight.shape[:1]):
-        raise ValueError(f"linear: residual must be {tuple(x.shape[:-1]) + (weight.shape[0],)} (it is not broadcast): got {tuple(residual.shape)}")
-    if any(t.device != x.device for t in given) or x.device.type != "cuda":
-        raise _abi.S2LError("linear: every tensor must be on one GPU (no CPU fallback)")
+    dtype, dev, w_shape, x_shape = x.dtype, x.device, weight.shape, x.shape
+    if dtype not in _LINEAR_DTYPES:
+        raise ValueError(f"linear: float32, bfloat16 or float16: got {dtype}")
+    if len(x_shape) < 1 or len(w_shape) != 2 or x_shape[-1] != w_shape[1] or w_shape[0] < 1 or w_shape[1] < 1:
+        raise ValueError(f"linear: x [..., in] and weight [out, in] with in, out >= 1: got {tuple(x_shape)} and {tuple(w_shape)}")
+    if bias is not None and bias.shape != w_shape[:1]:
+        raise ValueError(f"linear: bias must be [{w_shape[0]}]: got {tuple(bias.shape)}")
+    if residual is not None and (residual.shape[:-1] != x_shape[:-1] or residual.shape[-1:] != w_shape[:1]):
+        raise ValueError(f"linear: residual must be {tuple(x_shape[:-1]) + (w_shape[0],)} (it is not broadcast): got {tuple(residual.shape)}")
+    for t in given:
+        if t.dtype != dtype:
+            raise ValueError(f"linear: every tensor in one type: got {dtype} and {t.dtype}")
+    for t in given:
+        if t.device != dev or not t.is_cuda:
+            raise _abi.S2LError("linear: every tensor must be on one GPU (no CPU fallback)")
     act, slope = _abi.S2L_ACT[activation], float(negative_slope)
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return _Linear.apply(x, weight, bias, residual, act, slope)

@@ -579,8 +579,11 @@ template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, flo
   return (int)hipGetLastError();
 }
 
+// few rows, unless sign bits are wanted: a lane there has one column, a byte of them is eight
+inline bool skinny(int64_t rows, bool bits) { return rows <= kSkinnyRows && !bits; }
+
 template <typename T> int forward(Args g, float* work, hipStream_t st) {
-  if (g.m <= kSkinnyRows && !g.bits) {
+  if (skinny(g.m, g.bits != nullptr)) {
     const dim3 grid((unsigned)ceil_div(g.n, 4));
     if (g.m == 1) hipLaunchKernelGGL((skinny_kernel<T, 1>), grid, dim3(kThreads), 0, st, g);
     else if (g.m <= 4) hipLaunchKernelGGL((skinny_kernel<T, 4>), grid, dim3(kThreads), 0, st, g);
@@ -681,9 +684,9 @@ extern "C" int64_t s2l_linear_saved_bytes(int dtype, int act, int64_t rows, int6
   return 0;
 }
 
-extern "C" int64_t s2l_linear_forward_work_bytes(int dtype, int64_t rows, int64_t in_features, int64_t out_features) {
+extern "C" int64_t s2l_linear_forward_work_bytes(int dtype, int act, int keep, int64_t rows, int64_t in_features, int64_t out_features) {
   using namespace s2l::lin;
-  if (!size_of(dtype) || bad_dims(rows, in_features, out_features)) return 0;
+  if (!size_of(dtype) || bad_dims(rows, in_features, out_features) || skinny(rows, keep && (act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU))) return 0;
   return partial_bytes(plan_of(rows, out_features, in_features, size_of(dtype)), rows, out_features);
 }
 
@@ -703,7 +706,7 @@ extern "C" int s2l_linear_forward(int dtype, const void* x, int64_t ldx, const v
   if (rows == 0) return S2L_OK;
   if (!x || !weight || !out) return S2L_E_NULL;
   if ((rows > 1 && (ldx < in_features || ldo < out_features || (residual && ldr < out_features))) || (out_features > 1 && ldw < in_features)) return S2L_E_SIZE;
-  const int64_t need = s2l_linear_forward_work_bytes(dtype, rows, in_features, out_features);
+  const int64_t need = s2l_linear_forward_work_bytes(dtype, act, saved != nullptr, rows, in_features, out_features);
   if (need && !work) return S2L_E_NULL;
   if (off(x, size) || off(weight, size) || off(bias, size) || off(residual, size) || off(out, size) || off(work, 16)) return S2L_E_ALIGN;
   const bool kinked = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU, smooth = act == S2L_ACT_GELU || act == S2L_ACT_SILU;

@@ -1,0 +1,588 @@
+// Newton-Schulz orthogonalisation of a set of matrices, and the optimiser step that is built on it.
+//
+//   X0 = G / max(||G||_F, eps);   `steps` times:  A = X X^T,  B = a I + b A + c A A,  X <- B X      (X: the shorter side first)
+//   Muon:  m <- m + (1 - mu) (g - m),  u = g + mu (m - g)  (or m),  p <- (1 - lr wd) p - lr_p X_steps(u)
+//
+// Every singular value s of X0 becomes p(p(...s)) with p(s) = a s + b s^3 + c s^5; with the usual (3.4445, -4.7750, 2.0315) and five steps all but
+// the smallest end in 0.7 .. 1.2: U V^T but for that band.  p amplifies small singular values by a = 3.44 a step (485 over five), and with them
+// whatever rounding put into their directions, so the products' precision goes by the STEP, not by the type alone: X, A and B are held as two
+// IEEE halves (hi = f16(x), lo = f16(x - hi): 22 significant bits) and a product is three f16 MFMAs, hi hi + hi lo + lo hi, summed in fp32 --
+// fp32's own accuracy at 2.7 times the fp32 MFMA's peak -- in every step for fp32 input, and in all but the last two steps for bf16 / f16 input,
+// whose last two run on hi alone (their roundings of 2^-12 are amplified at most 12-fold; one product in every step would leave 2-4 % of error on
+// matrices of fast falling spectrum, and bf16 products 15-30 %).
+// Values are scaled by 2^11: |X| <= ||X||_2 <= 1.2 and the entries of A and B <= 3.5 use the range of the halves from 2^-24 to 7168.
+//
+// All matrices of a call go through the same 2 + 3 * steps launches: one pass for the Frobenius norms (with the momentum update), one that scales
+// and splits into X and X^T, then per step the Gram product (symmetric: tiles on and below the diagonal, written twice), the polynomial (the
+// same, its epilogue adds a I + b A), and X <- B X, which leaves X and X^T for the next step's two products -- both operands of every product
+// are then contiguous in k -- or, last, writes the result: the rounded output, or the parameter's update.  Matrices lie zero-padded to multiples
+// of 64 in the workspace, so that the products' main loop has no edges.
+#include <cmath>
+
+#include "tile_core.h"
+
+namespace s2l {
+namespace ns {
+
+using core::f16v;
+using core::u4;
+
+constexpr int kPad = 64;
+constexpr int kMaxMatrices = 56;            // of one set of launches: the table crosses as a kernel argument (below 4 KiB)
+constexpr int kMaxPartials = 1024;          // partial sums of squares of a matrix
+constexpr float kScale = 2048.f;
+constexpr int kThreads = 256;
+
+struct Mat {
+  const void* in;       // [rows][cols] dense: the update, or (Muon) the gradient
+  void* out;            // the result, or (Muon) the parameter
+  float* momentum;      // Muon
+  int64_t base;         // byte offset of this matrix's arrays in the workspace
+  int rows, cols;
+  float step;           // Muon: lr_p
+  int stat, pack, sym, rect;      // first workgroup of each kind of launch
+};
+
+struct Table {
+  int count;
+  int stat_blocks, pack_blocks, sym_tiles, rect_tiles;
+  Mat mat[kMaxMatrices];
+};
+static_assert(sizeof(Table) <= 3840, "the table and a few scalars share the 4 KiB of kernel arguments");
+
+__host__ __device__ inline int padded(int v) { return (v + kPad - 1) / kPad * kPad; }
+__host__ __device__ inline int64_t elements_of(const Mat& t) { return (int64_t)t.rows * t.cols; }
+__host__ __device__ inline int64_t chunk_of(int64_t elements) {      // elements of one workgroup of the first pass: a multiple of its 2048
+  const int64_t c = (elements + kMaxPartials - 1) / kMaxPartials;
+  return c <= 4096 ? 4096 : (c + 2047) / 2048 * 2048;
+}
+
+// the arrays of one matrix, in halves from its base; `part` = distance of the lo array from the hi one
+struct Arrays {
+  int m, n, mp, np;
+  int64_t x, xt[2], a, b, total;
+};
+__host__ __device__ inline Arrays arrays_of(int rows, int cols) {
+  Arrays r;
+  r.m = rows < cols ? rows : cols;
+  r.n = rows < cols ? cols : rows;
+  r.mp = padded(r.m);
+  r.np = padded(r.n);
+  const int64_t mn = (int64_t)r.mp * r.np, mm = (int64_t)r.mp * r.mp;
+  r.x = 0;
+  r.xt[0] = 2 * mn;
+  r.xt[1] = 4 * mn;
+  r.a = 6 * mn;
+  r.b = r.a + 2 * mm;
+  r.total = r.b + 2 * mm;
+  return r;
+}
+
+constexpr int64_t kTableBytes = 4096;
+constexpr int64_t partial_bytes(int stat_blocks) { return ((int64_t)stat_blocks * 8 + 255) / 256 * 256; }
+
+// which matrix workgroup `id` of a launch belongs to: every lane compares one first workgroup
+__device__ __forceinline__ int owner(const Table* t, int id, int Mat::*first) {
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < t->count ? t->mat[lane].*first : 0x7fffffff;
+  return __popcll(__ballot(mine <= id)) - 1;
+}
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, float* v) {
+  if (left >= 8) {
+    T t[8];
+    __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void store8f(float* p, int64_t left, const float* v) {
+  if (left >= 8) {
+    __builtin_memcpy(p, v, 32);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = v[i];
+  }
+}
+
+struct Momentum {
+  float mu;
+  int nesterov;
+};
+
+// ---- first pass: the sums of squares in 64 bits (every later product scales with the norm: a sum over millions of squares in 32 bits is off by
+// more than all other roundings together), with the momentum update.  Memory bound: reads g, reads and writes m.
+template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, char* work, Momentum mo) {
+  __shared__ double part[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x == 0) {      // the table for the launches that follow
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(&t);
+    for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += kThreads) reinterpret_cast<uint32_t*>(work)[i] = src[i];
+  }
+  int k = 0;
+  while (k + 1 < t.count && t.mat[k + 1].stat <= (int)blockIdx.x) ++k;
+  const Mat& mat = t.mat[k];
+  const int64_t total = elements_of(mat), chunk = chunk_of(total);
+  const int64_t begin = (int64_t)(blockIdx.x - mat.stat) * chunk, end = begin + chunk < total ? begin + chunk : total;
+  const T* g = static_cast<const T*>(mat.in);
+  double sum = 0.0;
+#pragma unroll 2
+  for (int64_t i = begin + threadIdx.x * 8; i < end; i += kThreads * 8) {
+    float v[8];
+    load8(g + i, end - i, v);
+    if constexpr (MUON) {
+      float m[8];
+      load8(mat.momentum + i, end - i, m);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = fmaf(1.f - mo.mu, v[e] - m[e], m[e]);
+        v[e] = mo.nesterov ? fmaf(mo.mu, m[e] - v[e], v[e]) : m[e];
+      }
+      store8f(mat.momentum + i, end - i, m);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fma((double)v[e], (double)v[e], sum);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) reinterpret_cast<double*>(work + kTableBytes)[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__device__ __forceinline__ uint32_t halves(float v) {      // hi | lo << 16
+  const _Float16 hi = (_Float16)v;
+  const _Float16 lo = (_Float16)(v - (float)hi);
+  return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
+}
+
+// eight neighbouring values (hi | lo << 16 each) to the hi array and, parts == 2, the lo array
+__device__ __forceinline__ void put8(_Float16* hi, int64_t part, int parts, const uint32_t* w) {
+  u4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (w[2 * e] & 0xffffu) | w[2 * e + 1] << 16;
+  *reinterpret_cast<u4*>(hi) = v;
+  if (parts == 2) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = w[2 * e] >> 16 | (w[2 * e + 1] & 0xffff0000u);
+    *reinterpret_cast<u4*>(hi + part) = v;
+  }
+}
+
+// ---- second pass: X and X^T = 2^11 u / max(norm, eps), split into halves, zero-padded.  A workgroup: 64 x 64 of the padded matrix as it lies.
+template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void split_kernel(char* work, Momentum mo, float eps, int parts) {
+  __shared__ uint32_t tile[64][65];
+  __shared__ double part[4];
+  const Table* t = reinterpret_cast<const Table*>(work);
+  const int k = owner(t, blockIdx.x, &Mat::pack);
+  const Mat mat = t->mat[k];
+  const Arrays r = arrays_of(mat.rows, mat.cols);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const double* partial = reinterpret_cast<const double*>(work + kTableBytes) + mat.stat;
+  const int64_t total = elements_of(mat), chunk = chunk_of(total);
+  const int partials = (int)((total + chunk - 1) / chunk);
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  const double norm = sqrt((part[0] + part[1]) + (part[2] + part[3]));
+  const double scale = (double)kScale / (norm < (double)eps ? (double)eps : norm);      // (a NaN norm stays one)
+
+  const int tiles_c = padded(mat.cols) / 64, id = blockIdx.x - mat.pack;
+  const int r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
+  const bool tall = mat.rows > mat.cols;      // then X is the transpose of the matrix as it lies
+  _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
+  _Float16* same = arrays + (tall ? r.xt[0] : r.x);
+  _Float16* turned = arrays + (tall ? r.x : r.xt[0]);
+  const int64_t mn = (int64_t)r.mp * r.np;
+  const int ld_same = padded(mat.cols), ld_turned = padded(mat.rows);
+#pragma unroll
+  for (int p = threadIdx.x; p < 512; p += kThreads) {
+    const int row = r0 + (p >> 3), col = c0 + (p & 7) * 8;
+    float v[8];
+    if (row < mat.rows && col < mat.cols) {
+      const int64_t at = (int64_t)row * mat.cols + col;
+      load8(static_cast<const T*>(mat.in) + at, mat.cols - col, v);
+      if constexpr (MUON) {
+        float m[8];
+        load8(mat.momentum + at, mat.cols - col, m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = mo.nesterov ? fmaf(mo.mu, m[e] - v[e], v[e]) : m[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = row < mat.rows && col + e < mat.cols ? halves((float)((double)v[e] * scale)) : 0u;
+      tile[p >> 3][(p & 7) * 8 + e] = w[e];
+    }
+    put8(same + (int64_t)row * ld_same + col, mn, parts, w);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = threadIdx.x; p < 512; p += kThreads) {
+    const int col = p & 63, row = (p >> 6) * 8;
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = tile[row + e][col];
+    put8(turned + (int64_t)(c0 + col) * ld_turned + r0 + row, mn, parts, w);
+  }
+}
+
+enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
+
+struct Step {
+  float a, b, c;
+  int from;             // which of the two X^T arrays holds this step's
+  int parts_out;        // halves that the next reader wants
+  float shrink;         // LAST, Muon: 1 - lr wd
+  int* nan_flags;       // LAST, Muon: one int per matrix, set where the parameter as read holds a NaN
+};
+
+// Tiles: 128 x 128 by four waves of 64 x 64, or 64 x 64 by four of 32 x 32.  PARTS 2: 32 k a stage, PARTS 1: 64.
+template <int TILE, int PARTS>
+using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, true, true, PARTS == 2 ? 64 : 128, TILE == 128 ? 2 : 3>;
+
+template <int TILE, int PARTS, int KIND, bool MUON, typename T>
+__global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step st) {
+  using C = Core<TILE, PARTS>;
+  constexpr int W = TILE / 2, F = W / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const Table* t = reinterpret_cast<const Table*>(work);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr bool kSym = KIND == GRAM || KIND == POLY;
+  const int id0 = core::xcd_order(blockIdx.x, gridDim.x);
+  const int k = __builtin_amdgcn_readfirstlane(owner(t, id0, kSym ? &Mat::sym : &Mat::rect));
+  const Mat& mat = t->mat[k];
+  const Arrays r = arrays_of(mat.rows, mat.cols);
+  _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
+  const int64_t mn = (int64_t)r.mp * r.np, mm = (int64_t)r.mp * r.mp;
+  int ti, tj;
+  if constexpr (kSym) {      // tile id of the lower triangle: id = ti (ti + 1) / 2 + tj
+    const int id = id0 - mat.sym;
+    ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > id) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+    tj = id - ti * (ti + 1) / 2;
+  } else {
+    const int id = id0 - mat.rect, tiles_n = (r.np + TILE - 1) / TILE;
+    ti = id / tiles_n;
+    tj = id % tiles_n;
+  }
+  const int m0 = ti * TILE, n0 = tj * TILE;
+
+  typename C::SA sa;
+  typename C::SB sb;
+  int depth;
+  if constexpr (KIND == GRAM) {
+    sa.setup(arrays + r.x, r.np, m0, r.mp, 0, mn, wave, lane);
+    sb.setup(arrays + r.x, r.np, n0, r.mp, 0, mn, wave, lane);
+    depth = r.np;
+  } else if constexpr (KIND == POLY) {
+    sa.setup(arrays + r.a, r.mp, m0, r.mp, 0, mm, wave, lane);
+    sb.setup(arrays + r.a, r.mp, n0, r.mp, 0, mm, wave, lane);
+    depth = r.mp;
+  } else {
+    sa.setup(arrays + r.b, r.mp, m0, r.mp, 0, mm, wave, lane);
+    sb.setup(arrays + (st.from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, mn, wave, lane);
+    depth = r.mp;
+  }
+  f16v acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+  C::run(sa, sb, depth / C::BK, smem, acc, wave, lane, [](auto&) {});
+
+  // lane: row lane & 31 of a 32 x 32 block, register q: column 8 (q / 4) + 4 (lane / 32) + q % 4.  Through LDS, a block at a time and a wave by
+  // itself, so that both orientations leave as whole 16-byte pieces.
+  const int wm = m0 + (wave >> 1) * W, wn = n0 + (wave & 1) * W;
+  const int rows_end = r.mp, cols_end = kSym ? r.mp : r.np;
+  if (wm >= rows_end || wn >= cols_end) return;      // (a 128-wide tile of an odd number of 64s)
+  uint32_t* scratch = reinterpret_cast<uint32_t*>(smem) + wave * 32 * 33;
+  const int li = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+      const int rb = wm + 32 * i, cb = wn + 32 * j;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = rb + li, col = cb + 8 * q + 4 * h;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+        if constexpr (KIND == POLY) {
+          const _Float16* a = arrays + r.a + (int64_t)row * r.mp + col;
+          _Float16 hi[4], lo[4];
+          __builtin_memcpy(hi, a, 8);
+          if constexpr (PARTS == 2) __builtin_memcpy(lo, a + mm, 8);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = (float)hi[e];
+            if constexpr (PARTS == 2) x += (float)lo[e];
+            v[e] = fmaf(st.c, v[e] * (1.f / kScale), st.b * x) + (row == col + e ? st.a * kScale : 0.f);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= KIND == LAST ? 1.f / (kScale * kScale) : 1.f / kScale;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) scratch[li * 33 + 8 * q + 4 * h + e] = KIND == LAST ? __builtin_bit_cast(uint32_t, v[e]) : halves(v[e]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if constexpr (KIND == LAST) {
+        const bool tall = mat.rows > mat.cols;
+        T* out = static_cast<T*>(mat.out);
+#pragma unroll 4
+        for (int e = 0; e < 16; ++e) {
+          // neighbouring lanes: neighbouring columns of the matrix as it lies
+          const int major = 2 * e + h, minor = li;
+          const int row = tall ? cb + major : rb + major, col = tall ? rb + minor : cb + minor;
+          if (row < mat.rows && col < mat.cols) {
+            const float o = __builtin_bit_cast(float, tall ? scratch[minor * 33 + major] : scratch[major * 33 + minor]);
+            T* at = out + (int64_t)row * mat.cols + col;
+            if constexpr (MUON) {
+              const float p = *at;
+              if (st.nan_flags && p != p) st.nan_flags[k] = 1;
+              *at = fmaf(p, st.shrink, -mat.step * o);
+            } else {
+              *at = (T)o;
+            }
+          }
+        }
+      } else {
+        // direct and transposed: 32 rows of four pieces, two pieces a lane
+        _Float16* direct = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : r.x);
+        _Float16* turned = KIND == APPLY ? arrays + (st.from ? r.xt[0] : r.xt[1]) : direct;
+        const int64_t part = kSym ? mm : mn;
+        const int ld = kSym ? r.mp : r.np;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = (lane >> 2) + 16 * e, c = lane & 3;
+          uint32_t w[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
+          put8(direct + (int64_t)(rb + row) * ld + cb + 8 * c, part, st.parts_out, w);
+        }
+        if (!kSym || ti != tj) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = (lane >> 2) + 16 * e, c = lane & 3;
+            uint32_t w[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
+            put8(turned + (int64_t)(cb + row) * r.mp + rb + 8 * c, part, st.parts_out, w);
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------------------------
+
+constexpr int kMaxSide = 1 << 17;
+constexpr int kMaxSteps = 100;
+
+struct Layout {
+  int tile_sym, tile_rect;
+  int64_t bytes;
+};
+
+inline int64_t tiles(int v, int tile) { return (padded(v) + tile - 1) / tile; }
+
+// Table and workspace of one set of launches.  128-wide tiles where they alone occupy the part's 256 CUs (they read half as much per product),
+// else 64-wide ones: four times the workgroups.
+inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
+  int64_t sym = 0, rect = 0;
+  for (int i = 0; i < count; ++i) {
+    const int m = in[i].rows < in[i].cols ? in[i].rows : in[i].cols, n = in[i].rows < in[i].cols ? in[i].cols : in[i].rows;
+    sym += tiles(m, 128) * (tiles(m, 128) + 1) / 2;
+    rect += tiles(m, 128) * tiles(n, 128);
+  }
+  l->tile_sym = sym >= 256 ? 128 : 64;
+  l->tile_rect = rect >= 256 ? 128 : 64;
+  int64_t stat = 0, pack = 0, base = 0;
+  sym = rect = 0;
+  t->count = count;
+  for (int i = 0; i < count; ++i) {
+    Mat& m = t->mat[i];
+    m = Mat{};
+    m.in = in[i].in;
+    m.out = in[i].out;
+    m.momentum = in[i].momentum;
+    m.rows = in[i].rows;
+    m.cols = in[i].cols;
+    m.step = in[i].step;
+    const Arrays r = arrays_of(m.rows, m.cols);
+    const int64_t total = elements_of(m), chunk = chunk_of(total), ts = tiles(r.m, l->tile_sym);
+    m.stat = (int)stat;
+    m.pack = (int)pack;
+    m.sym = (int)sym;
+    m.rect = (int)rect;
+    m.base = base;
+    stat += (total + chunk - 1) / chunk;
+    pack += (int64_t)(r.mp / 64) * (r.np / 64);
+    sym += ts * (ts + 1) / 2;
+    rect += tiles(r.m, l->tile_rect) * tiles(r.n, l->tile_rect);
+    base += r.total * 2;
+    if (pack > 0x7ffffff0 || sym > 0x7ffffff0) return S2L_E_SIZE;
+  }
+  t->stat_blocks = (int)stat;
+  t->pack_blocks = (int)pack;
+  t->sym_tiles = (int)sym;
+  t->rect_tiles = (int)rect;
+  const int64_t front = kTableBytes + partial_bytes((int)stat);
+  for (int i = 0; i < count; ++i) t->mat[i].base += front;
+  l->bytes = front + base;
+  return 0;
+}
+
+// Whether the halves hold every X, A and B of `steps` steps with these coefficients: singular values start at most at 1 (the Frobenius norm) and
+// p's largest value on the interval so far bounds the next; entries are bounded by the largest singular value.  2^11 * 16 < 65504.
+inline bool within_range(double a, double b, double c, int steps) {
+  double top = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    double next = 0.0, poly = 0.0;
+    for (int i = 0; i <= 256; ++i) {
+      const double s = top * i / 256, q = std::fabs(a + b * s * s + c * s * s * s * s);
+      if (!(q <= 16.0)) return false;
+      poly = q > poly ? q : poly;
+      next = s * q > next ? s * q : next;
+    }
+    top = next * 1.01;      // between two samples, and the roundings
+    if (k + 1 < steps && !(top <= 4.0)) return false;      // A's entries: top^2 <= 16
+    if (top < 1e-6) top = 1e-6;
+  }
+  return true;
+}
+
+template <typename K> int launch(K kernel, int blocks, int lds, hipStream_t st, char* work, const Step& s) {
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, st, work, s);
+  return (int)hipGetLastError();
+}
+
+template <int TILE, int PARTS, int KIND, bool MUON, typename T> int one(int blocks, hipStream_t st, char* work, const Step& s) {
+  constexpr int lds = Core<TILE, PARTS>::kLds > 4 * 32 * 33 * 4 ? Core<TILE, PARTS>::kLds : 4 * 32 * 33 * 4;
+  static_assert(lds <= 65536, "above 64 KiB the launch needs an opt-in");
+  return launch(product_kernel<TILE, PARTS, KIND, MUON, T>, blocks, lds, st, work, s);
+}
+
+template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, hipStream_t st, char* work, const Step& s) {
+  if (tile == 128) return parts == 2 ? one<128, 2, KIND, MUON, T>(blocks, st, work, s) : one<128, 1, KIND, MUON, T>(blocks, st, work, s);
+  return parts == 2 ? one<64, 2, KIND, MUON, T>(blocks, st, work, s) : one<64, 1, KIND, MUON, T>(blocks, st, work, s);
+}
+
+template <typename T, bool MUON>
+int run(const s2l_matrix* in, int count, double a, double b, double c, float eps, int steps, Momentum mo, float shrink, int* nan_flags, char* work, hipStream_t st) {
+  for (int first = 0; first < count; first += kMaxMatrices) {
+    const int n = count - first < kMaxMatrices ? count - first : kMaxMatrices;
+    Table t;
+    Layout l;
+    int rc = lay_out(in + first, n, &t, &l);
+    if (rc) return rc;
+    const auto parts = [&](int k) { return sizeof(T) == 4 || k < steps - 2 ? 2 : 1; };
+    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(t.stat_blocks), dim3(kThreads), 0, st, t, work, mo);
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+    hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(t.pack_blocks), dim3(kThreads), 0, st, work, mo, eps, parts(0));
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+    for (int k = 0; k < steps; ++k) {
+      Step s{(float)a, (float)b, (float)c, k & 1, parts(k), shrink, nan_flags ? nan_flags + first : nullptr};
+      // (GRAM, POLY and APPLY do not depend on the matrices' type: one instance)
+      rc = any<GRAM, false, float>(l.tile_sym, parts(k), t.sym_tiles, st, work, s);
+      if (rc) return rc;
+      rc = any<POLY, false, float>(l.tile_sym, parts(k), t.sym_tiles, st, work, s);
+      if (rc) return rc;
+      if (k + 1 < steps) {
+        s.parts_out = parts(k + 1);
+        rc = any<APPLY, false, float>(l.tile_rect, parts(k), t.rect_tiles, st, work, s);
+      } else {
+        rc = any<LAST, MUON, T>(l.tile_rect, parts(k), t.rect_tiles, st, work, s);
+      }
+      if (rc) return rc;
+    }
+  }
+  return 0;
+}
+
+inline int check(const s2l_matrix* mats, int64_t count, bool muon, int size) {
+  if (count < 0 || count > (1 << 20)) return S2L_E_SIZE;
+  if (count && !mats) return S2L_E_NULL;
+  for (int64_t i = 0; i < count; ++i) {
+    if (mats[i].rows < 1 || mats[i].cols < 1 || mats[i].rows > kMaxSide || mats[i].cols > kMaxSide) return S2L_E_SIZE;
+    if (!mats[i].in || !mats[i].out || (muon && !mats[i].momentum)) return S2L_E_NULL;
+    for (const void* p : {mats[i].in, (const void*)mats[i].out, (const void*)(muon ? mats[i].momentum : nullptr)})
+      if (reinterpret_cast<uintptr_t>(p) & (size - 1)) return S2L_E_ALIGN;
+  }
+  return 0;
+}
+
+}  // namespace ns
+}  // namespace s2l
+
+extern "C" int64_t s2l_orthogonalize_work_bytes(const s2l_matrix* matrices_host, int64_t count) {
+  using namespace s2l::ns;
+  if (count <= 0 || !matrices_host || count > (1 << 20)) return 0;
+  int64_t most = 0;
+  for (int64_t first = 0; first < count; first += kMaxMatrices) {
+    const int n = (int)(count - first < kMaxMatrices ? count - first : kMaxMatrices);
+    for (int i = 0; i < n; ++i) {
+      const s2l_matrix& m = matrices_host[first + i];
+      if (m.rows < 1 || m.cols < 1 || m.rows > kMaxSide || m.cols > kMaxSide) return 0;
+    }
+    Table t;
+    Layout l;
+    if (lay_out(matrices_host + first, n, &t, &l)) return 0;
+    most = l.bytes > most ? l.bytes : most;
+  }
+  return most;
+}
+
+extern "C" int s2l_orthogonalize(int dtype, const s2l_matrix* matrices_host, int64_t count, double a, double b, double c, float eps, int steps, void* work,
+                                 s2l_stream_t stream) {
+  using namespace s2l::ns;
+  const int size = dtype == S2L_DTYPE_F32 ? 4 : dtype == S2L_DTYPE_BF16 || dtype == S2L_DTYPE_F16 ? 2 : 0;
+  if (!size) return S2L_E_UNSUPPORTED;
+  const int rc = check(matrices_host, count, false, size);
+  if (rc) return rc;
+  if (steps < 1 || steps > kMaxSteps || !(eps > 0.f) || !within_range(a, b, c, steps)) return S2L_E_SIZE;
+  if (count == 0) return S2L_OK;
+  if (!work) return S2L_E_NULL;
+  if (s2l::misaligned16(work)) return S2L_E_ALIGN;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(work);
+  const int n = (int)count;
+  if (dtype == S2L_DTYPE_F32) return run<float, false>(matrices_host, n, a, b, c, eps, steps, Momentum{}, 0.f, nullptr, ws, st);
+  if (dtype == S2L_DTYPE_BF16) return run<__bf16, false>(matrices_host, n, a, b, c, eps, steps, Momentum{}, 0.f, nullptr, ws, st);
+  return run<_Float16, false>(matrices_host, n, a, b, c, eps, steps, Momentum{}, 0.f, nullptr, ws, st);
+}
+
+extern "C" int s2l_muon_step(const s2l_matrix* matrices_host, int64_t count, float momentum, int nesterov, float shrink, double a, double b, double c, float eps,
+                             int steps, int* nan_flags, void* work, s2l_stream_t stream) {
+  using namespace s2l::ns;
+  const int rc = check(matrices_host, count, true, 4);
+  if (rc) return rc;
+  if (steps < 1 || steps > kMaxSteps || !(eps > 0.f) || !within_range(a, b, c, steps)) return S2L_E_SIZE;
+  if (count == 0) return S2L_OK;
+  if (!work) return S2L_E_NULL;
+  if (s2l::misaligned16(work)) return S2L_E_ALIGN;
+  return run<float, true>(matrices_host, (int)count, a, b, c, eps, steps, Momentum{momentum, nesterov}, shrink, nan_flags, static_cast<char*>(work),
+                          static_cast<hipStream_t>(stream));
+}

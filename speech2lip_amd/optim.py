@@ -8,10 +8,16 @@ the pass reads every parameter anyway -- the NaN scan of `check_weights` (src/co
 
 Same constructor arguments, same `state_dict()` layout (`step`, `exp_avg`, `exp_avg_sq` per parameter) as `torch.optim.Adam`: a checkpoint
 written by either loads into the other (the reference's checkpoints carry `optimizer.state_dict()`, checkpoints.py:38-41).  fp32 CUDA
-parameters with dense gradients; no amsgrad / maximize / capturable (the reference uses none of them).  There is no CPU path."""
+parameters with dense gradients; no amsgrad / maximize / capturable (the reference uses none of them).  There is no CPU path.
+
+`FusedMuon` is the same for `torch.optim.Muon` (the update of a weight matrix orthogonalised before it is applied; its arithmetic in 32 bits where
+torch's is bf16), with an Adam of its own for the parameters that are no such matrix; `orthogonalize` is its Newton-Schulz iteration alone
+(csrc/orthogonalize.hip: every matrix of a group in the same 2 + 3 * steps launches)."""
 from __future__ import annotations
 
 import ctypes
+import math
+import struct
 
 import torch
 
@@ -56,60 +62,63 @@ class FusedAdam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = _abi.load()
         self._flag_jobs = []
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
-            if not ps:
-                continue
-            dev = ps[0].device
-            for p in ps:
-                if p.device != dev or dev.type != "cuda" or p.dtype != torch.float32 or p.grad.is_sparse or not p.is_contiguous():
-                    raise _abi.S2LError("FusedAdam takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
-                st = self.state[p]
-                if not st:
-                    st["step"] = torch.tensor(0.0, dtype=torch.float32)          # (torch.optim.Adam's own layout: a host scalar tensor)
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            steps = {float(self.state[p]["step"]) for p in ps}
-            if len(steps) != 1:
-                raise _abi.S2LError("FusedAdam: the parameters of one group must share their step count (one launch has one bias correction)")
-            step_no = int(steps.pop()) + 1
-            plan = self._plan(gi, ps)
-            grads = [p.grad if (p.grad.dtype == torch.float32 and p.grad.is_contiguous()) else p.grad.to(torch.float32).contiguous() for p in ps]
-            ptrs = []
-            for p, g in zip(ps, grads):
-                st = self.state[p]
-                ptrs += [p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()]
-            with torch.cuda.device(dev):
-                stream = torch.cuda.current_stream()
-                if ptrs != plan["ptrs"]:      # (gradients are fresh tensors every step in the fused trainer: 2.4 KB of pointers cross once per step)
-                    if plan["copied"] is not None:
-                        plan["copied"].synchronize()      # the pinned staging block of the previous step has left
-                    plan["host"].copy_(torch.tensor(ptrs, dtype=torch.int64))
-                    plan["table"].copy_(plan["host"], non_blocking=True)
-                    plan["copied"] = torch.cuda.Event()
-                    plan["copied"].record(stream)
-                    plan["ptrs"] = ptrs
-                # (flags per step, not per plan: a pipelined caller reads step k's report after step k + 1 has been queued; the pinned block
-                #  comes from torch's caching host allocator)
-                flags = torch.zeros(len(ps), dtype=torch.int32, device=dev)
-                flags_host = torch.empty(len(ps), dtype=torch.int32, pin_memory=True)
-                b1, b2 = group["betas"]
-                _abi.check(lib.s2l_adam_step(ctypes.c_void_p(plan["table"].data_ptr()), ctypes.c_void_p(plan["blocks"].data_ptr()),
-                                             ctypes.c_void_p(plan["counts"].data_ptr()), len(ps), plan["n_blocks"], float(group["lr"]), float(b1),
-                                             float(b2), float(group["eps"]), float(group["weight_decay"]), step_no,
-                                             ctypes.c_void_p(flags.data_ptr()), ctypes.c_void_p(stream.cuda_stream)), "s2l_adam_step")
-                flags_host.copy_(flags, non_blocking=True)
-                done = torch.cuda.Event()
-                done.record(stream)
-            self._flag_jobs.append((ps, flags_host, done, grads))      # (`grads` keeps converted copies alive until the launch has run)
-            for p in ps:
-                self.state[p]["step"] += 1
-                # the kernel wrote through raw pointers: tell autograd the tensor changed in place, as torch's own in-place update would --
-                # the model's packed-weight caches (TalkingFace.packed_weights, SimpleUnetLight.packed_weights*) key on the version counters
-                torch.autograd.graph.increment_version(p)
+            if ps:
+                self._step_group(gi, group, ps)
         return loss
+
+    def _step_group(self, gi, group, ps):
+        """One launch of s2l_adam_step for the parameters `ps` of group `gi`."""
+        lib = _abi.load()
+        dev = ps[0].device
+        for p in ps:
+            if p.device != dev or dev.type != "cuda" or p.dtype != torch.float32 or p.grad.is_sparse or not p.is_contiguous():
+                raise _abi.S2LError("FusedAdam takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
+            st = self.state[p]
+            if not st:
+                st["step"] = torch.tensor(0.0, dtype=torch.float32)          # (torch.optim.Adam's own layout: a host scalar tensor)
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        steps = {float(self.state[p]["step"]) for p in ps}
+        if len(steps) != 1:
+            raise _abi.S2LError("FusedAdam: the parameters of one group must share their step count (one launch has one bias correction)")
+        step_no = int(steps.pop()) + 1
+        plan = self._plan(gi, ps)
+        grads = [p.grad if (p.grad.dtype == torch.float32 and p.grad.is_contiguous()) else p.grad.to(torch.float32).contiguous() for p in ps]
+        ptrs = []
+        for p, g in zip(ps, grads):
+            st = self.state[p]
+            ptrs += [p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()]
+        with torch.cuda.device(dev):
+            stream = torch.cuda.current_stream()
+            if ptrs != plan["ptrs"]:      # (gradients are fresh tensors every step in the fused trainer: 2.4 KB of pointers cross once per step)
+                if plan["copied"] is not None:
+                    plan["copied"].synchronize()      # the pinned staging block of the previous step has left
+                plan["host"].copy_(torch.tensor(ptrs, dtype=torch.int64))
+                plan["table"].copy_(plan["host"], non_blocking=True)
+                plan["copied"] = torch.cuda.Event()
+                plan["copied"].record(stream)
+                plan["ptrs"] = ptrs
+            # (flags per step, not per plan: a pipelined caller reads step k's report after step k + 1 has been queued; the pinned block
+            #  comes from torch's caching host allocator)
+            flags = torch.zeros(len(ps), dtype=torch.int32, device=dev)
+            flags_host = torch.empty(len(ps), dtype=torch.int32, pin_memory=True)
+            b1, b2 = group["betas"]
+            _abi.check(lib.s2l_adam_step(ctypes.c_void_p(plan["table"].data_ptr()), ctypes.c_void_p(plan["blocks"].data_ptr()),
+                                         ctypes.c_void_p(plan["counts"].data_ptr()), len(ps), plan["n_blocks"], float(group["lr"]), float(b1),
+                                         float(b2), float(group["eps"]), float(group["weight_decay"]), step_no,
+                                         ctypes.c_void_p(flags.data_ptr()), ctypes.c_void_p(stream.cuda_stream)), "s2l_adam_step")
+            flags_host.copy_(flags, non_blocking=True)
+            done = torch.cuda.Event()
+            done.record(stream)
+        self._flag_jobs.append((ps, flags_host, done, grads))      # (`grads` keeps converted copies alive until the launch has run)
+        for p in ps:
+            self.state[p]["step"] += 1
+            # the kernel wrote through raw pointers: tell autograd the tensor changed in place, as torch's own in-place update would --
+            # the model's packed-weight caches (TalkingFace.packed_weights, SimpleUnetLight.packed_weights*) key on the version counters
+            torch.autograd.graph.increment_version(p)
 
     def take_nan_jobs(self):
         """The last `step()`'s flag transfers, handed over to the caller (Trainer keeps them with its pending step): pass to `nan_report`."""
@@ -131,3 +140,188 @@ class FusedAdam(torch.optim.Optimizer):
     def covers(self):
         """The parameters whose NaN state `nan_report()` answers for (ids), given the gradients present now."""
         return {id(p) for g in self.param_groups for p in g["params"] if p.grad is not None}
+
+
+def _matrix_table(records):
+    """s2l_matrix records (in, out, momentum, rows, cols, step) as one host block."""
+    words = []
+    for src, out, momentum, rows, cols, step in records:
+        words += (src, out, momentum, rows | cols << 32, struct.unpack("i", struct.pack("f", step))[0])
+    return (ctypes.c_int64 * len(words))(*words)
+
+
+def _check_iteration(who, steps, coefficients, eps):
+    if not (isinstance(steps, int) and 1 <= steps <= 100):
+        raise ValueError(f"{who}: steps must be a whole number from 1 to 100: got {steps!r}")
+    if len(coefficients) != 3 or not all(math.isfinite(float(c)) for c in coefficients):
+        raise ValueError(f"{who}: three finite coefficients (a, b, c): got {coefficients!r}")
+    if not eps > 0:
+        raise ValueError(f"{who}: eps must be above 0: got {eps!r}")
+    a, b, c = (float(v) for v in coefficients)
+    top = 1.0      # the largest singular value so far (the Frobenius norm starts at 1): the same bound as the library's, checked there again
+    for k in range(steps):
+        s = [top * i / 2048 for i in range(2049)]
+        q = [abs(a + b * x * x + c * x ** 4) for x in s]
+        top = max(max(x * y for x, y in zip(s, q)) * 1.01, 1e-6)
+        if max(q) > 16 or (k + 1 < steps and top > 4):
+            raise ValueError(f"{who}: with the coefficients {coefficients!r} a singular value can grow past 4 (or its factor past 16) in step {k + 1}: "
+                             "beyond the range of the iteration's halves")
+    return a, b, c
+
+
+_ORTH_DTYPES = {torch.float32: _abi.S2L_DTYPE_F32, torch.bfloat16: _abi.S2L_DTYPE_BF16, torch.float16: _abi.S2L_DTYPE_F16}
+_CHECKED = set()      # iterations that passed _check_iteration: (steps, coefficients, eps)
+
+
+def _iteration(who, steps, coefficients, eps):
+    key = (steps, tuple(coefficients), eps)
+    if key not in _CHECKED:
+        _check_iteration(who, steps, coefficients, eps)
+        _CHECKED.add(key)
+    return key[1]
+
+
+def _orthogonalize_into(sources, outs, steps, coefficients, eps):
+    """The matrices of `sources` (dense [..., rows, cols], one type, one GPU) to `outs`, in one set of launches."""
+    lib = _abi.load()
+    records = []
+    for src, out in zip(sources, outs):
+        rows, cols = src.shape[-2:]
+        stride = rows * cols * src.element_size()
+        if stride:
+            records += [(src.data_ptr() + i * stride, out.data_ptr() + i * stride, 0, rows, cols, 0.0) for i in range(src.numel() // (rows * cols))]
+    if not records:
+        return
+    dev = sources[0].device
+    table = _matrix_table(records)
+    with torch.cuda.device(dev):
+        work = torch.empty(lib.s2l_orthogonalize_work_bytes(table, len(records)), dtype=torch.uint8, device=dev)
+        a, b, c = coefficients
+        _abi.check(lib.s2l_orthogonalize(_ORTH_DTYPES[sources[0].dtype], table, len(records), a, b, c, eps, steps, work.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream), "s2l_orthogonalize")
+
+
+@torch.no_grad()
+def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+    """The Newton-Schulz iteration of Muon: X0 = G / max(||G||_F, eps), then `steps` times X <- (a I + b A + c A A) X with A = X X^T of the shorter
+    side.  With the default coefficients the singular values end in 0.7 .. 1.2 (but for the smallest): nearly U V^T.
+
+    update [..., rows, cols], or a list of such tensors of any sizes, all float32, all bfloat16 or all float16 on one GPU -> the same shape(s) and type,
+    in one set of launches.  float32: fp32's accuracy throughout; the 16-bit types: rounded once, their last two steps on half-precision products.
+    A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not)."""
+    many = isinstance(update, (list, tuple))
+    given = list(update) if many else [update]
+    for t in given:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("orthogonalize: a tensor [..., rows, cols] or a list of them")
+        if t.dim() < 2:
+            raise ValueError(f"orthogonalize: matrices [..., rows, cols]: got {tuple(t.shape)}")
+        if t.dtype not in _ORTH_DTYPES or t.dtype != given[0].dtype:
+            raise ValueError(f"orthogonalize: all float32, all bfloat16 or all float16: got {t.dtype}")
+        if max(t.shape[-2:]) > 131072:
+            raise ValueError(f"orthogonalize: at most 131072 rows and columns: got {tuple(t.shape)}")
+    coefficients = _iteration("orthogonalize", steps, coefficients, eps)
+    for t in given:
+        if not t.is_cuda or t.device != given[0].device:
+            raise _abi.S2LError("orthogonalize: every tensor must be on one GPU (no CPU fallback)")
+    sources = [t.contiguous() for t in given]
+    outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in sources]
+    if sources:
+        _orthogonalize_into(sources, outs, steps, coefficients, eps)
+    return outs if many else outs[0]
+
+
+class FusedMuon(FusedAdam):
+    """`torch.optim.Muon` -- momentum, orthogonalisation of the update, decoupled weight decay -- for every matrix of a parameter group in one set of
+    launches (s2l_muon_step), the Newton-Schulz products at fp32's accuracy; the same constructor arguments and `state_dict()` layout
+    (`momentum_buffer` per parameter).  Parameters of more than two dimensions (convolutions) are taken as [shape[0], everything else].
+
+        m <- m + (1 - momentum) (g - m);  u = g + momentum (m - g) if nesterov else m
+        p <- (1 - lr weight_decay) p - lr_p orth(u),  lr_p = lr sqrt(max(1, rows / cols))             adjust_lr_fn None or "original"
+                                                            = lr 0.2 sqrt(max(rows, cols))               "match_rms_adamw"
+    A group with `algorithm="adam"` is stepped by FusedAdam (its own lr 1e-3, betas, eps 1e-8, weight_decay 0 unless given): biases, embeddings, the
+    output layer, whatever is no weight matrix -- so that a Trainer drives both through one optimiser (`muon_groups` splits a model).
+    fp32 CUDA parameters, contiguous, dense gradients; NaN report as FusedAdam's.  No CPU path, not for capture into a graph."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5,
+                 adjust_lr_fn=None):
+        self._plans, self.nan_flags, self._flag_jobs = {}, None, []
+        torch.optim.Optimizer.__init__(self, params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                                          ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                                                          algorithm="muon"))
+
+    def add_param_group(self, param_group):
+        g = dict(param_group)
+        if g.get("algorithm", "muon") == "adam":
+            for key, value in (("lr", 1e-3), ("betas", (0.9, 0.999)), ("eps", 1e-8), ("weight_decay", 0.0), ("amsgrad", False)):
+                g.setdefault(key, value)
+            if g["amsgrad"]:
+                raise NotImplementedError("FusedMuon: amsgrad is not supported")
+            if g["lr"] < 0 or g["eps"] < 0 or g["weight_decay"] < 0 or not all(0 <= v < 1 for v in g["betas"]):
+                raise ValueError("FusedMuon: invalid hyper-parameter of an adam group")
+        elif g.get("algorithm", "muon") != "muon":
+            raise ValueError(f"FusedMuon: algorithm must be \"muon\" or \"adam\": got {g['algorithm']!r}")
+        else:
+            full = {**self.defaults, **g}
+            if full["lr"] < 0 or full["weight_decay"] < 0 or not 0 <= full["momentum"] <= 1:
+                raise ValueError("FusedMuon: invalid hyper-parameter (lr, weight_decay >= 0, momentum in 0 .. 1)")
+            if full["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
+                raise ValueError(f"FusedMuon: adjust_lr_fn must be None, \"original\" or \"match_rms_adamw\": got {full['adjust_lr_fn']!r}")
+            _iteration("FusedMuon", full["ns_steps"], full["ns_coefficients"], full["eps"])
+            g["params"] = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            for p in g["params"]:
+                t = p[1] if isinstance(p, tuple) else p
+                if isinstance(t, torch.Tensor) and (t.dim() < 2 or t.numel() == 0 or max(t.shape[0], t.numel() // t.shape[0]) > 131072):
+                    raise ValueError(f"FusedMuon: a muon group takes matrices of 1 .. 131072 rows and columns (others: a group with algorithm=\"adam\"): "
+                                     f"got {tuple(t.shape)}")
+        super().add_param_group(g)
+
+    def _step_group(self, gi, group, ps):
+        if group.get("algorithm", "muon") == "adam":
+            return super()._step_group(gi, group, ps)
+        lib = _abi.load()
+        dev = ps[0].device
+        lr, mode = float(group["lr"]), group["adjust_lr_fn"]
+        records, grads, buffers = [], [], []
+        for p in ps:
+            g = p.grad
+            if p.device != dev or not p.is_cuda or p.dtype != torch.float32 or g.is_sparse or not p.is_contiguous():
+                raise _abi.S2LError("FusedMuon takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
+            st = self.state[p]
+            m = st.get("momentum_buffer")
+            if m is None:
+                m = st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            if m.shape != p.shape or m.dtype != torch.float32 or m.device != dev or not m.is_contiguous():
+                m = st["momentum_buffer"] = m.to(device=dev, dtype=torch.float32).reshape(p.shape).contiguous()
+            if g.dtype != torch.float32 or not g.is_contiguous():
+                g = g.to(torch.float32).contiguous()
+            rows = p.shape[0]
+            cols = p.numel() // rows
+            scale = 0.2 * math.sqrt(max(rows, cols)) if mode == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
+            records.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols, lr * scale))
+            grads.append(g)
+            buffers.append(m)
+        table = _matrix_table(records)
+        a, b, c = _iteration("FusedMuon", group["ns_steps"], group["ns_coefficients"], group["eps"])
+        with torch.cuda.device(dev):
+            stream = torch.cuda.current_stream()
+            flags = torch.zeros(len(ps), dtype=torch.int32, device=dev)
+            flags_host = torch.empty(len(ps), dtype=torch.int32, pin_memory=True)
+            work = torch.empty(lib.s2l_orthogonalize_work_bytes(table, len(ps)), dtype=torch.uint8, device=dev)
+            _abi.check(lib.s2l_muon_step(table, len(ps), float(group["momentum"]), int(bool(group["nesterov"])), 1.0 - lr * float(group["weight_decay"]), a, b, c,
+                                         float(group["eps"]), group["ns_steps"], flags.data_ptr(), work.data_ptr(), stream.cuda_stream), "s2l_muon_step")
+            flags_host.copy_(flags, non_blocking=True)
+            done = torch.cuda.Event()
+            done.record(stream)
+        self._flag_jobs.append((ps, flags_host, done, grads))
+        torch.autograd.graph.increment_version(ps + buffers)      # written through raw pointers (see FusedAdam)
+
+
+def muon_groups(model, adam_names=("output_linear.", "outc.", "canonical_depth_head"), muon=None, adam=None):
+    """Parameter groups of `model` for FusedMuon: its weight matrices (two or more dimensions), and, stepped by Adam, everything else and whatever
+    `adam_names` name by their beginning (the output layers, the depth image).  muon / adam: options of the two groups."""
+    named = [(k, p) for k, p in model.named_parameters() if p.requires_grad]
+    is_matrix = lambda k, p: p.dim() >= 2 and not any(part in "." + k for part in ("." + a for a in adam_names))  # noqa: E731
+    groups = [{"params": [p for k, p in named if is_matrix(k, p)], **(muon or {}), "algorithm": "muon"},
+              {"params": [p for k, p in named if not is_matrix(k, p)], **(adam or {}), "algorithm": "adam"}]
+    return [g for g in groups if g["params"]]

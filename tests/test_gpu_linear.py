@@ -237,7 +237,7 @@ def test_rows_behind_the_last_one_are_left_alone(dev):
             ldo = n + 5
             out = torch.full((rows + 2, ldo), 7.0, dtype=dtype, device=dev)
             saved = torch.full((lib.s2l_linear_saved_bytes(dt, 4, rows, n) + 64,), 85, dtype=torch.uint8, device=dev)
-            work = torch.full((lib.s2l_linear_forward_work_bytes(dt, rows, k, n) + 64,), 85, dtype=torch.uint8, device=dev)
+            work = torch.full((lib.s2l_linear_forward_work_bytes(dt, 4, 1, rows, k, n) + 64,), 85, dtype=torch.uint8, device=dev)
             s = torch.cuda.current_stream().cuda_stream
             _abi.check(lib.s2l_linear_forward(dt, d["x"].data_ptr(), k, d["weight"].data_ptr(), k, d["bias"].data_ptr(), d["residual"].data_ptr(), n,
                                               out.data_ptr() + (ldo + 2) * size, ldo, saved.data_ptr(), work.data_ptr(), rows, k, n, 4, 0.0, s), "forward")
@@ -316,7 +316,7 @@ def test_c_entry_refusals_need_no_gpu():
     assert fwd(x=0) == -1 and fwd(w=0) == -1 and fwd(o=0) == -1
     assert fwd(ldx=7) == -2 and fwd(ldw=7) == -2 and fwd(ldo=5) == -2 and fwd(ldr=5) == -2
     assert fwd(x=odd) == -3 and fwd(dt=1, w=odd) == -3 and fwd(b=p + 2) == -3 and fwd(work=p + 8) == -3
-    assert lib.s2l_linear_forward_work_bytes(0, 33, 5000, 17) > 0 and fwd(rows=33, k=5000, n=17, ldx=5000, ldw=5000, ldr=17, ldo=17, work=0) == -1
+    assert lib.s2l_linear_forward_work_bytes(0, 1, 0, 33, 5000, 17) > 0 and fwd(rows=33, k=5000, n=17, ldx=5000, ldw=5000, ldr=17, ldo=17, work=0) == -1
     bwd = lambda dt=0, dy=p, lddy=6, x=p, ldx=8, w=p, ldw=8, saved=p, dx=p, lddx=8, dw=p, db=p, work=p, rows=3, k=8, n=6, act=1: lib.s2l_linear_backward(  # noqa: E731
         dt, dy, lddy, x, ldx, w, ldw, saved, dx, lddx, dw, db, work, rows, k, n, act, 0.0, 0)
     assert bwd(dx=0, dw=0, db=0) == 0
@@ -324,5 +324,5 @@ def test_c_entry_refusals_need_no_gpu():
     assert bwd(dt=7) == -5 and bwd(act=9) == -5 and bwd(rows=-1) == -2 and bwd(lddy=5) == -2 and bwd(lddx=7) == -2 and bwd(ldx=7) == -2 and bwd(ldw=7) == -2
     assert bwd(dy=odd) == -3 and bwd(work=p + 4) == -3 and bwd(act=3, saved=p + 1) == -3
     for act in range(5):      # no rows: sizes are asked for all the same
-        assert lib.s2l_linear_forward_work_bytes(0, 0, 20, 12) == 0 and lib.s2l_linear_backward_work_bytes(0, act, 0, 20, 12) == 256
+        assert lib.s2l_linear_forward_work_bytes(0, act, 1, 0, 20, 12) == 0 and lib.s2l_linear_backward_work_bytes(0, act, 0, 20, 12) == 256
     assert lib.s2l_linear_saved_bytes(0, 1, 10, 17) == 30 and lib.s2l_linear_saved_bytes(1, 4, 10, 17) == 340 and lib.s2l_linear_saved_bytes(1, 0, 10, 17) == 0
