@@ -40,12 +40,13 @@ struct Mat {
   int64_t base;         // byte offset of this matrix's arrays in the workspace
   int rows, cols;
   float step;           // Muon: lr_p
-  int stat, pack, sym, rect;      // first workgroup of each kind of launch
+  int stat;             // first partial sum of squares
 };
 
+enum { STAT = 0, PACK = 1, SYM = 2, RECT = 3, KINDS = 4 };      // the kinds of launches
+
 struct Table {
-  int count;
-  int stat_blocks, pack_blocks, sym_tiles, rect_tiles;
+  int first[KINDS][kMaxMatrices];      // each matrix's first workgroup; 0x7fffffff behind the last matrix
   Mat mat[kMaxMatrices];
 };
 static_assert(sizeof(Table) <= 3840, "the table and a few scalars share the 4 KiB of kernel arguments");
@@ -57,7 +58,7 @@ __host__ __device__ inline int64_t chunk_of(int64_t elements) {      // elements
   return c <= 4096 ? 4096 : (c + 2047) / 2048 * 2048;
 }
 
-// the arrays of one matrix, in halves from its base; `part` = distance of the lo array from the hi one
+// the arrays of one matrix, in halves from its base: each has room for pairs (core::pair_at); in steps on hi alone it holds rows of those
 struct Arrays {
   int m, n, mp, np;
   int64_t x, xt[2], a, b, total;
@@ -82,10 +83,46 @@ constexpr int64_t kTableBytes = 4096;
 constexpr int64_t partial_bytes(int stat_blocks) { return ((int64_t)stat_blocks * 8 + 255) / 256 * 256; }
 
 // which matrix workgroup `id` of a launch belongs to: every lane compares one first workgroup
-__device__ __forceinline__ int owner(const Table* t, int id, int Mat::*first) {
+__device__ __forceinline__ int owner(const int* first, int id) {
   const int lane = threadIdx.x & 63;
-  const int mine = lane < t->count ? t->mat[lane].*first : 0x7fffffff;
-  return __popcll(__ballot(mine <= id)) - 1;
+  const int mine = lane < kMaxMatrices ? first[lane] : 0x7fffffff;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= id)) - 1);
+}
+
+// Matrices of one size, their inputs and outputs at equal distances (one matrix; a batch): the first and the distances are in the kernel's arguments
+// and there is no table to look through, two memory round trips less in every launch (of 3 .. 6 us where the matrices are small).
+struct Alike {
+  Mat mat;
+  int per[KINDS];      // workgroups of one matrix; 0: not alike, look into the table
+  int stride;          // bytes from one input / output to the next (at most 56 of them: below 2^31 checked)
+  int64_t bytes;       // of one matrix's arrays
+};
+struct Place {
+  Mat mat;
+  int index;      // of the matrix
+  int id;         // workgroup within the matrix
+};
+__device__ __forceinline__ Place place_of(const char* work, const Alike& alike, int kind, int id) {
+  if (alike.per[0]) {
+    const int k = id / alike.per[kind];
+    Mat m = alike.mat;
+    m.in = static_cast<const char*>(m.in) + (int64_t)k * alike.stride;
+    m.out = static_cast<char*>(m.out) + (int64_t)k * alike.stride;
+    m.base += k * alike.bytes;
+    m.stat += k * alike.per[STAT];
+    return Place{m, k, id - k * alike.per[kind]};
+  }
+  const Table* t = reinterpret_cast<const Table*>(work);
+  const int k = owner(t->first[kind], id);
+  Mat m = t->mat[k];      // (one value for the workgroup: in scalar registers)
+  m.in = core::uniform64(m.in);
+  m.out = core::uniform64(m.out);
+  m.momentum = core::uniform64(m.momentum);
+  m.base = core::uniform64(m.base);
+  m.rows = __builtin_amdgcn_readfirstlane(m.rows);
+  m.cols = __builtin_amdgcn_readfirstlane(m.cols);
+  m.stat = __builtin_amdgcn_readfirstlane(m.stat);
+  return Place{m, k, id - __builtin_amdgcn_readfirstlane(t->first[kind][k])};
 }
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, float* v) {
@@ -123,9 +160,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void nor
     const uint32_t* src = reinterpret_cast<const uint32_t*>(&t);
     for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += kThreads) reinterpret_cast<uint32_t*>(work)[i] = src[i];
   }
-  int k = 0;
-  while (k + 1 < t.count && t.mat[k + 1].stat <= (int)blockIdx.x) ++k;
-  const Mat& mat = t.mat[k];
+  const Mat& mat = t.mat[owner(t.first[STAT], blockIdx.x)];
   const int64_t total = elements_of(mat), chunk = chunk_of(total);
   const int64_t begin = (int64_t)(blockIdx.x - mat.stat) * chunk, end = begin + chunk < total ? begin + chunk : total;
   const T* g = static_cast<const T*>(mat.in);
@@ -160,8 +195,9 @@ __device__ __forceinline__ uint32_t halves(float v) {      // hi | lo << 16
   return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, lo) << 16;
 }
 
-// eight neighbouring values (hi | lo << 16 each) to the hi array and, parts == 2, the lo array
-__device__ __forceinline__ void put8(_Float16* hi, int64_t part, int parts, const uint32_t* w) {
+// eight neighbouring values (hi | lo << 16 each) to (row, col) of a matrix of `parts` halves
+__device__ __forceinline__ void put8(_Float16* p, int64_t row, int64_t col, int64_t ld, int parts, const uint32_t* w) {
+  _Float16* hi = p + (parts == 2 ? core::pair_at<2>(row, col, ld) : core::pair_at<1>(row, col, ld));
   u4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = (w[2 * e] & 0xffffu) | w[2 * e + 1] << 16;
@@ -169,17 +205,16 @@ __device__ __forceinline__ void put8(_Float16* hi, int64_t part, int parts, cons
   if (parts == 2) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = w[2 * e] >> 16 | (w[2 * e + 1] & 0xffff0000u);
-    *reinterpret_cast<u4*>(hi + part) = v;
+    *reinterpret_cast<u4*>(hi + core::kPairs) = v;
   }
 }
 
 // ---- second pass: X and X^T = 2^11 u / max(norm, eps), split into halves, zero-padded.  A workgroup: 64 x 64 of the padded matrix as it lies.
-template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void split_kernel(char* work, Momentum mo, float eps, int parts) {
+template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void split_kernel(char* work, Alike alike, Momentum mo, float eps, int parts) {
   __shared__ uint32_t tile[64][65];
   __shared__ double part[4];
-  const Table* t = reinterpret_cast<const Table*>(work);
-  const int k = owner(t, blockIdx.x, &Mat::pack);
-  const Mat mat = t->mat[k];
+  const Place at0 = place_of(work, alike, PACK, blockIdx.x);
+  const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const double* partial = reinterpret_cast<const double*>(work + kTableBytes) + mat.stat;
@@ -194,13 +229,12 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
   const double norm = sqrt((part[0] + part[1]) + (part[2] + part[3]));
   const double scale = (double)kScale / (norm < (double)eps ? (double)eps : norm);      // (a NaN norm stays one)
 
-  const int tiles_c = padded(mat.cols) / 64, id = blockIdx.x - mat.pack;
+  const int tiles_c = padded(mat.cols) / 64, id = at0.id;
   const int r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
   const bool tall = mat.rows > mat.cols;      // then X is the transpose of the matrix as it lies
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
   _Float16* same = arrays + (tall ? r.xt[0] : r.x);
   _Float16* turned = arrays + (tall ? r.x : r.xt[0]);
-  const int64_t mn = (int64_t)r.mp * r.np;
   const int ld_same = padded(mat.cols), ld_turned = padded(mat.rows);
 #pragma unroll
   for (int p = threadIdx.x; p < 512; p += kThreads) {
@@ -225,7 +259,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
       w[e] = row < mat.rows && col + e < mat.cols ? halves((float)((double)v[e] * scale)) : 0u;
       tile[p >> 3][(p & 7) * 8 + e] = w[e];
     }
-    put8(same + (int64_t)row * ld_same + col, mn, parts, w);
+    put8(same, row, col, ld_same, parts, w);
   }
   __syncthreads();
 #pragma unroll
@@ -234,7 +268,7 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
     uint32_t w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = tile[row + e][col];
-    put8(turned + (int64_t)(c0 + col) * ld_turned + r0 + row, mn, parts, w);
+    put8(turned, c0 + col, r0 + row, ld_turned, parts, w);
   }
 }
 
@@ -248,33 +282,30 @@ struct Step {
   int* nan_flags;       // LAST, Muon: one int per matrix, set where the parameter as read holds a NaN
 };
 
-// Tiles: 128 x 128 by four waves of 64 x 64, or 64 x 64 by four of 32 x 32.  PARTS 2: 32 k a stage, PARTS 1: 64.
-template <int TILE, int PARTS>
-using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, true, true, PARTS == 2 ? 64 : 128, TILE == 128 ? 2 : 3>;
+// Tiles: 128 x 128 by four waves of 64 x 64 (two halves: 32 k a stage, two workgroups to a CU), or 64 x 64 by four of 32 x 32.  Else 64 k a stage.
+template <int TILE, int PARTS, int STAGES>
+using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, true, true, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES>;
 
-template <int TILE, int PARTS, int KIND, bool MUON, typename T>
-__global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step st) {
-  using C = Core<TILE, PARTS>;
+template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T>
+__global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike alike, Step st) {
+  using C = Core<TILE, PARTS, STAGES>;
   constexpr int W = TILE / 2, F = W / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const Table* t = reinterpret_cast<const Table*>(work);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr bool kSym = KIND == GRAM || KIND == POLY;
-  const int id0 = core::xcd_order(blockIdx.x, gridDim.x);
-  const int k = __builtin_amdgcn_readfirstlane(owner(t, id0, kSym ? &Mat::sym : &Mat::rect));
-  const Mat& mat = t->mat[k];
+  const Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
-  const int64_t mn = (int64_t)r.mp * r.np, mm = (int64_t)r.mp * r.mp;
   int ti, tj;
   if constexpr (kSym) {      // tile id of the lower triangle: id = ti (ti + 1) / 2 + tj
-    const int id = id0 - mat.sym;
+    const int id = at0.id;
     ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > id) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
     tj = id - ti * (ti + 1) / 2;
   } else {
-    const int id = id0 - mat.rect, tiles_n = (r.np + TILE - 1) / TILE;
+    const int id = at0.id, tiles_n = (r.np + TILE - 1) / TILE;
     ti = id / tiles_n;
     tj = id % tiles_n;
   }
@@ -284,16 +315,16 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
   typename C::SB sb;
   int depth;
   if constexpr (KIND == GRAM) {
-    sa.setup(arrays + r.x, r.np, m0, r.mp, 0, mn, wave, lane);
-    sb.setup(arrays + r.x, r.np, n0, r.mp, 0, mn, wave, lane);
+    sa.setup(arrays + r.x, r.np, m0, r.mp, 0, wave, lane);
+    sb.setup(arrays + r.x, r.np, n0, r.mp, 0, wave, lane);
     depth = r.np;
   } else if constexpr (KIND == POLY) {
-    sa.setup(arrays + r.a, r.mp, m0, r.mp, 0, mm, wave, lane);
-    sb.setup(arrays + r.a, r.mp, n0, r.mp, 0, mm, wave, lane);
+    sa.setup(arrays + r.a, r.mp, m0, r.mp, 0, wave, lane);
+    sb.setup(arrays + r.a, r.mp, n0, r.mp, 0, wave, lane);
     depth = r.mp;
   } else {
-    sa.setup(arrays + r.b, r.mp, m0, r.mp, 0, mm, wave, lane);
-    sb.setup(arrays + (st.from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, mn, wave, lane);
+    sa.setup(arrays + r.b, r.mp, m0, r.mp, 0, wave, lane);
+    sb.setup(arrays + (st.from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, wave, lane);
     depth = r.mp;
   }
   f16v acc[F][F];
@@ -303,6 +334,16 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
     for (int j = 0; j < F; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+  // POLY's own A, requested ahead of the main loop's stream where there are registers for it (small tiles: their time is latency)
+  constexpr bool kAhead = KIND == POLY && F == 1;
+  uint64_t own[kAhead ? 4 : 1][PARTS];
+  if constexpr (kAhead) {
+    const _Float16* a = arrays + r.a + core::pair_at<PARTS>(m0 + (wave >> 1) * W + (lane & 31), n0 + (wave & 1) * W, r.mp) + 4 * (lane >> 5);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) __builtin_memcpy(&own[q][p], a + 8 * q + p * core::kPairs, 8);
+  }
   C::run(sa, sb, depth / C::BK, smem, acc, wave, lane, [](auto&) {});
 
   // lane: row lane & 31 of a 32 x 32 block, register q: column 8 (q / 4) + 4 (lane / 32) + q % 4.  Through LDS, a block at a time and a wave by
@@ -324,10 +365,15 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
         if constexpr (KIND == POLY) {
-          const _Float16* a = arrays + r.a + (int64_t)row * r.mp + col;
           _Float16 hi[4], lo[4];
-          __builtin_memcpy(hi, a, 8);
-          if constexpr (PARTS == 2) __builtin_memcpy(lo, a + mm, 8);
+          if constexpr (kAhead) {
+            __builtin_memcpy(hi, &own[q][0], 8);
+            if constexpr (PARTS == 2) __builtin_memcpy(lo, &own[q][1], 8);
+          } else {
+            const _Float16* a = arrays + r.a + core::pair_at<PARTS>(row, col, r.mp);
+            __builtin_memcpy(hi, a, 8);
+            if constexpr (PARTS == 2) __builtin_memcpy(lo, a + core::kPairs, 8);
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = (float)hi[e];
@@ -346,28 +392,33 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
       if constexpr (KIND == LAST) {
         const bool tall = mat.rows > mat.cols;
         T* out = static_cast<T*>(mat.out);
-#pragma unroll 4
+        // neighbouring lanes: neighbouring columns of the matrix as it lies
+        const int row0 = (tall ? cb : rb) + h, col = (tall ? rb : cb) + li;
+        T* at = out + (int64_t)row0 * mat.cols + col;
+        float p[16];
+        if constexpr (MUON) {      // (all sixteen requests before the first use)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[e] = row0 + 2 * e < mat.rows && col < mat.cols ? at[(int64_t)2 * e * mat.cols] : 0.f;
+        }
+        bool bad = false;
+#pragma unroll
         for (int e = 0; e < 16; ++e) {
-          // neighbouring lanes: neighbouring columns of the matrix as it lies
-          const int major = 2 * e + h, minor = li;
-          const int row = tall ? cb + major : rb + major, col = tall ? rb + minor : cb + minor;
-          if (row < mat.rows && col < mat.cols) {
-            const float o = __builtin_bit_cast(float, tall ? scratch[minor * 33 + major] : scratch[major * 33 + minor]);
-            T* at = out + (int64_t)row * mat.cols + col;
+          const int major = 2 * e + h;
+          const float o = __builtin_bit_cast(float, tall ? scratch[li * 33 + major] : scratch[major * 33 + li]);
+          if (row0 + 2 * e < mat.rows && col < mat.cols) {
             if constexpr (MUON) {
-              const float p = *at;
-              if (st.nan_flags && p != p) st.nan_flags[k] = 1;
-              *at = fmaf(p, st.shrink, -mat.step * o);
+              bad |= p[e] != p[e];
+              at[(int64_t)2 * e * mat.cols] = fmaf(p[e], st.shrink, -mat.step * o);
             } else {
-              *at = (T)o;
+              at[(int64_t)2 * e * mat.cols] = (T)o;
             }
           }
         }
+        if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
       } else {
         // direct and transposed: 32 rows of four pieces, two pieces a lane
         _Float16* direct = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : r.x);
         _Float16* turned = KIND == APPLY ? arrays + (st.from ? r.xt[0] : r.xt[1]) : direct;
-        const int64_t part = kSym ? mm : mn;
         const int ld = kSym ? r.mp : r.np;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -375,7 +426,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
           uint32_t w[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
-          put8(direct + (int64_t)(rb + row) * ld + cb + 8 * c, part, st.parts_out, w);
+          put8(direct, rb + row, cb + 8 * c, ld, st.parts_out, w);
         }
         if (!kSym || ti != tj) {
 #pragma unroll
@@ -384,13 +435,162 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Step s
             uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
-            put8(turned + (int64_t)(cb + row) * r.mp + rb + 8 * c, part, st.parts_out, w);
+            put8(turned, cb + row, rb + 8 * c, r.mp, st.parts_out, w);
           }
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+  }
+}
+
+// ---- few and small matrices: 32 x 32 tiles, the k-steps of a stage dealt to the four waves ------------------------------------------------
+// Four times the workgroups of the 64-wide tiles, a quarter of the work each: the launches of a few 256 x 256 matrices then use the whole chip
+// instead of a quarter of it, and a workgroup's LDS (what the 64-wide tiles wait for: 768 of their 1000 cycles a stage) moves a quarter.  The
+// waves' partial sums meet in LDS, in a fixed order; 128 threads then write the tile, 128 its mirror image.
+constexpr int kSmallStages = 4;
+template <int PARTS> struct Small {
+  using S = core::Stream<_Float16, 32, true, 128, PARTS, 4>;
+  using L = typename S::L;
+  static constexpr int kStage = 2 * PARTS * L::kBytes, kLds = kSmallStages * kStage, kRequests = 2 * PARTS * S::kPer;
+  static_assert(kLds >= 4 * 32 * 36 * 4, "the waves' sums");
+};
+
+template <int N, int REQUESTS> __device__ __forceinline__ void wait_younger(int younger) {
+  if (N == 0 || younger >= N) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N * REQUESTS) : "memory");
+  else wait_younger<(N > 0 ? N - 1 : 0), REQUESTS>(younger);
+}
+
+template <int PARTS, int KIND, bool MUON, typename T>
+__global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike alike, Step st) {
+  using C = Small<PARTS>;
+  using L = typename C::L;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool kSym = KIND == GRAM || KIND == POLY;
+  const Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  const Mat& mat = at0.mat;
+  const Arrays r = arrays_of(mat.rows, mat.cols);
+  _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
+  int ti, tj;
+  if constexpr (kSym) {
+    const int id = at0.id;
+    ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > id) --ti;
+    while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+    tj = id - ti * (ti + 1) / 2;
+  } else {
+    ti = at0.id / (r.np / 32);
+    tj = at0.id - ti * (r.np / 32);
+  }
+  const int m0 = ti * 32, n0 = tj * 32;
+  typename C::S sa, sb;
+  const _Float16* oa = arrays + (KIND == GRAM ? r.x : KIND == POLY ? r.a : r.b);
+  const _Float16* ob = kSym ? oa : arrays + (st.from ? r.xt[1] : r.xt[0]);
+  const int ld = KIND == GRAM ? r.np : r.mp;
+  sa.setup(oa, ld, m0, r.mp, 0, wave, lane);
+  sb.setup(ob, ld, n0, kSym ? r.mp : r.np, 0, wave, lane);
+  const int stages = __builtin_amdgcn_readfirstlane(ld / 64);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+  int put = 0, get = 0;
+  auto fill = [&]() {
+    sa.issue(lds0 + put * C::kStage, wave);
+    sb.issue(lds0 + put * C::kStage + PARTS * L::kBytes, wave);
+    put = put + 1 == kSmallStages ? 0 : put + 1;
+  };
+  f16v acc;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) acc[q] = 0.f;
+  asm volatile("s_nop 4" : : : "memory");      // scalar registers that a vector instruction wrote, read by the assembly text's loads
+  for (int s = 0; s < kSmallStages - 1 && s < stages; ++s) fill();
+  for (int kt = 0; kt < stages; ++kt) {
+    wait_younger<kSmallStages - 2, C::kRequests>(stages - 1 - kt);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    if (kt + kSmallStages - 1 < stages) fill();
+    const char* la = smem + get * C::kStage;
+    const char* lb = la + PARTS * L::kBytes;
+    get = get + 1 == kSmallStages ? 0 : get + 1;
+    u4 fa[PARTS], fb[PARTS];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      fa[q] = L::fragment(la + q * L::kBytes, 0, wave, lane);
+      fb[q] = L::fragment(lb + q * L::kBytes, 0, wave, lane);
+    }
+    if constexpr (PARTS == 2) {
+      acc = core::mma<_Float16>(fb[1], fa[0], acc);
+      acc = core::mma<_Float16>(fb[0], fa[1], acc);
+    }
+    acc = core::mma<_Float16>(fb[0], fa[0], acc);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
+  // sums: [wave][row 32][36]; lane: row lane & 31, register q: column 8 (q / 4) + 4 (lane / 32) + q % 4
+  float* sums = reinterpret_cast<float*>(smem);
+  {
+    float* mine = sums + wave * 32 * 36 + (lane & 31) * 36 + 4 * (lane >> 5);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<f4*>(mine + 8 * q) = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  }
+  __syncthreads();
+  const auto total = [&](int row, int col) {
+    const float* p = sums + row * 36 + col;
+    return (p[0] + p[32 * 36]) + (p[2 * 32 * 36] + p[3 * 32 * 36]);
+  };
+  if constexpr (KIND == LAST) {
+    const bool tall = mat.rows > mat.cols;
+    T* out = static_cast<T*>(mat.out);
+    const int minor = threadIdx.x & 31, major0 = threadIdx.x >> 5;      // neighbouring lanes: neighbouring columns of the matrix as it lies
+    const int row0 = (tall ? n0 : m0) + major0, col = (tall ? m0 : n0) + minor;
+    T* at = out + (int64_t)row0 * mat.cols + col;
+    float p[4];
+    if constexpr (MUON) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = row0 + 8 * e < mat.rows && col < mat.cols ? at[(int64_t)8 * e * mat.cols] : 0.f;
+    }
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int major = major0 + 8 * e;
+      const float o = (tall ? total(minor, major) : total(major, minor)) * (1.f / (kScale * kScale));
+      if (row0 + 8 * e < mat.rows && col < mat.cols) {
+        if constexpr (MUON) {
+          bad |= p[e] != p[e];
+          at[(int64_t)8 * e * mat.cols] = fmaf(p[e], st.shrink, -mat.step * o);
+        } else {
+          at[(int64_t)8 * e * mat.cols] = (T)o;
+        }
+      }
+    }
+    if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
+  } else {
+    const bool mirror = threadIdx.x >= 128;
+    if (mirror && kSym && ti == tj) return;
+    const int row = (threadIdx.x & 127) >> 2, c = (threadIdx.x & 3) * 8;      // of the (mirrored) tile: eight columns of one row
+    const int grow = (mirror ? n0 : m0) + row, gcol = (mirror ? m0 : n0) + c;
+    uint32_t w[8];
+    [[maybe_unused]] _Float16 hi[8], lo[8];
+    if constexpr (KIND == POLY) {      // A is its own mirror image, to a rounding of its sums
+      const _Float16* a = arrays + r.a + core::pair_at<PARTS>(grow, gcol, r.mp);
+      __builtin_memcpy(hi, a, 16);
+      if constexpr (PARTS == 2) __builtin_memcpy(lo, a + core::kPairs, 16);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = mirror ? total(c + e, row) : total(row, c + e);
+      if constexpr (KIND == POLY) {
+        float x = (float)hi[e];
+        if constexpr (PARTS == 2) x += (float)lo[e];
+        v = fmaf(st.c, v * (1.f / kScale), st.b * x) + (grow == gcol + e ? st.a * kScale : 0.f);
+      } else {
+        v *= 1.f / kScale;
+      }
+      w[e] = halves(v);
+    }
+    _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : !mirror ? r.x : st.from ? r.xt[0] : r.xt[1]);
+    put8(to, grow, gcol, kSym || mirror ? r.mp : r.np, st.parts_out, w);
   }
 }
 
@@ -401,28 +601,36 @@ constexpr int kMaxSteps = 100;
 
 struct Layout {
   int tile_sym, tile_rect;
+  int blocks[KINDS];
   int64_t bytes;
 };
 
 inline int64_t tiles(int v, int tile) { return (padded(v) + tile - 1) / tile; }
 
-// Table and workspace of one set of launches.  128-wide tiles where they alone occupy the part's 256 CUs (they read half as much per product),
-// else 64-wide ones: four times the workgroups.
+// Table and workspace of one set of launches.  128-wide tiles where they alone occupy half of the part's 256 CUs (they read half as much per
+// product and their waves twice as little of LDS), else 64-wide ones: four times the workgroups; 32-wide where those are too few as well.
+#ifndef EXP_T32
+#define EXP_T32 128
+#endif
+inline int tile_for(int64_t of128, int64_t of64) { return of128 >= 128 ? 128 : of64 >= EXP_T32 ? 64 : 32; }
+
 inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
-  int64_t sym = 0, rect = 0;
+  int64_t sym[2] = {}, rect[2] = {};
   for (int i = 0; i < count; ++i) {
     const int m = in[i].rows < in[i].cols ? in[i].rows : in[i].cols, n = in[i].rows < in[i].cols ? in[i].cols : in[i].rows;
-    sym += tiles(m, 128) * (tiles(m, 128) + 1) / 2;
-    rect += tiles(m, 128) * tiles(n, 128);
+    for (int k = 0; k < 2; ++k) {
+      const int tile = k ? 64 : 128;
+      sym[k] += tiles(m, tile) * (tiles(m, tile) + 1) / 2;
+      rect[k] += tiles(m, tile) * tiles(n, tile);
+    }
   }
-  l->tile_sym = sym >= 256 ? 128 : 64;
-  l->tile_rect = rect >= 256 ? 128 : 64;
-  int64_t stat = 0, pack = 0, base = 0;
-  sym = rect = 0;
-  t->count = count;
+  l->tile_sym = tile_for(sym[0], sym[1]);
+  l->tile_rect = tile_for(rect[0], rect[1]);
+  int64_t at[KINDS] = {}, base = 0;
+  for (int i = 0; i < kMaxMatrices; ++i)
+    for (int k = 0; k < KINDS; ++k) t->first[k][i] = 0x7fffffff;
   for (int i = 0; i < count; ++i) {
     Mat& m = t->mat[i];
-    m = Mat{};
     m.in = in[i].in;
     m.out = in[i].out;
     m.momentum = in[i].momentum;
@@ -431,26 +639,36 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
     m.step = in[i].step;
     const Arrays r = arrays_of(m.rows, m.cols);
     const int64_t total = elements_of(m), chunk = chunk_of(total), ts = tiles(r.m, l->tile_sym);
-    m.stat = (int)stat;
-    m.pack = (int)pack;
-    m.sym = (int)sym;
-    m.rect = (int)rect;
+    for (int k = 0; k < KINDS; ++k) t->first[k][i] = (int)at[k];
+    m.stat = (int)at[STAT];
     m.base = base;
-    stat += (total + chunk - 1) / chunk;
-    pack += (int64_t)(r.mp / 64) * (r.np / 64);
-    sym += ts * (ts + 1) / 2;
-    rect += tiles(r.m, l->tile_rect) * tiles(r.n, l->tile_rect);
+    at[STAT] += (total + chunk - 1) / chunk;
+    at[PACK] += (int64_t)(r.mp / 64) * (r.np / 64);
+    at[SYM] += ts * (ts + 1) / 2;
+    at[RECT] += tiles(r.m, l->tile_rect) * tiles(r.n, l->tile_rect);
     base += r.total * 2;
-    if (pack > 0x7ffffff0 || sym > 0x7ffffff0) return S2L_E_SIZE;
+    if (at[PACK] > 0x7ffffff0 || at[SYM] > 0x7ffffff0) return S2L_E_SIZE;
   }
-  t->stat_blocks = (int)stat;
-  t->pack_blocks = (int)pack;
-  t->sym_tiles = (int)sym;
-  t->rect_tiles = (int)rect;
-  const int64_t front = kTableBytes + partial_bytes((int)stat);
+  for (int k = 0; k < KINDS; ++k) l->blocks[k] = (int)at[k];
+  const int64_t front = kTableBytes + partial_bytes((int)at[STAT]);
   for (int i = 0; i < count; ++i) t->mat[i].base += front;
   l->bytes = front + base;
   return 0;
+}
+
+inline Alike alike_of(const Table& t, const Layout& l, int count, int size, bool muon) {
+  Alike a{};
+  a.mat = t.mat[0];
+  const int64_t stride = count > 1 ? static_cast<const char*>(t.mat[1].in) - static_cast<const char*>(t.mat[0].in) : 0;
+  if (count > 1 && (muon || stride < 0 || stride > 0x7fffffff / count)) return a;
+  for (int i = 1; i < count; ++i)
+    if (t.mat[i].rows != a.mat.rows || t.mat[i].cols != a.mat.cols || static_cast<const char*>(t.mat[i].in) != static_cast<const char*>(a.mat.in) + i * stride ||
+        static_cast<char*>(t.mat[i].out) != static_cast<char*>(a.mat.out) + i * stride)
+      return a;
+  for (int k = 0; k < KINDS; ++k) a.per[k] = l.blocks[k] / count;
+  a.stride = (int)stride;
+  a.bytes = arrays_of(a.mat.rows, a.mat.cols).total * 2;
+  return a;
 }
 
 // Whether the halves hold every X, A and B of `steps` steps with these coefficients: singular values start at most at 1 (the Frobenius norm) and
@@ -472,49 +690,69 @@ inline bool within_range(double a, double b, double c, int steps) {
   return true;
 }
 
-template <typename K> int launch(K kernel, int blocks, int lds, hipStream_t st, char* work, const Step& s) {
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, st, work, s);
+struct Call {
+  Alike alike;
+  char* work;
+  hipStream_t st;
+  int dev;
+};
+
+template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int one(int blocks, const Call& c, const Step& s) {
+  using C = Core<TILE, PARTS, STAGES>;
+  constexpr int lds = C::kLds > 4 * 32 * 33 * 4 ? C::kLds : 4 * 32 * 33 * 4;
+  const auto kernel = product_kernel<TILE, PARTS, STAGES, KIND, MUON, T>;
+  if constexpr (lds > 65536) {
+    static LdsOptIn opted;
+    const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, opted, c.dev);
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, c.st, c.work, c.alike, s);
   return (int)hipGetLastError();
 }
 
-template <int TILE, int PARTS, int KIND, bool MUON, typename T> int one(int blocks, hipStream_t st, char* work, const Step& s) {
-  constexpr int lds = Core<TILE, PARTS>::kLds > 4 * 32 * 33 * 4 ? Core<TILE, PARTS>::kLds : 4 * 32 * 33 * 4;
-  static_assert(lds <= 65536, "above 64 KiB the launch needs an opt-in");
-  return launch(product_kernel<TILE, PARTS, KIND, MUON, T>, blocks, lds, st, work, s);
+template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, const Call& c, const Step& s) {
+  static_assert(Small<PARTS>::kLds <= 65536, "above 64 KiB the launch needs an opt-in");
+  hipLaunchKernelGGL((small_kernel<PARTS, KIND, MUON, T>), dim3(blocks), dim3(kThreads), Small<PARTS>::kLds, c.st, c.work, c.alike, s);
+  return (int)hipGetLastError();
 }
 
-template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, hipStream_t st, char* work, const Step& s) {
-  if (tile == 128) return parts == 2 ? one<128, 2, KIND, MUON, T>(blocks, st, work, s) : one<128, 1, KIND, MUON, T>(blocks, st, work, s);
-  return parts == 2 ? one<64, 2, KIND, MUON, T>(blocks, st, work, s) : one<64, 1, KIND, MUON, T>(blocks, st, work, s);
+template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, const Call& c, const Step& s) {
+  if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, s) : small<1, KIND, MUON, T>(blocks, c, s);
+  if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, s);
+  return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, s);
 }
 
 template <typename T, bool MUON>
 int run(const s2l_matrix* in, int count, double a, double b, double c, float eps, int steps, Momentum mo, float shrink, int* nan_flags, char* work, hipStream_t st) {
+  int dev, cus;
+  int rc = current_device_cus(&dev, &cus);
+  if (rc) return rc;
   for (int first = 0; first < count; first += kMaxMatrices) {
     const int n = count - first < kMaxMatrices ? count - first : kMaxMatrices;
     Table t;
     Layout l;
-    int rc = lay_out(in + first, n, &t, &l);
+    rc = lay_out(in + first, n, &t, &l);
     if (rc) return rc;
+    const Call call{alike_of(t, l, n, sizeof(T), MUON), work, st, dev};
     const auto parts = [&](int k) { return sizeof(T) == 4 || k < steps - 2 ? 2 : 1; };
-    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(t.stat_blocks), dim3(kThreads), 0, st, t, work, mo);
+    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo);
     rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(t.pack_blocks), dim3(kThreads), 0, st, work, mo, eps, parts(0));
+    hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(l.blocks[PACK]), dim3(kThreads), 0, st, work, call.alike, mo, eps, parts(0));
     rc = (int)hipGetLastError();
     if (rc) return rc;
     for (int k = 0; k < steps; ++k) {
       Step s{(float)a, (float)b, (float)c, k & 1, parts(k), shrink, nan_flags ? nan_flags + first : nullptr};
       // (GRAM, POLY and APPLY do not depend on the matrices' type: one instance)
-      rc = any<GRAM, false, float>(l.tile_sym, parts(k), t.sym_tiles, st, work, s);
+      rc = any<GRAM, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, s);
       if (rc) return rc;
-      rc = any<POLY, false, float>(l.tile_sym, parts(k), t.sym_tiles, st, work, s);
+      rc = any<POLY, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, s);
       if (rc) return rc;
       if (k + 1 < steps) {
         s.parts_out = parts(k + 1);
-        rc = any<APPLY, false, float>(l.tile_rect, parts(k), t.rect_tiles, st, work, s);
+        rc = any<APPLY, false, float>(l.tile_rect, parts(k), l.blocks[RECT], call, s);
       } else {
-        rc = any<LAST, MUON, T>(l.tile_rect, parts(k), t.rect_tiles, st, work, s);
+        rc = any<LAST, MUON, T>(l.tile_rect, parts(k), l.blocks[RECT], call, s);
       }
       if (rc) return rc;
     }

@@ -99,8 +99,15 @@ template <typename T, int ROWS, bool KC, int ROWB> struct Tile {
   }
 };
 
-// The LDS-DMA stream of one operand (`PARTS` equal arrays: an fp32 value's halves, hi then lo).  WAVES waves share a k-tile; a wave's request
-// moves 1 KiB.  Rows (KC) or columns past the end are clamped to valid ones: what they produce is not stored.
+// Where element (row, col) of a matrix of halves pairs lies: 32 hi, then their 32 lo -- one 128-byte line, so that tiles of 32 columns write whole
+// lines and a k-tile's two parts are neighbours.  One part: rows of hi alone.
+constexpr int kPairs = 32;
+template <int PARTS> __host__ __device__ inline int64_t pair_at(int64_t row, int64_t col, int64_t ld) {
+  return PARTS == 1 ? row * ld + col : row * 2 * ld + col / kPairs * (2 * kPairs) + col % kPairs;
+}
+
+// The LDS-DMA stream of one operand (PARTS 2: halves pairs as pair_at lays them).  WAVES waves share a k-tile; a wave's request moves 1 KiB.  Rows
+// (KC) or columns past the end are clamped to valid ones: what they produce is not stored.
 template <typename T, int ROWS, bool KC, int ROWB, int PARTS, int WAVES> struct Stream {
   using L = Tile<T, ROWS, KC, ROWB>;
   static constexpr int kPer = L::kBytes / 1024 / WAVES;      // requests of a wave per part and k-tile
@@ -109,13 +116,14 @@ template <typename T, int ROWS, bool KC, int ROWB, int PARTS, int WAVES> struct 
   uint32_t off[kPer];
   int64_t step;                                              // bytes from one k-tile to the next
 
-  // ld: row stride in elements; row0: first row (KC) / column of the tile; rows: how many there are; k0: first k.  part_stride: elements.
-  // (128 * ld * sizeof(T) < 2^32: the caller checks)
-  __device__ __forceinline__ void setup(const T* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int64_t part_stride, int wave, int lane) {
-    const T* origin = KC ? p + row0 * ld + k0 : p + k0 * ld + row0;
-    step = uniform64((KC ? (int64_t)L::BK : (int64_t)L::BK * ld) * (int64_t)sizeof(T));
+  // ld: row stride in elements (of one part); row0: first row (KC) / column of the tile; rows: how many there are; k0: first k.
+  // (PARTS * 128 * ld * sizeof(T) < 2^32: the caller checks)
+  __device__ __forceinline__ void setup(const T* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int wave, int lane) {
+    static_assert(PARTS == 1 || KC, "");
+    const T* origin = KC ? p + pair_at<PARTS>(row0, k0, ld) : p + k0 * ld + row0;
+    step = uniform64((KC ? (int64_t)L::BK * PARTS : (int64_t)L::BK * ld) * (int64_t)sizeof(T));
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) base[q] = uniform64(reinterpret_cast<const char*>(origin + q * part_stride));
+    for (int q = 0; q < PARTS; ++q) base[q] = uniform64(reinterpret_cast<const char*>(origin + q * kPairs));
     const int64_t left = rows - row0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -124,7 +132,7 @@ template <typename T, int ROWS, bool KC, int ROWB, int PARTS, int WAVES> struct 
       int piece = L::swizzle(line, at % L::kLine / 16);
       if constexpr (KC) line = line < left ? line : (int)left - 1;
       else piece = (piece + 1) * L::C <= left ? piece : 0;
-      off[j] = (uint32_t)(line * ld * (int64_t)sizeof(T)) + piece * 16;
+      off[j] = (uint32_t)(line * ld * PARTS * (int64_t)sizeof(T)) + (PARTS == 2 ? (piece >> 2) * 128 + (piece & 3) * 16 : piece * 16);
     }
   }
   __device__ __forceinline__ void issue(uint32_t lds, int wave) {      // the next k-tile, to LDS at `lds`
@@ -154,10 +162,19 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool 
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
   }
 
+  // at most N younger k-tiles in flight, fewer at the end
+  template <int N> __device__ __forceinline__ static void wait_younger(int younger) {
+    static_assert(N * kRequests < 64, "the counter's range");
+    if constexpr (N == 0) wait<0>();
+    else if (younger >= N) wait<N * kRequests>();
+    else wait_younger<N - 1>(younger);
+  }
+
   // acc += over k-tiles [0, tiles).  `each(fa)` sees every k-step's A fragments (PARTS == 1).
   template <typename Each>
-  __device__ __forceinline__ static void run(SA& a, SB& b, int tiles, char* smem, f16v (&acc)[FM][FN], int wave, int lane, Each&& each) {
+  __device__ __forceinline__ static void run(SA& a, SB& b, int count, char* smem, f16v (&acc)[FM][FN], int wave, int lane, Each&& each) {
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
+    const int tiles = __builtin_amdgcn_readfirstlane(count);
     const int uwave = __builtin_amdgcn_readfirstlane(wave);
     const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
     int put = 0, get = 0;      // stage to fill, stage to use
@@ -170,41 +187,51 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool 
     for (int s = 0; s < STAGES - 1 && s < tiles; ++s) fill();
     for (int kt = 0; kt < tiles; ++kt) {
       // k-tile kt has landed when at most the younger ones' requests are outstanding (loads retire in order)
-      const int younger = tiles - 1 - kt;
-      if (STAGES >= 4 && younger >= 2) wait<2 * kRequests>();
-      else if (STAGES >= 3 && younger >= 1) wait<kRequests>();
-      else wait<0>();
+      wait_younger<STAGES - 2>(tiles - 1 - kt);
       __builtin_amdgcn_s_barrier();      // everybody's part of k-tile kt is in LDS; everybody has left k-tile kt - 1, whose stage is filled next
       asm volatile("" : : : "memory");
       if (kt + STAGES - 1 < tiles) fill();
       const char* la = smem + get * kStage;
       const char* lb = la + PARTS * LA::kBytes;
       get = get + 1 == STAGES ? 0 : get + 1;
+      // the fragments of a k-step are read while the matrix cores work on the step before (left to itself the compiler reads them right
+      // before their use, and every step waits out the LDS latency)
+      u4 fa[2][PARTS][FM], fb[2][PARTS][FN];
+      auto fetch = [&](int s) {
+#pragma unroll
+        for (int q = PARTS - 1; q >= 0; --q) {
+#pragma unroll
+          for (int j = 0; j < FN; ++j) fb[s & 1][q][j] = LB::fragment(lb + q * LB::kBytes, wn + 32 * j, s, lane);
+#pragma unroll
+          for (int i = 0; i < FM; ++i) fa[s & 1][PARTS - 1 - q][i] = LA::fragment(la + (PARTS - 1 - q) * LA::kBytes, wm + 32 * i, s, lane);
+        }
+      };
+      constexpr bool kPin = FM * FN == 1;
+      fetch(0);
 #pragma unroll
       for (int s = 0; s < ROWB / 32; ++s) {
-        u4 fa[PARTS][FM], fb[PARTS][FN];
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-#pragma unroll
-          for (int i = 0; i < FM; ++i) fa[q][i] = LA::fragment(la + q * LA::kBytes, wm + 32 * i, s, lane);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) fb[q][j] = LB::fragment(lb + q * LB::kBytes, wn + 32 * j, s, lane);
+        if (s + 1 < ROWB / 32) {
+          fetch(s + 1);
+          if (kPin) __builtin_amdgcn_sched_barrier(0);
         }
+        const auto& a0 = fa[s & 1];
+        const auto& b0 = fb[s & 1];
         if constexpr (PARTS == 2) {      // the small products first
 #pragma unroll
           for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[1][j], fa[0][i], acc[i][j]);
+            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(b0[1][j], a0[0][i], acc[i][j]);
 #pragma unroll
           for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[0][j], fa[1][i], acc[i][j]);
+            for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(b0[0][j], a0[1][i], acc[i][j]);
         }
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(fb[0][j], fa[0][i], acc[i][j]);
-        each(fa);
+          for (int j = 0; j < FN; ++j) acc[i][j] = mma<T>(b0[0][j], a0[0][i], acc[i][j]);
+        each(a0);
+        if (kPin && s + 1 < ROWB / 32) __builtin_amdgcn_sched_barrier(0);
       }
     }
     wait<0>();
