@@ -13,10 +13,11 @@
 // Values are scaled by 2^11: |X| <= ||X||_2 <= 1.2 and the entries of A and B <= 3.5 use the range of the halves from 2^-24 to 7168.
 //
 // All matrices of a call go through the same 2 + 3 * steps launches: one pass for the Frobenius norms (with the momentum update), one that scales
-// and splits into X and X^T, then per step the Gram product (symmetric: tiles on and below the diagonal, written twice), the polynomial (the
-// same, its epilogue adds a I + b A), and X <- B X, which leaves X and X^T for the next step's two products -- both operands of every product
-// are then contiguous in k -- or, last, writes the result: the rounded output, or the parameter's update.  Matrices lie zero-padded to multiples
-// of 64 in the workspace, so that the products' main loop has no edges.
+// and splits into X^T, then per step the Gram product (symmetric: tiles on and below the diagonal, written twice), the polynomial (the same, its
+// epilogue adds a I + b A), and X <- B X, which leaves X^T or, last, writes the result: the rounded output, or the parameter's update.  X is held
+// transposed only: X <- B X reads it with k contiguous, the Gram product along its rows, through the transposing LDS read (X beside it cost
+// twice the stores: four 2048 x 2048 206 against 186 us a product, and what a launch leaves in L2 is written back before the next one starts).
+// Matrices lie zero-padded to multiples of 64 in the workspace, so that the products' main loop has no edges.
 #include <cmath>
 
 #include "tile_core.h"
@@ -61,7 +62,7 @@ __host__ __device__ inline int64_t chunk_of(int64_t elements) {      // elements
 // the arrays of one matrix, in halves from its base: each has room for pairs (core::pair_at); in steps on hi alone it holds rows of those
 struct Arrays {
   int m, n, mp, np;
-  int64_t x, xt[2], a, b, total;
+  int64_t xt[2], a, b, total;
 };
 __host__ __device__ inline Arrays arrays_of(int rows, int cols) {
   Arrays r;
@@ -70,10 +71,9 @@ __host__ __device__ inline Arrays arrays_of(int rows, int cols) {
   r.mp = padded(r.m);
   r.np = padded(r.n);
   const int64_t mn = (int64_t)r.mp * r.np, mm = (int64_t)r.mp * r.mp;
-  r.x = 0;
-  r.xt[0] = 2 * mn;
-  r.xt[1] = 4 * mn;
-  r.a = 6 * mn;
+  r.xt[0] = 0;
+  r.xt[1] = 2 * mn;
+  r.a = 4 * mn;
   r.b = r.a + 2 * mm;
   r.total = r.b + 2 * mm;
   return r;
@@ -231,11 +231,9 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
 
   const int tiles_c = padded(mat.cols) / 64, id = at0.id;
   const int r0 = id / tiles_c * 64, c0 = id % tiles_c * 64;
-  const bool tall = mat.rows > mat.cols;      // then X is the transpose of the matrix as it lies
-  _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
-  _Float16* same = arrays + (tall ? r.xt[0] : r.x);
-  _Float16* turned = arrays + (tall ? r.x : r.xt[0]);
-  const int ld_same = padded(mat.cols), ld_turned = padded(mat.rows);
+  // X^T has the longer side's length in rows: the matrix as it lies where that is tall, else turned through LDS
+  const bool tall = mat.rows > mat.cols;
+  _Float16* xt = reinterpret_cast<_Float16*>(work + mat.base) + r.xt[0];
 #pragma unroll
   for (int p = threadIdx.x; p < 512; p += kThreads) {
     const int row = r0 + (p >> 3), col = c0 + (p & 7) * 8;
@@ -255,20 +253,23 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
     }
     uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = row < mat.rows && col + e < mat.cols ? halves((float)((double)v[e] * scale)) : 0u;
-      tile[p >> 3][(p & 7) * 8 + e] = w[e];
+    for (int e = 0; e < 8; ++e) w[e] = row < mat.rows && col + e < mat.cols ? halves((float)((double)v[e] * scale)) : 0u;
+    if (tall) {
+      put8(xt, row, col, r.mp, parts, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tile[p >> 3][(p & 7) * 8 + e] = w[e];
     }
-    put8(same, row, col, ld_same, parts, w);
   }
+  if (tall) return;
   __syncthreads();
 #pragma unroll
-  for (int p = threadIdx.x; p < 512; p += kThreads) {
-    const int col = p & 63, row = (p >> 6) * 8;
+  for (int p = threadIdx.x; p < 512; p += kThreads) {      // neighbouring lanes: neighbouring pieces of a row of X^T
+    const int col = p >> 3, row = (p & 7) * 8;
     uint32_t w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = tile[row + e][col];
-    put8(turned, c0 + col, r0 + row, ld_turned, parts, w);
+    put8(xt, c0 + col, r0 + row, r.mp, parts, w);
   }
 }
 
@@ -283,12 +284,12 @@ struct Step {
 };
 
 // Tiles: 128 x 128 by four waves of 64 x 64 (two halves: 32 k a stage, two workgroups to a CU), or 64 x 64 by four of 32 x 32.  Else 64 k a stage.
-template <int TILE, int PARTS, int STAGES>
-using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, true, true, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES>;
+template <int TILE, int PARTS, int STAGES, int KIND>
+using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, KIND != GRAM, KIND != GRAM, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES>;
 
 template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T>
 __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike alike, Step st) {
-  using C = Core<TILE, PARTS, STAGES>;
+  using C = Core<TILE, PARTS, STAGES, KIND>;
   constexpr int W = TILE / 2, F = W / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -315,8 +316,9 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
   typename C::SB sb;
   int depth;
   if constexpr (KIND == GRAM) {
-    sa.setup(arrays + r.x, r.np, m0, r.mp, 0, wave, lane);
-    sb.setup(arrays + r.x, r.np, n0, r.mp, 0, wave, lane);
+    const _Float16* xt = arrays + (st.from ? r.xt[1] : r.xt[0]);
+    sa.setup(xt, r.mp, m0, r.mp, 0, wave, lane);
+    sb.setup(xt, r.mp, n0, r.mp, 0, wave, lane);
     depth = r.np;
   } else if constexpr (KIND == POLY) {
     sa.setup(arrays + r.a, r.mp, m0, r.mp, 0, wave, lane);
@@ -416,17 +418,15 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
         }
         if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
       } else {
-        // direct and transposed: 32 rows of four pieces, two pieces a lane
-        _Float16* direct = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : r.x);
-        _Float16* turned = KIND == APPLY ? arrays + (st.from ? r.xt[0] : r.xt[1]) : direct;
-        const int ld = kSym ? r.mp : r.np;
+        // 32 rows of four pieces, two pieces a lane: the symmetric ones as they are and mirrored, X^T mirrored
+        _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : st.from ? r.xt[0] : r.xt[1]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; kSym && e < 2; ++e) {
           const int row = (lane >> 2) + 16 * e, c = lane & 3;
           uint32_t w[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
-          put8(direct, rb + row, cb + 8 * c, ld, st.parts_out, w);
+          put8(to, rb + row, cb + 8 * c, r.mp, st.parts_out, w);
         }
         if (!kSym || ti != tj) {
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
             uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
-            put8(turned, cb + row, rb + 8 * c, r.mp, st.parts_out, w);
+            put8(to, cb + row, rb + 8 * c, r.mp, st.parts_out, w);
           }
         }
       }
@@ -450,8 +450,8 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
 // instead of a quarter of it, and a workgroup's LDS (what the 64-wide tiles wait for: 768 of their 1000 cycles a stage) moves a quarter.  The
 // waves' partial sums meet in LDS, in a fixed order; 128 threads then write the tile, 128 its mirror image.
 constexpr int kSmallStages = 4;
-template <int PARTS> struct Small {
-  using S = core::Stream<_Float16, 32, true, 128, PARTS, 4>;
+template <int PARTS, int KIND> struct Small {
+  using S = core::Stream<_Float16, 32, KIND != GRAM, 128, PARTS, 4>;
   using L = typename S::L;
   static constexpr int kStage = 2 * PARTS * L::kBytes, kLds = kSmallStages * kStage, kRequests = 2 * PARTS * S::kPer;
   static_assert(kLds >= 4 * 32 * 36 * 4, "the waves' sums");
@@ -464,7 +464,7 @@ template <int N, int REQUESTS> __device__ __forceinline__ void wait_younger(int 
 
 template <int PARTS, int KIND, bool MUON, typename T>
 __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike alike, Step st) {
-  using C = Small<PARTS>;
+  using C = Small<PARTS, KIND>;
   using L = typename C::L;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,12 +486,10 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
   }
   const int m0 = ti * 32, n0 = tj * 32;
   typename C::S sa, sb;
-  const _Float16* oa = arrays + (KIND == GRAM ? r.x : KIND == POLY ? r.a : r.b);
-  const _Float16* ob = kSym ? oa : arrays + (st.from ? r.xt[1] : r.xt[0]);
-  const int ld = KIND == GRAM ? r.np : r.mp;
-  sa.setup(oa, ld, m0, r.mp, 0, wave, lane);
-  sb.setup(ob, ld, n0, kSym ? r.mp : r.np, 0, wave, lane);
-  const int stages = __builtin_amdgcn_readfirstlane(ld / 64);
+  const _Float16* xt = arrays + (st.from ? r.xt[1] : r.xt[0]);
+  sa.setup(KIND == GRAM ? xt : KIND == POLY ? arrays + r.a : arrays + r.b, r.mp, m0, r.mp, 0, wave, lane);
+  sb.setup(KIND == POLY ? arrays + r.a : xt, r.mp, n0, kSym ? r.mp : r.np, 0, wave, lane);
+  const int stages = __builtin_amdgcn_readfirstlane((KIND == GRAM ? r.np : r.mp) / 64);
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
   int put = 0, get = 0;
   auto fill = [&]() {
@@ -566,8 +564,8 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
     }
     if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
   } else {
-    const bool mirror = threadIdx.x >= 128;
-    if (mirror && kSym && ti == tj) return;
+    const bool mirror = KIND == APPLY || threadIdx.x >= 128;      // X^T is written mirrored only
+    if (KIND == APPLY ? threadIdx.x >= 128 : mirror && ti == tj) return;
     const int row = (threadIdx.x & 127) >> 2, c = (threadIdx.x & 3) * 8;      // of the (mirrored) tile: eight columns of one row
     const int grow = (mirror ? n0 : m0) + row, gcol = (mirror ? m0 : n0) + c;
     uint32_t w[8];
@@ -589,8 +587,7 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
       }
       w[e] = halves(v);
     }
-    _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : !mirror ? r.x : st.from ? r.xt[0] : r.xt[1]);
-    put8(to, grow, gcol, kSym || mirror ? r.mp : r.np, st.parts_out, w);
+    put8(arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : st.from ? r.xt[0] : r.xt[1]), grow, gcol, r.mp, st.parts_out, w);
   }
 }
 
@@ -698,7 +695,7 @@ struct Call {
 };
 
 template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int one(int blocks, const Call& c, const Step& s) {
-  using C = Core<TILE, PARTS, STAGES>;
+  using C = Core<TILE, PARTS, STAGES, KIND>;
   constexpr int lds = C::kLds > 4 * 32 * 33 * 4 ? C::kLds : 4 * 32 * 33 * 4;
   const auto kernel = product_kernel<TILE, PARTS, STAGES, KIND, MUON, T>;
   if constexpr (lds > 65536) {
@@ -711,8 +708,9 @@ template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int 
 }
 
 template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, const Call& c, const Step& s) {
-  static_assert(Small<PARTS>::kLds <= 65536, "above 64 KiB the launch needs an opt-in");
-  hipLaunchKernelGGL((small_kernel<PARTS, KIND, MUON, T>), dim3(blocks), dim3(kThreads), Small<PARTS>::kLds, c.st, c.work, c.alike, s);
+  constexpr int lds = Small<PARTS, KIND>::kLds;
+  static_assert(lds <= 65536, "above 64 KiB the launch needs an opt-in");
+  hipLaunchKernelGGL((small_kernel<PARTS, KIND, MUON, T>), dim3(blocks), dim3(kThreads), lds, c.st, c.work, c.alike, s);
   return (int)hipGetLastError();
 }
 

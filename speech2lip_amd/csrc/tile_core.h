@@ -119,9 +119,8 @@ template <typename T, int ROWS, bool KC, int ROWB, int PARTS, int WAVES> struct 
   // ld: row stride in elements (of one part); row0: first row (KC) / column of the tile; rows: how many there are; k0: first k.
   // (PARTS * 128 * ld * sizeof(T) < 2^32: the caller checks)
   __device__ __forceinline__ void setup(const T* p, int64_t ld, int64_t row0, int64_t rows, int64_t k0, int wave, int lane) {
-    static_assert(PARTS == 1 || KC, "");
-    const T* origin = KC ? p + pair_at<PARTS>(row0, k0, ld) : p + k0 * ld + row0;
-    step = uniform64((KC ? (int64_t)L::BK * PARTS : (int64_t)L::BK * ld) * (int64_t)sizeof(T));
+    const T* origin = p + (KC ? pair_at<PARTS>(row0, k0, ld) : pair_at<PARTS>(k0, row0, ld));
+    step = uniform64((KC ? (int64_t)L::BK : (int64_t)L::BK * ld) * PARTS * (int64_t)sizeof(T));
 #pragma unroll
     for (int q = 0; q < PARTS; ++q) base[q] = uniform64(reinterpret_cast<const char*>(origin + q * kPairs));
     const int64_t left = rows - row0;
