@@ -13,7 +13,8 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libs2l_hip.so")
 REF_LIB = os.path.join(PKG, "libs2l_hip_ref.so")      # the same ABI + the non-default kernel forms (-DS2L_WITH_REFERENCE_KERNELS): tests / tools only
 RESOURCES = os.path.join(PKG, "kernel_resources.json")      # per-kernel registers / spills / scratch / LDS of the last build
-SOURCES = ["pack.hip", "frontend.hip", "rows.hip", "render.hip", "ensemble.hip", "train.hip", "composite.hip", "unet.hip", "warp.hip", "syncnet.hip", "lpips.hip", "syncchain.hip", "train_bf16.hip", "quant.hip", "render16.hip", "convh.hip", "linear.hip", "orthogonalize.hip"]
+SOURCES = ["pack.hip", "frontend.hip", "rows.hip", "render.hip", "ensemble.hip", "train.hip", "composite.hip", "unet.hip", "warp.hip", "syncnet.hip", "lpips.hip", "syncchain.hip", "train_bf16.hip", "quant.hip", "render16.hip", "convh.hip",
+           "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "orthogonalize.hip"]
 # translation units that differ in the reference library: the split convolution's generated-assembly form (conv16.hip, its dispatch in
 # unet.hip) and the four-wave / alternating-roles forms of the half-width convolution (convh.hip).  Every other object is shared.
 REF_SOURCES = ["unet.hip", "convh.hip", "conv16.hip"]
@@ -23,7 +24,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 # without packed fp32 instructions (v_pk_add / mul / fma_f32), whose generated forms are not relied on here; the sources that are not listed hold
 # such instructions in their own assembly text and are compiled as they were measured
 SCALAR_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"linear.hip": SCALAR_FP32, "orthogonalize.hip": SCALAR_FP32}
+SOURCE_FLAGS = {s: SCALAR_FP32 for s in SOURCES if s.startswith(("linear", "orthogonalize"))}
 _REMARK = re.compile(r"remark:\s+(Function Name|VGPRs|AGPRs|ScratchSize \[bytes/lane\]|SGPRs Spill|VGPRs Spill|LDS Size \[bytes/block\]|"
                      r"Occupancy \[waves/SIMD\]):\s*(\S+)")
 

@@ -1,670 +1,16 @@
-// A dense layer of any size with its epilogue, and its gradients:
-//
-//   z = x W^T + b     y = act(z) + residual                          x [rows, in], W [out, in], y [rows, out]
-//   dz = dy * act'(z)     dx = dz W     dW = dz^T x     db = sum over rows of dz     (d residual = dy)
-//
-// in fp32 (fp32 MFMA), bf16 or f16 (16-bit MFMA), all sums in fp32, one rounding at each store.  What is kept between the passes: for the
-// kinked activations one BIT per element, the exact sign of the fp32 z (so that the gradient's side of the kink never depends on how z would
-// round), for the smooth ones z in the call's own type (its relative rounding 2^-9 / 2^-12 moves act' by |z act''| times that, below the
-// rounding of the gradient itself).
-//
-// One tile kernel serves the three products.  An operand whose contraction index is contiguous in memory (KC: x and W of the forward, dz of
-// dx) lies in LDS as [row][128 bytes of k] with its 16-byte pieces XOR-swizzled by the row; one whose contraction index is the row (W of dx,
-// both operands of dW) lies as it comes, [k][columns], and is transposed on the way out of LDS (the 16-bit types by the transposing LDS
-// read, fp32 by 4-byte reads).  Global memory is read as 16-byte pieces at element alignment into registers one k-tile ahead, so odd widths
-// and row strides take the same path; only tiles at an edge check bounds.  The bit gate of a kinked activation is applied between register
-// and LDS, which saves the pass that would write dz.  v_mfma_f32_32x32x* throughout, with the operands swapped so that a lane holds four
-// consecutive columns of ONE output row.
-#include <type_traits>
-
-#include "s2l_common.h"
+// The C entries of the dense layer.  linear.h holds the mathematics and the kernels; each type's are compiled in a translation unit of its own.
+#include "linear.h"
 
 namespace s2l {
 namespace lin {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-
-constexpr int kThreads = 256;
-constexpr int kBkBytes = 128;               // bytes of contraction per LDS row and k-tile: 64 16-bit values or 32 floats
-constexpr int kSkinnyRows = 8;              // up to this many rows the forward is one pass over W (skinny_kernel)
-
-struct Args {
-  const void* a;        // KC: [m][k]; else [k][m]
-  const void* b;        // KC: [n][k]; else [k][n]
-  const uint8_t* gate;  // sign bits of z, laid over operand a's memory layout: byte (row * gate_ld + column / 8)
-  int64_t lda, ldb, gate_ld;
-  int64_t m, n, k;
-  int64_t k_per_split;  // multiple of the k-tile; grid.y splits
-  float slope;          // gate: factor where the bit is 0
-  // epilogue
-  const void* bias;
-  const void* residual;
-  void* out;
-  uint8_t* bits;        // forward: sign bits out, row stride ceil(n/8)
-  void* zsave;          // forward: z out, row stride n
-  float* partial;       // != NULL: [split][m][n] fp32 instead of the epilogue
-  float* colsum;        // wgrad: [split][m] sums of operand a over k (the bias gradient), written by the first column of tiles
-  int64_t ldr, ldo;
-  int act;
-};
-
-template <typename T> struct Traits;
-template <> struct Traits<float> { static constexpr int kChunk = 4; };
-template <> struct Traits<_Float16> { static constexpr int kChunk = 8; };
-template <> struct Traits<__bf16> { static constexpr int kChunk = 8; };
-
-template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
-
-// 16 bytes at element alignment: the target's unaligned global access makes this one load
-template <typename T> __device__ __forceinline__ u4 load16(const T* p) { u4 v; __builtin_memcpy(&v, p, 16); return v; }
-template <typename T> __device__ __forceinline__ void store16(T* p, u4 v) { __builtin_memcpy(p, &v, 16); }
-
-// the first `count` (< a piece) elements, the rest zero
-template <typename T> __device__ __forceinline__ u4 load_some(const T* p, int count) {
-  union { u4 v; T e[Traits<T>::kChunk]; } r;
-  r.v = u4{0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < Traits<T>::kChunk; ++i)
-    if (i < count) r.e[i] = p[i];
-  return r.v;
-}
-
-__device__ __forceinline__ float act_of(float z, int act, float slope) {
-  switch (act) {
-    case S2L_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-    case S2L_ACT_LEAKY_RELU: return z > 0.f ? z : z * slope;
-    case S2L_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case S2L_ACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
-  }
-}
-
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == S2L_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-  const float s = 1.f / (1.f + expf(-z));      // silu; z -> -inf: s = 0 and z s = 0 (z (1 - s) s with s = 0 is 0 for every finite z)
-  return s * (1.f + z * (1.f - s));
-}
-
-// ---- epilogue of one piece: eight consecutive columns (a byte of sign bits) of one row --------------------------------------------------
-constexpr int kFinish = 8;
-template <typename T> struct Eight { T e[kFinish]; };
-template <typename T> __device__ __forceinline__ Eight<T> load8(const T* p, bool full, int count) {
-  Eight<T> v;
-  if (full) {
-    __builtin_memcpy(&v, p, sizeof(v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i) v.e[i] = i < count ? p[i] : (T)0.f;
-  }
-  return v;
-}
-template <typename T> __device__ __forceinline__ void store8(T* p, const Eight<T>& v, bool full, int count) {
-  if (full) {
-    __builtin_memcpy(p, &v, sizeof(v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i)
-      if (i < count) p[i] = v.e[i];
-  }
-}
-
-// z as the backward pass reads it: a 16-bit type's largest value in place of an overflow (act' has long settled there, and no inf * 0 comes of it)
-template <typename T> __device__ __forceinline__ T saved_z(float z) {
-  if constexpr (std::is_same_v<T, _Float16>) z = z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z;
-  if constexpr (std::is_same_v<T, __bf16>) z = z > 3.3895313892515355e38f ? 3.3895313892515355e38f : z < -3.3895313892515355e38f ? -3.3895313892515355e38f : z;
-  return from_f<T>(z);
-}
-
-template <typename T> __device__ __forceinline__ void finish_piece(const Args& g, int64_t row, int64_t col, const float* acc) {
-  const bool full = col + kFinish <= g.n;
-  const int count = full ? kFinish : (int)(g.n - col);
-  const T* bias = static_cast<const T*>(g.bias);
-  const T* res = static_cast<const T*>(g.residual);
-  float z[kFinish];
-#pragma unroll
-  for (int i = 0; i < kFinish; ++i) z[i] = acc[i];
-  if (bias) {
-    const Eight<T> b = load8(bias + col, full, count);
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i) z[i] += (float)b.e[i];
-  }
-  if (g.bits) {      // the side of the kink, from the fp32 z
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i) m |= z[i] > 0.f ? 1u << i : 0u;
-    g.bits[row * ((g.n + 7) >> 3) + (col >> 3)] = (uint8_t)m;
-  }
-  if (g.zsave) {
-    Eight<T> s;
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i) s.e[i] = saved_z<T>(z[i]);
-    store8(static_cast<T*>(g.zsave) + row * g.n + col, s, full, count);
-  }
-  Eight<T> r, o;
-  if (res) r = load8(res + row * g.ldr + col, full, count);
-#pragma unroll
-  for (int i = 0; i < kFinish; ++i) z[i] = act_of(z[i], g.act, g.slope);
-  if (res) {
-#pragma unroll
-    for (int i = 0; i < kFinish; ++i) z[i] += (float)r.e[i];
-  }
-#pragma unroll
-  for (int i = 0; i < kFinish; ++i) o.e[i] = from_f<T>(z[i]);
-  store8(static_cast<T*>(g.out) + row * g.ldo + col, o, full, count);
-}
-
-// ---- one operand's k-tile: global -> registers -> LDS -> MFMA fragments ----------------------------------------------------------------
-// ROWS output rows (or columns) x kBkBytes of k.  KC: LDS [row][8 pieces], piece c of row r at c ^ (r & 7).  Not KC: LDS [k][ROWS elements];
-// 16-bit: the 32-byte blocks of a k-row at block ^ ((k & 3) | (k >> 3 & 1) << 2), which spreads the eight k-rows that one transposing read
-// touches over all banks (a 64-row tile has four blocks: the top bit drops out, two k-rows share banks).
-template <typename T, int ROWS, bool KC, bool GATE> struct Operand {
-  static constexpr int C = Traits<T>::kChunk;
-  static constexpr int BK = kBkBytes / (int)sizeof(T);
-  static constexpr int kPieces = ROWS * 8 / kThreads;                     // per thread
-  static constexpr int kRowPieces = KC ? 8 : ROWS / C;                    // pieces per LDS row
-  static constexpr int kBytes = ROWS * kBkBytes;
-  static constexpr int kBlockMask = ROWS * (int)sizeof(T) / 32 - 1;
-  u4 r[kPieces];
-  uint32_t gate[GATE ? kPieces : 1];
-
-  __device__ __forceinline__ static int place(int line, int piece) {      // byte offset of a piece in LDS
-    if constexpr (KC) return line * kBkBytes + ((piece ^ (line & 7)) << 4);
-    else if constexpr (sizeof(T) == 2) return line * ROWS * 2 + (((((piece >> 1) ^ ((line & 3) | ((line >> 1) & 4))) & kBlockMask) << 5) | ((piece & 1) << 4));
-    else return line * ROWS * 4 + (piece << 4);
-  }
-
-  // base: the operand; row0 / k0: origin of the tile; rows / k_end: ends
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t k0, int64_t rows, int64_t k_end, const uint8_t* gates,
-                                       int64_t gate_ld) {
-    const int64_t line0 = KC ? row0 : k0, col0 = KC ? k0 : row0;
-    const int64_t lines = KC ? rows : k_end, cols = KC ? k_end : rows;
-    constexpr int kLines = KC ? ROWS : BK;
-    const bool inside = line0 + kLines <= lines && col0 + kRowPieces * C <= cols;      // uniform: the whole tile
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = threadIdx.x + i * kThreads;
-      const int64_t line = line0 + p / kRowPieces, col = col0 + (p % kRowPieces) * C;
-      if (inside) {
-        r[i] = load16(base + line * ld + col);
-        if constexpr (GATE) gate[i] = gates[line * gate_ld + (col >> 3)];
-      } else {
-        r[i] = u4{0, 0, 0, 0};
-        if constexpr (GATE) gate[i] = 0;
-        if (line < lines && col < cols) {
-          r[i] = col + C <= cols ? load16(base + line * ld + col) : load_some(base + line * ld + col, (int)(cols - col));
-          if constexpr (GATE) gate[i] = gates[line * gate_ld + (col >> 3)];
-        }
-      }
-      if constexpr (GATE && C == 4) gate[i] >>= (col & 4);
-    }
-  }
-
-  __device__ __forceinline__ void commit(char* lds, float slope) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int p = threadIdx.x + i * kThreads;
-      u4 v = r[i];
-      if constexpr (GATE) {
-        union { u4 v; T e[C]; } x;
-        x.v = v;
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (!((gate[i] >> j) & 1)) x.e[j] = slope == 0.f ? (T)0.f : from_f<T>((float)x.e[j] * slope);
-        v = x.v;
-      }
-      *reinterpret_cast<u4*>(lds + place(p / kRowPieces, p % kRowPieces)) = v;
-    }
-  }
-
-  // 16 bytes of fragment for k-step s (32 bytes of k): rows row .. row + 31; the half-wave h holds the h-th 16 bytes
-  __device__ __forceinline__ static u4 fragment(const char* lds, int row, int s, int lane) {
-    const int h = lane >> 5;
-    if constexpr (KC) {
-      return *reinterpret_cast<const u4*>(lds + place(row + (lane & 31), 2 * s + h));
-    } else if constexpr (sizeof(T) == 2) {
-      // each 16-lane group reads a [4 k][16 columns] block; lane i of it passes the address of k-row i / 4, columns 4 (i % 4) .. and
-      // receives column i of the four k-rows
-      const int i = lane & 15, col = row + (lane & 16) + 4 * (i & 3), k = 16 * s + 8 * h + (i >> 2);
-      typedef __attribute__((address_space(3))) s4* lds_s4;
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + place(k, col >> 3) + ((col & 4) << 1)));
-      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(lds + place(k + 4, col >> 3) + ((col & 4) << 1)));
-      union { s4 a[2]; u4 v; } x;
-      x.a[0] = lo;
-      x.a[1] = hi;
-      return x.v;
-    } else {
-      union { float f[4]; u4 v; } x;
-      const float* p = reinterpret_cast<const float*>(lds) + (8 * s + 4 * h) * ROWS + row + (lane & 31);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x.f[j] = p[j * ROWS];
-      return x.v;
-    }
-  }
-};
-
-template <typename T> __device__ __forceinline__ f16v mma(u4 a, u4 b, f16v c) {
-  if constexpr (std::is_same_v<T, float>) {
-    union { u4 v; float f[4]; } x, y;
-    x.v = a;
-    y.v = b;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.f[j], y.f[j], c, 0, 0, 0);
-    return c;
-  } else if constexpr (std::is_same_v<T, _Float16>) {
-    union { u4 v; h8 h; } x, y;
-    x.v = a;
-    y.v = b;
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, y.h, c, 0, 0, 0);
-  } else {
-    union { u4 v; b8 h; } x, y;
-    x.v = a;
-    y.v = b;
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.h, y.h, c, 0, 0, 0);
-  }
-}
-
-template <typename T> __device__ __forceinline__ u4 ones16() {
-  union { u4 v; T e[Traits<T>::kChunk]; } x;
-#pragma unroll
-  for (int i = 0; i < Traits<T>::kChunk; ++i) x.e[i] = (T)1.f;
-  return x.v;
-}
-
-// Workgroups of one XCD (blockIdx mod 8, the hardware's round robin) take neighbouring tiles, whose operand panels then meet in its L2.
-__device__ __forceinline__ int64_t xcd_order(int64_t id, int64_t n) {
-  const int64_t per = n >> 3, rest = n & 7, x = id & 7, i = id >> 3;
-  return x * per + (x < rest ? x : rest) + i;
-}
-
-// TILE x TILE outputs per workgroup, four waves of TILE/2 x TILE/2.
-template <typename T, int TILE, bool AKC, bool BKC, bool GATE>
-__global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args g) {
-  constexpr int W = TILE / 2, F = W / 32;
-  using OpA = Operand<T, TILE, AKC, GATE>;
-  using OpB = Operand<T, TILE, BKC, false>;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tiles_n = (g.n + TILE - 1) / TILE;
-  const int64_t tile = xcd_order(blockIdx.x, gridDim.x);
-  const int64_t m0 = tile / tiles_n * TILE, n0 = tile % tiles_n * TILE;
-  const int64_t k_begin = (int64_t)blockIdx.y * g.k_per_split;
-  const int64_t k_end = k_begin + g.k_per_split < g.k ? k_begin + g.k_per_split : g.k;
-  const int wm = (wave >> 1) * W, wn = (wave & 1) * W;
-  const bool sums = g.colsum != nullptr && n0 == 0 && wn == 0;
-
-  f16v acc[F][F], accs[F];
-#pragma unroll
-  for (int i = 0; i < F; ++i) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) accs[i][r] = 0.f;
-#pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  }
-
-  OpA oa;
-  OpB ob;
-  const T* a = static_cast<const T*>(g.a);
-  const T* b = static_cast<const T*>(g.b);
-  if (k_begin < k_end) {
-    oa.load(a, g.lda, m0, k_begin, g.m, k_end, g.gate, g.gate_ld);
-    ob.load(b, g.ldb, n0, k_begin, g.n, k_end, nullptr, 0);
-  }
-  int buf = 0;
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += OpA::BK) {
-    char* la = smem + buf * (OpA::kBytes + OpB::kBytes);
-    char* lb = la + OpA::kBytes;
-    oa.commit(la, g.slope);
-    ob.commit(lb, 0.f);
-    __syncthreads();      // the other buffer's readers passed this barrier before they can be overtaken: one barrier per k-tile
-    if (k0 + OpA::BK < k_end) {
-      oa.load(a, g.lda, m0, k0 + OpA::BK, g.m, k_end, g.gate, g.gate_ld);
-      ob.load(b, g.ldb, n0, k0 + OpA::BK, g.n, k_end, nullptr, 0);
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u4 fa[F], fb[F];
-#pragma unroll
-      for (int i = 0; i < F; ++i) fa[i] = OpA::fragment(la, wm + 32 * i, s, lane);
-#pragma unroll
-      for (int j = 0; j < F; ++j) fb[j] = OpB::fragment(lb, wn + 32 * j, s, lane);
-#pragma unroll
-      for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = mma<T>(fb[j], fa[i], acc[i][j]);
-      if (!AKC && sums)
-#pragma unroll
-        for (int i = 0; i < F; ++i) accs[i] = mma<T>(ones16<T>(), fa[i], accs[i]);
-    }
-    buf ^= 1;
-  }
-
-  // lane: output row (lane & 31) of the 32 x 32 block, register r: column 8 (r / 4) + 4 (lane / 32) + r % 4
-  if (!AKC && sums && lane < 32) {
-#pragma unroll
-    for (int i = 0; i < F; ++i) {
-      const int64_t row = m0 + wm + 32 * i + lane;
-      if (row < g.m) g.colsum[blockIdx.y * g.m + row] = accs[i][0];
-    }
-  }
-  __syncthreads();      // the k-tiles are dead: LDS is the waves' own scratch from here
-  // through LDS in fp32, 32 rows at a time, so that a lane finishes whole pieces of a row and neighbouring lanes neighbouring pieces
-  constexpr int kLd = W + 4;
-  float* scratch = reinterpret_cast<float*>(smem) + wave * 32 * kLd;
-#pragma unroll
-  for (int i = 0; i < F; ++i) {
-#pragma unroll
-    for (int j = 0; j < F; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f4*>(scratch + (lane & 31) * kLd + 32 * j + 8 * q + 4 * (lane >> 5)) =
-            f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int64_t rbase = m0 + wm + 32 * i, cbase = n0 + wn;
-    if (g.partial) {
-      constexpr int kPer = W / 4;
-      float* out = g.partial + (int64_t)blockIdx.y * g.m * g.n;
-#pragma unroll
-      for (int p = lane; p < 32 * kPer; p += 64) {
-        const int64_t row = rbase + p / kPer, col = cbase + (p % kPer) * 4;
-        const f4 v = *reinterpret_cast<const f4*>(scratch + (p / kPer) * kLd + (p % kPer) * 4);
-        if (row < g.m && col < g.n) {
-          if (col + 4 <= g.n) __builtin_memcpy(out + row * g.n + col, &v, 16);
-          else {
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-              if (col + e < g.n) out[row * g.n + col + e] = v[e];
-          }
-        }
-      }
-    } else {
-      constexpr int kPer = W / kFinish;
-#pragma unroll 1
-      for (int p = lane; p < 32 * kPer; p += 64) {
-        const int64_t row = rbase + p / kPer, col = cbase + (p % kPer) * kFinish;
-        float v[kFinish];
-        const float* src = scratch + (p / kPer) * kLd + (p % kPer) * kFinish;
-        *reinterpret_cast<f4*>(v) = *reinterpret_cast<const f4*>(src);
-        *reinterpret_cast<f4*>(v + 4) = *reinterpret_cast<const f4*>(src + 4);
-        if (row < g.m && col < g.n) finish_piece<T>(g, row, col, v);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-}
-
-// ---- the splits of a long contraction joined, in a fixed order: out = finish(sum over s of partial[s]) -----------------------------------
-// 64 pieces per workgroup, the splits dealt to its four waves and joined through LDS.
-template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Args g, int splits) {
-  constexpr int C = kFinish;
-  __shared__ float part[4][64][C + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t per = (g.n + C - 1) / C, id = (int64_t)blockIdx.x * 64 + lane;
-  const int64_t row = id / per, col = id % per * C;
-  float v[C];
-#pragma unroll
-  for (int e = 0; e < C; ++e) v[e] = 0.f;
-  const bool live = row < g.m, full = col + C <= g.n;
-  if (live) {
-    const float* src = g.partial + row * g.n + col;
-    if (full) {
-#pragma unroll 4
-      for (int s = wave; s < splits; s += 4) {
-        float t[C];
-        __builtin_memcpy(t, src + (int64_t)s * g.m * g.n, sizeof(t));
-#pragma unroll
-        for (int e = 0; e < C; ++e) v[e] += t[e];
-      }
-    } else {
-      for (int s = wave; s < splits; s += 4)
-#pragma unroll
-        for (int e = 0; e < C; ++e)
-          if (col + e < g.n) v[e] += src[(int64_t)s * g.m * g.n + e];
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < C; ++e) part[wave][lane][e] = v[e];
-  __syncthreads();
-  if (wave == 0 && live) {
-#pragma unroll
-    for (int e = 0; e < C; ++e) v[e] = (part[0][lane][e] + part[1][lane][e]) + (part[2][lane][e] + part[3][lane][e]);
-    finish_piece<T>(g, row, col, v);
-  }
-}
-
-template <typename T> __global__ __launch_bounds__(kThreads) void join_sums_kernel(const float* __restrict__ colsum, T* __restrict__ out, int64_t n, int splits) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n) return;
-  float v = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) v += colsum[(int64_t)s * n + i];
-  out[i] = from_f<T>(v);
-}
-
-// ---- few rows: one pass over W, a wave per output column, the contraction over its lanes -------------------------------------------------
-template <typename T, int R> __global__ __launch_bounds__(kThreads) void skinny_kernel(Args g) {
-  constexpr int C = Traits<T>::kChunk;
-  const int lane = threadIdx.x & 63;
-  const int64_t col = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (col >= g.n) return;
-  const T* x = static_cast<const T*>(g.a);
-  const T* w = static_cast<const T*>(g.b) + col * g.ldb;
-  float acc[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = 0.f;
-  union P { u4 v; T e[C]; };
-#pragma unroll 2
-  for (int64_t k = lane * C; k < g.k; k += 64 * C) {
-    const bool full = k + C <= g.k;
-    const int count = full ? C : (int)(g.k - k);
-    P pw, px;
-    pw.v = full ? load16(w + k) : load_some(w + k, count);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (r < g.m) {
-        px.v = full ? load16(x + r * g.lda + k) : load_some(x + r * g.lda + k, count);
-#pragma unroll
-        for (int e = 0; e < C; ++e) acc[r] = fmaf((float)px.e[e], (float)pw.e[e], acc[r]);
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int d = 32; d; d >>= 1) acc[r] += __shfl_xor(acc[r], d);
-  // lane r finishes row r
-  float z = acc[0];
-#pragma unroll
-  for (int r = 1; r < R; ++r) z = lane == r ? acc[r] : z;
-  if (lane < g.m) {
-    const T* bias = static_cast<const T*>(g.bias);
-    const T* res = static_cast<const T*>(g.residual);
-    if (bias) z += (float)bias[col];
-    float y = act_of(z, g.act, g.slope);
-    if (g.zsave) static_cast<T*>(g.zsave)[lane * g.n + col] = saved_z<T>(z);
-    if (res) y += (float)res[lane * g.ldr + col];
-    static_cast<T*>(g.out)[lane * g.ldo + col] = from_f<T>(y);
-  }
-}
-
-// dz = dy * act'(z) for the smooth activations, rounded to the call's type (2^-9 / 2^-12 relative, once, before sums that average it out)
-template <typename T> __global__ __launch_bounds__(kThreads) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ z, T* __restrict__ dz,
-                                                                                int64_t rows, int64_t n, int act) {
-  constexpr int C = Traits<T>::kChunk;
-  const int64_t per = (n + C - 1) / C, id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = id / per, col = id % per * C;
-  if (row >= rows) return;
-  union P { u4 v; T e[C]; };
-  P a, b, o;
-  const bool full = col + C <= n;
-  const int count = full ? C : (int)(n - col);
-  a.v = full ? load16(dy + row * lddy + col) : load_some(dy + row * lddy + col, count);
-  b.v = full ? load16(z + row * n + col) : load_some(z + row * n + col, count);
-#pragma unroll
-  for (int e = 0; e < C; ++e) o.e[e] = from_f<T>((float)a.e[e] * act_slope((float)b.e[e], act));
-  if (full) store16(dz + row * n + col, o.v);
-  else {
-#pragma unroll
-    for (int e = 0; e < C; ++e)
-      if (e < count) dz[row * n + col + e] = o.e[e];
-  }
-}
-
-// ---- host --------------------------------------------------------------------------------------------------------------------------------
-
-constexpr int64_t kMaxDim = (int64_t)1 << 31;
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-struct Plan {
-  int tile;        // 128 or 64
-  int splits;
-  int64_t k_per_split;
-};
-
-// The workgroups of a product of [m, k] and [k, n]: 128-wide tiles where they alone give every CU one, else 64-wide ones (a quarter of the
-// outputs each: four times the workgroups); where that is still too few the contraction is split, down to four k-tiles a split.  The CU
-// count is the part's (256): a plan must not depend on the device that is current when the workspace is sized.
-inline Plan plan_of(int64_t m, int64_t n, int64_t k, int size) {
-  constexpr int64_t kCus = 256;
-  const int64_t bk = kBkBytes / size, k_tiles = ceil_div(k, bk);
-  Plan p;
-  p.tile = ceil_div(m, 128) * ceil_div(n, 128) >= kCus ? 128 : 64;
-  if (p.tile == 64 && ceil_div(m, 64) * ceil_div(n, 64) < kCus && k_tiles >= 64) p.tile = m >= 128 && n >= 128 ? 128 : 64;      // long contraction: wide tiles, split
-  const int64_t tiles = ceil_div(m, p.tile) * ceil_div(n, p.tile);
-  int64_t s = tiles == 0 || tiles >= kCus ? 1 : ceil_div(kCus, tiles);      // (no rows: no tiles)
-  if (s > k_tiles / 4) s = k_tiles / 4;
-  if (s < 1) s = 1;
-  p.k_per_split = ceil_div(ceil_div(k_tiles, s), 1) * bk;
-  if (p.k_per_split == 0) p.k_per_split = bk;
-  p.splits = (int)(k ? ceil_div(k, p.k_per_split) : 1);
-  return p;
-}
-
-inline int64_t align256(int64_t b) { return (b + 255) & ~(int64_t)255; }
-inline int64_t partial_bytes(const Plan& p, int64_t m, int64_t n) { return p.splits > 1 ? align256((int64_t)p.splits * m * n * 4) : 0; }
-
-template <typename T, int TILE, bool AKC, bool BKC, bool GATE> int launch_tile(const Args& g, const Plan& p, hipStream_t st) {
-  constexpr int kStage = 2 * TILE * kBkBytes;
-  constexpr int kScratch = 4 * 32 * (TILE / 2 + 4) * 4;
-  constexpr int kLds = 2 * kStage > kScratch ? 2 * kStage : kScratch;
-  static_assert(kLds <= 65536, "above 64 KiB the launch needs an opt-in");
-  const int64_t tiles = ceil_div(g.m, TILE) * ceil_div(g.n, TILE);
-  if (tiles >= kMaxDim) return S2L_E_SIZE;
-  hipLaunchKernelGGL((tile_kernel<T, TILE, AKC, BKC, GATE>), dim3((unsigned)tiles, (unsigned)p.splits), dim3(kThreads), kLds, st, g);
-  return (int)hipGetLastError();
-}
-
-template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st) {
-  g.k_per_split = p.k_per_split;
-  g.partial = p.splits > 1 ? partial : nullptr;
-  int rc;
-  if constexpr (AKC && BKC) {
-    rc = p.tile == 128 ? launch_tile<T, 128, AKC, BKC, false>(g, p, st) : launch_tile<T, 64, AKC, BKC, false>(g, p, st);
-  } else {
-    if (g.gate) rc = p.tile == 128 ? launch_tile<T, 128, AKC, BKC, true>(g, p, st) : launch_tile<T, 64, AKC, BKC, true>(g, p, st);
-    else rc = p.tile == 128 ? launch_tile<T, 128, AKC, BKC, false>(g, p, st) : launch_tile<T, 64, AKC, BKC, false>(g, p, st);
-  }
-  if (rc || p.splits == 1) return rc;
-  const int64_t blocks = ceil_div(g.m * ceil_div(g.n, kFinish), 64);
-  if (blocks >= kMaxDim) return S2L_E_SIZE;
-  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g, p.splits);
-  return (int)hipGetLastError();
-}
-
-// few rows, unless sign bits are wanted: a lane there has one column, a byte of them is eight
-inline bool skinny(int64_t rows, bool bits) { return rows <= kSkinnyRows && !bits; }
-
-template <typename T> int forward(Args g, float* work, hipStream_t st) {
-  if (skinny(g.m, g.bits != nullptr)) {
-    const dim3 grid((unsigned)ceil_div(g.n, 4));
-    if (g.m == 1) hipLaunchKernelGGL((skinny_kernel<T, 1>), grid, dim3(kThreads), 0, st, g);
-    else if (g.m <= 4) hipLaunchKernelGGL((skinny_kernel<T, 4>), grid, dim3(kThreads), 0, st, g);
-    else hipLaunchKernelGGL((skinny_kernel<T, 8>), grid, dim3(kThreads), 0, st, g);
-    return (int)hipGetLastError();
-  }
-  return product<T, true, true>(g, plan_of(g.m, g.n, g.k, sizeof(T)), work, st);
-}
-
-struct Back {      // the workspace of the backward pass
-  Plan dx, dw;
-  int64_t dz, partial, colsum, total;      // bytes; the partials of dx and of dW take turns
-};
-
-inline Back back_plan(int64_t rows, int64_t in, int64_t out, int size, int act) {
-  Back b;
-  b.dx = plan_of(rows, in, out, size);
-  b.dw = plan_of(out, in, rows, size);
-  b.dz = act == S2L_ACT_GELU || act == S2L_ACT_SILU ? align256(rows * out * size) : 0;
-  const int64_t p1 = partial_bytes(b.dx, rows, in), p2 = partial_bytes(b.dw, out, in);
-  b.partial = p1 > p2 ? p1 : p2;
-  b.colsum = align256((int64_t)b.dw.splits * out * 4);
-  b.total = b.dz + b.partial + b.colsum;
-  return b;
-}
-
-template <typename T> int backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* saved, void* dx, int64_t lddx,
-                                   void* dw, void* db, char* work, int64_t rows, int64_t in, int64_t out, int act, float slope, hipStream_t st) {
-  const Back b = back_plan(rows, in, out, sizeof(T), act);
-  const void* dz = dy;
-  int64_t lddz = lddy;
-  if (b.dz && rows) {
-    const int64_t blocks = ceil_div(rows * ceil_div(out, Traits<T>::kChunk), kThreads);
-    if (blocks >= kMaxDim) return S2L_E_SIZE;
-    hipLaunchKernelGGL((slope_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const T*>(saved),
-                       reinterpret_cast<T*>(work), rows, out, act);
-    const int rc = (int)hipGetLastError();
-    if (rc) return rc;
-    dz = work;
-    lddz = out;
-  }
-  const bool gated = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU;
-  float* partial = reinterpret_cast<float*>(work + b.dz);
-  Args g{};
-  g.a = dz;
-  g.lda = lddz;
-  g.gate = gated ? static_cast<const uint8_t*>(saved) : nullptr;
-  g.gate_ld = (out + 7) >> 3;
-  g.slope = act == S2L_ACT_LEAKY_RELU ? slope : 0.f;
-  g.act = S2L_ACT_NONE;
-  if (dx && rows) {
-    Args d = g;
-    d.b = w;
-    d.ldb = ldw;
-    d.m = rows;
-    d.n = in;
-    d.k = out;
-    d.out = dx;
-    d.ldo = lddx;
-    const int rc = product<T, true, false>(d, b.dx, partial, st);
-    if (rc) return rc;
-  }
-  if (dw) {
-    Args d = g;
-    d.b = x;
-    d.ldb = ldx;
-    d.m = out;
-    d.n = in;
-    d.k = rows;
-    d.out = dw;
-    d.ldo = in;
-    d.colsum = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
-    const int rc = product<T, false, false>(d, b.dw, partial, st);
-    if (rc) return rc;
-    if (db) {
-      hipLaunchKernelGGL((join_sums_kernel<T>), dim3((unsigned)ceil_div(out, kThreads)), dim3(kThreads), 0, st, d.colsum, static_cast<T*>(db), out, b.dw.splits);
-      return (int)hipGetLastError();
-    }
-  }
-  return 0;
-}
+#define S2L_LINEAR_EXTERN(T)                                                                                                                  \
+  extern template int forward<T>(Args, float*, hipStream_t);                                                                                  \
+  extern template int backward<T>(const void*, int64_t, const void*, int64_t, const void*, int64_t, const void*, void*, int64_t, void*, void*, \
+                                  char*, int64_t, int64_t, int64_t, int, float, hipStream_t);
+S2L_LINEAR_EXTERN(float)
+S2L_LINEAR_EXTERN(__bf16)
+S2L_LINEAR_EXTERN(_Float16)
 
 inline int size_of(int dtype) { return dtype == S2L_DTYPE_F32 ? 4 : dtype == S2L_DTYPE_BF16 || dtype == S2L_DTYPE_F16 ? 2 : 0; }
 inline bool bad_dims(int64_t rows, int64_t in, int64_t out) {
