@@ -70,20 +70,57 @@ template <typename T> __device__ __forceinline__ u4 load_some(const T* p, int co
   return r.v;
 }
 
-__device__ __forceinline__ float act_of(float z, int act, float slope) {
-  switch (act) {
-    case S2L_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-    case S2L_ACT_LEAKY_RELU: return z > 0.f ? z : z * slope;
-    case S2L_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case S2L_ACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
+// Phi(z), the normal distribution function, and density's exponential exp(-z^2 / 2).  fp32: the library's erf.  16-bit types: Abramowitz and
+// Stegun's formula 7.1.26, erfc(x) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2) with t = 1 / (1 + p x), off by at most 1.5e-7 -- 2^-14 of
+// a 16-bit rounding -- in a third of the instructions (erf's took as long as the whole product: 16384 x 1024 x 4096 294 us a forward, 147 without).
+template <typename T> __device__ __forceinline__ float normal_cdf(float z, float* density) {
+  if constexpr (std::is_same_v<T, float>) {
+    *density = expf(-0.5f * z * z);
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f));
+  } else {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f) * t * e * 0.5f;      // half of erfc(x)
+    *density = e;
+    return z > 0.f ? 1.f - q : q;
+  }
+}
+template <typename T> __device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (std::is_same_v<T, float>) return 1.f / (1.f + expf(-z));
+  else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+}
+
+// N values at once, one branch for all of them.  (gelu of -infinity: -inf * 0 is NaN, as the formula has it; of large finite z: exactly 0 or z)
+template <typename T, int N> __device__ __forceinline__ void activate(float (&z)[N], int act, float slope) {
+  if (act == S2L_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] != z[i] ? z[i] : 0.f;
+  } else if (act == S2L_ACT_LEAKY_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] * slope;
+  } else if (act == S2L_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float e;
+      z[i] *= normal_cdf<T>(z[i], &e);
+    }
+  } else if (act == S2L_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] *= sigmoid<T>(z[i]);
   }
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == S2L_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-  const float s = 1.f / (1.f + expf(-z));      // silu; z -> -inf: s = 0 and z s = 0 (z (1 - s) s with s = 0 is 0 for every finite z)
+template <typename T> __device__ __forceinline__ float act_slope(float z, int act) {
+  if (act == S2L_ACT_GELU) {
+    float e;
+    const float phi = normal_cdf<T>(z, &e);
+    return fmaf(z * e, 0.39894228040143268f, phi);
+  }
+  const float s = sigmoid<T>(z);      // silu; z -> -inf: s = 0 and s (1 + z (1 - s)) = 0 for every finite z
   return s * (1.f + z * (1.f - s));
 }
 
@@ -117,42 +154,56 @@ template <typename T> __device__ __forceinline__ T saved_z(float z) {
   return from_f<T>(z);
 }
 
-template <typename T> __device__ __forceinline__ void finish_piece(const Args& g, int64_t row, int64_t col, const float* acc) {
-  const bool full = col + kFinish <= g.n;
-  const int count = full ? kFinish : (int)(g.n - col);
+// N pieces of a lane: everything that they read is requested before the first is used (one after the other they wait out a memory latency each:
+// 36864 x 256 with a residual took 40 us where its bytes take 12).  row[i] < 0: nothing there.
+template <typename T, int N> __device__ __forceinline__ void finish_pieces(const Args& g, const int64_t (&row)[N], const int64_t (&col)[N], float (&z)[N * kFinish],
+                                                                           const Eight<T> (&res)[N]) {
   const T* bias = static_cast<const T*>(g.bias);
-  const T* res = static_cast<const T*>(g.residual);
-  float z[kFinish];
+  int count[N];
 #pragma unroll
-  for (int i = 0; i < kFinish; ++i) z[i] = acc[i];
+  for (int p = 0; p < N; ++p) count[p] = row[p] < 0 ? 0 : col[p] + kFinish <= g.n ? kFinish : (int)(g.n - col[p]);
   if (bias) {
-    const Eight<T> b = load8(bias + col, full, count);
 #pragma unroll
-    for (int i = 0; i < kFinish; ++i) z[i] += (float)b.e[i];
+    for (int p = 0; p < N; ++p) {
+      const Eight<T> b = load8(bias + col[p], count[p] == kFinish, count[p]);
+#pragma unroll
+      for (int i = 0; i < kFinish; ++i) z[p * kFinish + i] += (float)b.e[i];
+    }
   }
   if (g.bits) {      // the side of the kink, from the fp32 z
-    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < kFinish; ++i) m |= z[i] > 0.f ? 1u << i : 0u;
-    g.bits[row * ((g.n + 7) >> 3) + (col >> 3)] = (uint8_t)m;
+    for (int p = 0; p < N; ++p) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kFinish; ++i) m |= z[p * kFinish + i] > 0.f ? 1u << i : 0u;
+      if (count[p]) g.bits[row[p] * ((g.n + 7) >> 3) + (col[p] >> 3)] = (uint8_t)m;
+    }
   }
   if (g.zsave) {
-    Eight<T> s;
 #pragma unroll
-    for (int i = 0; i < kFinish; ++i) s.e[i] = saved_z<T>(z[i]);
-    store8(static_cast<T*>(g.zsave) + row * g.n + col, s, full, count);
+    for (int p = 0; p < N; ++p) {
+      Eight<T> s;
+#pragma unroll
+      for (int i = 0; i < kFinish; ++i) s.e[i] = saved_z<T>(z[p * kFinish + i]);
+      store8(static_cast<T*>(g.zsave) + row[p] * g.n + col[p], s, count[p] == kFinish, count[p]);
+    }
   }
-  Eight<T> r, o;
-  if (res) r = load8(res + row * g.ldr + col, full, count);
+  activate<T>(z, g.act, g.slope);
 #pragma unroll
-  for (int i = 0; i < kFinish; ++i) z[i] = act_of(z[i], g.act, g.slope);
-  if (res) {
+  for (int p = 0; p < N; ++p) {
+    Eight<T> o;
+    if (g.residual) {
 #pragma unroll
-    for (int i = 0; i < kFinish; ++i) z[i] += (float)r.e[i];
+      for (int i = 0; i < kFinish; ++i) z[p * kFinish + i] += (float)res[p].e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kFinish; ++i) o.e[i] = from_f<T>(z[p * kFinish + i]);
+    store8(static_cast<T*>(g.out) + row[p] * g.ldo + col[p], o, count[p] == kFinish, count[p]);
   }
-#pragma unroll
-  for (int i = 0; i < kFinish; ++i) o.e[i] = from_f<T>(z[i]);
-  store8(static_cast<T*>(g.out) + row * g.ldo + col, o, full, count);
+}
+template <typename T> __device__ __forceinline__ Eight<T> residual_at(const Args& g, int64_t row, int64_t col) {
+  const bool full = col + kFinish <= g.n;
+  return load8(static_cast<const T*>(g.residual) + row * g.ldr + col, full, full ? kFinish : (int)(g.n - col));
 }
 
 // ---- one operand's k-tile: global -> registers -> LDS, laid out as core::Tile ------------------------------------------------------------
@@ -221,9 +272,18 @@ template <typename T> __device__ __forceinline__ u4 ones16() {
 // ---- the waves' results, FM x FN blocks of 32 x 32, through LDS in fp32, 32 rows at a time, so that a lane finishes whole pieces of a row and
 // neighbouring lanes neighbouring pieces.  rbase / cbase: the wave's first row and column; scratch: 32 * (32 FN + 4) floats of its own.
 template <typename T, int FM, int FN> __device__ __forceinline__ void finish(const Args& g, f16v (&acc)[FM][FN], int64_t rbase, int64_t cbase, float* scratch, int lane) {
-  constexpr int W = 32 * FN, kLd = W + 4;
+  constexpr int W = 32 * FN, kLd = W + 4, kPieces = W / kFinish / 2;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
+    int64_t row[kPieces], col[kPieces];
+    Eight<T> res[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      row[p] = rbase + 32 * i + (lane + 64 * p) / (W / kFinish);
+      col[p] = cbase + lane % (W / kFinish) * kFinish;
+      if (row[p] >= g.m || col[p] >= g.n) row[p] = -1;
+      if (g.residual && !g.partial && row[p] >= 0) res[p] = residual_at<T>(g, row[p], col[p]);
+    }
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -249,16 +309,15 @@ template <typename T, int FM, int FN> __device__ __forceinline__ void finish(con
         }
       }
     } else {
-      constexpr int kPer = W / kFinish;
-#pragma unroll 1
-      for (int p = lane; p < 32 * kPer; p += 64) {
-        const int64_t row = rbase + 32 * i + p / kPer, col = cbase + (p % kPer) * kFinish;
-        float v[kFinish];
-        const float* src = scratch + (p / kPer) * kLd + (p % kPer) * kFinish;
-        *reinterpret_cast<f4*>(v) = *reinterpret_cast<const f4*>(src);
-        *reinterpret_cast<f4*>(v + 4) = *reinterpret_cast<const f4*>(src + 4);
-        if (row < g.m && col < g.n) finish_piece<T>(g, row, col, v);
+      constexpr int kPer = W / kFinish, N = 32 * kPer / 64;
+      float z[N * kFinish];
+#pragma unroll
+      for (int p = 0; p < N; ++p) {
+        const float* src = scratch + ((lane + 64 * p) / kPer) * kLd + (lane % kPer) * kFinish;
+        *reinterpret_cast<f4*>(z + p * kFinish) = *reinterpret_cast<const f4*>(src);
+        *reinterpret_cast<f4*>(z + p * kFinish + 4) = *reinterpret_cast<const f4*>(src + 4);
       }
+      finish_pieces<T, N>(g, row, col, z, res);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -384,10 +443,22 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void dma_kernel(Args g) 
 
 // ---- the splits of a long contraction joined, in a fixed order: out = finish(sum over s of partial[s]) -----------------------------------
 // 64 pieces per workgroup, the splits dealt to its four waves and joined through LDS.
-template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Args g, int splits) {
+template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Args g, int splits, int blocks, T* dbias) {
   constexpr int C = kFinish;
   __shared__ float part[4][64][C + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x >= blocks) {      // behind the pieces: the bias gradient, 64 columns to a workgroup
+    const int64_t i = (int64_t)(blockIdx.x - blocks) * 64 + lane;
+    float v = 0.f;
+    if (i < g.m) {
+#pragma unroll 4
+      for (int s = wave; s < splits; s += 4) v += g.colsum[(int64_t)s * g.m + i];
+    }
+    part[wave][lane][0] = v;
+    __syncthreads();
+    if (wave == 0 && i < g.m) dbias[i] = from_f<T>((part[0][lane][0] + part[1][lane][0]) + (part[2][lane][0] + part[3][lane][0]));
+    return;
+  }
   const int64_t per = (g.n + C - 1) / C, id = (int64_t)blockIdx.x * 64 + lane;
   const int64_t row = id / per, col = id % per * C;
   float v[C];
@@ -417,17 +488,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Ar
   if (wave == 0 && live) {
 #pragma unroll
     for (int e = 0; e < C; ++e) v[e] = (part[0][lane][e] + part[1][lane][e]) + (part[2][lane][e] + part[3][lane][e]);
-    finish_piece<T>(g, row, col, v);
+    const int64_t rows[1] = {row}, cols[1] = {col};
+    Eight<T> res[1];
+    if (g.residual) res[0] = residual_at<T>(g, row, col);
+    finish_pieces<T, 1>(g, rows, cols, v, res);
   }
-}
-
-template <typename T> __global__ __launch_bounds__(kThreads) void join_sums_kernel(const float* __restrict__ colsum, T* __restrict__ out, int64_t n, int splits) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n) return;
-  float v = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) v += colsum[(int64_t)s * n + i];
-  out[i] = from_f<T>(v);
 }
 
 // ---- few rows: one pass over W, a wave per output column, the contraction over its lanes -------------------------------------------------
@@ -469,34 +534,35 @@ template <typename T, int R> __global__ __launch_bounds__(kThreads) void skinny_
     const T* bias = static_cast<const T*>(g.bias);
     const T* res = static_cast<const T*>(g.residual);
     if (bias) z += (float)bias[col];
-    float y = act_of(z, g.act, g.slope);
+    float y[1] = {z};
+    activate<T>(y, g.act, g.slope);
     if (g.zsave) static_cast<T*>(g.zsave)[lane * g.n + col] = saved_z<T>(z);
-    if (res) y += (float)res[lane * g.ldr + col];
-    static_cast<T*>(g.out)[lane * g.ldo + col] = from_f<T>(y);
+    if (res) y[0] += (float)res[lane * g.ldr + col];
+    static_cast<T*>(g.out)[lane * g.ldo + col] = from_f<T>(y[0]);
   }
 }
 
-// dz = dy * act'(z) for the smooth activations, rounded to the call's type (2^-9 / 2^-12 relative, once, before sums that average it out)
-template <typename T> __global__ __launch_bounds__(kThreads) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ z, T* __restrict__ dz,
-                                                                                int64_t rows, int64_t n, int act) {
-  constexpr int C = Traits<T>::kChunk;
-  const int64_t per = (n + C - 1) / C, id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = id / per, col = id % per * C;
+// dz = dy * act'(z).  The smooth activations: rounded to the call's type (2^-8 / 2^-11 relative at most, once, before sums that average it out).
+// The kinked ones: where both products then take the LDS-DMA path (which has no place for the gate); exact but for leaky_relu's factor.
+template <typename T> __global__ __launch_bounds__(kThreads) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ saved, T* __restrict__ dz,
+                                                                                int64_t rows, int64_t n, int act, float slope) {
+  const int64_t per = (n + kFinish - 1) / kFinish, id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t row = id / per, col = id % per * kFinish;
   if (row >= rows) return;
-  union P { u4 v; T e[C]; };
-  P a, b, o;
-  const bool full = col + C <= n;
-  const int count = full ? C : (int)(n - col);
-  a.v = full ? load16(dy + row * lddy + col) : load_some(dy + row * lddy + col, count);
-  b.v = full ? load16(z + row * n + col) : load_some(z + row * n + col, count);
+  const bool full = col + kFinish <= n;
+  const int count = full ? kFinish : (int)(n - col);
+  Eight<T> a = load8(dy + row * lddy + col, full, count);
+  if (act == S2L_ACT_GELU || act == S2L_ACT_SILU) {
+    const Eight<T> z = load8(static_cast<const T*>(saved) + row * n + col, full, count);
 #pragma unroll
-  for (int e = 0; e < C; ++e) o.e[e] = from_f<T>((float)a.e[e] * act_slope((float)b.e[e], act));
-  if (full) store16(dz + row * n + col, o.v);
-  else {
+    for (int e = 0; e < kFinish; ++e) a.e[e] = from_f<T>((float)a.e[e] * act_slope<T>((float)z.e[e], act));
+  } else {
+    const uint32_t m = static_cast<const uint8_t*>(saved)[row * per + (col >> 3)];
 #pragma unroll
-    for (int e = 0; e < C; ++e)
-      if (e < count) dz[row * n + col + e] = o.e[e];
+    for (int e = 0; e < kFinish; ++e)
+      if (!((m >> e) & 1)) a.e[e] = slope == 0.f ? (T)0.f : from_f<T>((float)a.e[e] * slope);
   }
+  store8(dz + row * n + col, a, full, count);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
@@ -574,24 +640,24 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AKC, bool B
   return (int)hipGetLastError();
 }
 
-// after a product: its splits' partial sums joined
-template <typename T> int joined(int rc, const Args& g, const Plan& p, hipStream_t st) {
-  if (rc || p.splits == 1) return rc;
-  const int64_t blocks = ceil_div(g.m * ceil_div(g.n, kFinish), 64);
-  if (blocks >= kMaxDim) return S2L_E_SIZE;
-  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, g, p.splits);
+// after a product: its splits' partial sums joined, and the bias gradient's
+template <typename T> int joined(int rc, const Args& g, const Plan& p, void* dbias, hipStream_t st) {
+  if (rc || (p.splits == 1 && !dbias)) return rc;
+  const int64_t blocks = p.splits == 1 ? 0 : ceil_div(g.m * ceil_div(g.n, kFinish), 64), sums = dbias ? ceil_div(g.m, 64) : 0;
+  if (blocks + sums >= kMaxDim) return S2L_E_SIZE;
+  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + sums)), dim3(kThreads), 0, st, g, p.splits, (int)blocks, static_cast<T*>(dbias));
   return (int)hipGetLastError();
 }
 
-template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st) {
+template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st, void* dbias = nullptr) {
   g.k_per_split = p.k_per_split;
   g.partial = p.splits > 1 ? partial : nullptr;
   int rc;
   if (dense_pieces(g, AKC, BKC, sizeof(T))) {
-    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, 4>(g, p, st), g, p, st);
+    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, 4>(g, p, st), g, p, dbias, st);
     if constexpr (sizeof(T) == 2 && AKC)
-      if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, st);
-    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, 2>(g, p, st), g, p, st);
+      if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, dbias, st);
+    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, 2>(g, p, st), g, p, dbias, st);
   }
   if (p.tile >= 128) {
     if constexpr (AKC && BKC) rc = launch_tile<T, 128, AKC, BKC, false>(g, p, st);
@@ -600,7 +666,7 @@ template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, flo
     if constexpr (AKC && BKC) rc = launch_tile<T, 64, AKC, BKC, false>(g, p, st);
     else rc = g.gate ? launch_tile<T, 64, AKC, BKC, true>(g, p, st) : launch_tile<T, 64, AKC, BKC, false>(g, p, st);
   }
-  return joined<T>(rc, g, p, st);
+  return joined<T>(rc, g, p, dbias, st);
 }
 
 // few rows, unless sign bits are wanted: a lane there has one column, a byte of them is eight
@@ -626,7 +692,9 @@ inline Back back_plan(int64_t rows, int64_t in, int64_t out, int size, int act) 
   Back b;
   b.dx = plan_of(rows, in, out, size);
   b.dw = plan_of(out, in, rows, size, false);
-  b.dz = act == S2L_ACT_GELU || act == S2L_ACT_SILU ? align256(rows * out * size) : 0;
+  const int64_t bk = kBkBytes / size;
+  const bool gated = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU;      // (the rule goes by the sizes alone: the workspace's size does)
+  b.dz = act == S2L_ACT_GELU || act == S2L_ACT_SILU || (gated && rows % bk == 0 && out % bk == 0 && in % (16 / size) == 0) ? align256(rows * out * size) : 0;
   const int64_t p1 = partial_bytes(b.dx, rows, in), p2 = partial_bytes(b.dw, out, in);
   b.partial = p1 > p2 ? p1 : p2;
   b.colsum = align256((int64_t)b.dw.splits * out * 4);
@@ -640,16 +708,16 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
   const void* dz = dy;
   int64_t lddz = lddy;
   if (b.dz && rows) {
-    const int64_t blocks = ceil_div(rows * ceil_div(out, Traits<T>::kChunk), kThreads);
+    const int64_t blocks = ceil_div(rows * ceil_div(out, kFinish), kThreads);
     if (blocks >= kMaxDim) return S2L_E_SIZE;
-    hipLaunchKernelGGL((slope_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const T*>(saved),
-                       reinterpret_cast<T*>(work), rows, out, act);
+    hipLaunchKernelGGL((slope_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, saved, reinterpret_cast<T*>(work),
+                       rows, out, act, act == S2L_ACT_LEAKY_RELU ? slope : 0.f);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
     dz = work;
     lddz = out;
   }
-  const bool gated = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU;
+  const bool gated = (act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU) && !b.dz;
   float* partial = reinterpret_cast<float*>(work + b.dz);
   Args g{};
   g.a = dz;
@@ -680,12 +748,7 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
     d.out = dw;
     d.ldo = in;
     d.colsum = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
-    const int rc = product<T, false, false>(d, b.dw, partial, st);
-    if (rc) return rc;
-    if (db) {
-      hipLaunchKernelGGL((join_sums_kernel<T>), dim3((unsigned)ceil_div(out, kThreads)), dim3(kThreads), 0, st, d.colsum, static_cast<T*>(db), out, b.dw.splits);
-      return (int)hipGetLastError();
-    }
+    return product<T, false, false>(d, b.dw, partial, st, db);
   }
   return 0;
 }
