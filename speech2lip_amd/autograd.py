@@ -23,6 +23,7 @@ observed frames, warp grids) get none.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -342,6 +343,7 @@ def lpips_distance(module, in0_nhwc, in1_nhwc, from01: bool = False, precision: 
     return _LpipsDistance.apply(module, in0_nhwc, in1_nhwc, bool(from01), precision)
 
 
+_nothing = contextlib.nullcontext()
 _LINEAR_DTYPES = {torch.float32: _abi.S2L_DTYPE_F32, torch.bfloat16: _abi.S2L_DTYPE_BF16, torch.float16: _abi.S2L_DTYPE_F16}
 
 
@@ -354,15 +356,6 @@ def _dense_rows(t):
     return t, (t.stride(0) if rows > 1 else n)
 
 
-def _on_device(index, fn, *args):
-    """fn(*args, raw current stream of device `index`), with that device current.  (The context manager and the stream object cost 4 us a call;
-    one layer of one sample is 10.)"""
-    if torch.cuda.current_device() == index:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-
-
 def _linear_forward(x, weight, bias, residual, act, slope, keep):
     lib = _abi.load()
     dt = _LINEAR_DTYPES[x.dtype]
@@ -371,24 +364,27 @@ def _linear_forward(x, weight, bias, residual, act, slope, keep):
     (rows, k), n = x2.shape, w2.shape[0]
     out = x.new_empty((*x.shape[:-1], n))
     res, ldr = _dense_rows(residual) if residual is not None else (None, n)
-    b = bias.contiguous() if bias is not None else None
     saved = torch.empty(lib.s2l_linear_saved_bytes(dt, act, rows, n), dtype=torch.uint8, device=x.device) if keep and act else None
     need = lib.s2l_linear_forward_work_bytes(dt, act, saved is not None, rows, k, n)
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    rc = _on_device(x.get_device(), lib.s2l_linear_forward, dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(),
-                    0 if res is None else res.data_ptr(), ldr, out.data_ptr(), n, 0 if saved is None else saved.data_ptr(),
-                    0 if work is None else work.data_ptr(), rows, k, n, act, slope)
-    _abi.check(rc, "s2l_linear_forward")
+    b = bias if bias is None or bias.stride(0) == 1 else bias.contiguous()
+    index = x.get_device()
+    # (the context manager and the stream object cost 4 us a call; one layer of one sample is 10)
+    with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
+        rc = lib.s2l_linear_forward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(), 0 if res is None else res.data_ptr(), ldr,
+                                    out.data_ptr(), n, 0 if saved is None else saved.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, act, slope,
+                                    torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _abi.check(rc, "s2l_linear_forward")
     return out, x2, w2, saved
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, slope):
-        keep = any(ctx.needs_input_grad[:3])
-        out, x2, w2, saved = _linear_forward(x, weight, bias, residual, act, slope, keep)
-        need_w = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]      # the bias gradient is a by-product of dW
-        ctx.save_for_backward(x2 if need_w else None, w2 if ctx.needs_input_grad[0] else None, saved)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        out, x2, w2, saved = _linear_forward(x, weight, bias, residual, act, slope, need_x or need_w or need_b)
+        ctx.save_for_backward(x2 if need_w or need_b else None, w2 if need_x else None, saved)      # (the bias gradient is a by-product of dW)
         ctx.meta = (act, slope, x.shape, weight.shape)
         return out
 
@@ -403,19 +399,41 @@ class _Linear(torch.autograd.Function):
             lib = _abi.load()
             dt = _LINEAR_DTYPES[dy.dtype]
             d2, ldd = _dense_rows(dy)
-            rows, n = d2.shape
-            k = w_shape[1]
+            (rows, n), k = d2.shape, w_shape[1]
             dx = dy.new_empty(x_shape) if need_x else None
             dw = dy.new_empty(w_shape) if need_w or need_b else None
             db = dy.new_empty(n) if need_b else None
-            need = lib.s2l_linear_backward_work_bytes(dt, act, rows, k, n)
-            work = torch.empty(need, dtype=torch.uint8, device=dy.device)
-            rc = _on_device(dy.get_device(), lib.s2l_linear_backward, dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(),
-                            k if x2 is None or rows < 2 else x2.stride(0), 0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
-                            0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k, 0 if dw is None else dw.data_ptr(),
-                            0 if db is None else db.data_ptr(), work.data_ptr(), rows, k, n, act, slope)
-            _abi.check(rc, "s2l_linear_backward")
+            work = torch.empty(lib.s2l_linear_backward_work_bytes(dt, act, rows, k, n), dtype=torch.uint8, device=dy.device)
+            index = dy.get_device()
+            with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
+                rc = lib.s2l_linear_backward(dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(), k if x2 is None or rows < 2 else x2.stride(0),
+                                             0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
+                                             0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k,
+                                             0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), work.data_ptr(), rows, k, n, act, slope,
+                                             torch._C._cuda_getCurrentRawStream(index))
+            if rc:
+                _abi.check(rc, "s2l_linear_backward")
         return dx, dw if need_w else None, db, dy if need_r else None, None, None
+
+
+def _linear_refuse(x, weight, bias, residual):
+    """What is wrong with the arguments of `linear`, as an exception."""
+    given = [t for t in (x, weight, bias, residual) if t is not None]
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor) or not all(isinstance(t, torch.Tensor) for t in given):
+        raise TypeError("linear: x, weight, bias and residual are tensors")
+    xs, ws = x.shape, weight.shape
+    if x.dtype not in _LINEAR_DTYPES:
+        raise ValueError(f"linear: float32, bfloat16 or float16: got {x.dtype}")
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1] or ws[0] < 1 or ws[1] < 1:
+        raise ValueError(f"linear: x [..., in] and weight [out, in] with in, out >= 1: got {tuple(xs)} and {tuple(ws)}")
+    if bias is not None and bias.shape != ws[:1]:
+        raise ValueError(f"linear: bias must be [{ws[0]}]: got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != xs[:-1] + ws[:1]:
+        raise ValueError(f"linear: residual must be {tuple(xs[:-1] + ws[:1])} (it is not broadcast): got {tuple(residual.shape)}")
+    for t in given:
+        if t.dtype != x.dtype:
+            raise ValueError(f"linear: every tensor in one type: got {x.dtype} and {t.dtype}")
+    raise _abi.S2LError("linear: every tensor must be on one GPU (no CPU fallback)")
 
 
 def linear(x, weight, bias=None, residual=None, activation: str = "none", negative_slope: float = 0.02):
@@ -425,27 +443,22 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     activation: "none", "relu", "leaky_relu" (`negative_slope`; 0.02 is the audio encoder's), "gelu" (erf form) or "silu".  Sums, activation and
     residual are evaluated in fp32 and rounded once.  The backward pass keeps one bit per output for the kinked activations and the pre-activation
     for the smooth ones; it can run once (no double backward).  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
-    if activation not in _abi.S2L_ACT:
+    act = _abi.S2L_ACT.get(activation)
+    if act is None:
         raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")
-    given = [t for t in (x, weight, bias, residual) if t is not None]
-    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor) or not all(isinstance(t, torch.Tensor) for t in given):
-        raise TypeError("linear: x, weight, bias and residual are tensors")
-    dtype, dev, w_shape, x_shape = x.dtype, x.device, weight.shape, x.shape
-    if dtype not in _LINEAR_DTYPES:
-        raise ValueError(f"linear: float32, bfloat16 or float16: got {dtype}")
-    if len(x_shape) < 1 or len(w_shape) != 2 or x_shape[-1] != w_shape[1] or w_shape[0] < 1 or w_shape[1] < 1:
-        raise ValueError(f"linear: x [..., in] and weight [out, in] with in, out >= 1: got {tuple(x_shape)} and {tuple(w_shape)}")
-    if bias is not None and bias.shape != w_shape[:1]:
-        raise ValueError(f"linear: bias must be [{w_shape[0]}]: got {tuple(bias.shape)}")
-    if residual is not None and (residual.shape[:-1] != x_shape[:-1] or residual.shape[-1:] != w_shape[:1]):
-        raise ValueError(f"linear: residual must be {tuple(x_shape[:-1]) + (w_shape[0],)} (it is not broadcast): got {tuple(residual.shape)}")
-    for t in given:
-        if t.dtype != dtype:
-            raise ValueError(f"linear: every tensor in one type: got {dtype} and {t.dtype}")
-    for t in given:
-        if t.device != dev or not t.is_cuda:
-            raise _abi.S2LError("linear: every tensor must be on one GPU (no CPU fallback)")
-    act, slope = _abi.S2L_ACT[activation], float(negative_slope)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        return _Linear.apply(x, weight, bias, residual, act, slope)
-    return _linear_forward(x, weight, bias, residual, act, slope, False)[0]
+    grad = False
+    try:
+        dtype, index, xs, ws = x.dtype, x.get_device(), x.shape, weight.shape
+        fine = (dtype in _LINEAR_DTYPES and index >= 0 and len(ws) == 2 and xs[-1] == ws[1] and ws[0] > 0 and ws[1] > 0
+                and (bias is None or bias.shape == ws[:1]) and (residual is None or residual.shape == xs[:-1] + ws[:1]))
+        for t in (x, weight, bias, residual):
+            if t is not None:
+                fine = fine and t.dtype == dtype and t.get_device() == index
+                grad = grad or t.requires_grad
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _linear_refuse(x, weight, bias, residual)
+    if grad and torch.is_grad_enabled():
+        return _Linear.apply(x, weight, bias, residual, act, float(negative_slope))
+    return _linear_forward(x, weight, bias, residual, act, float(negative_slope), False)[0]

@@ -271,7 +271,7 @@ template <typename T> __device__ __forceinline__ u4 ones16() {
 
 // ---- the waves' results, FM x FN blocks of 32 x 32, through LDS in fp32, 32 rows at a time, so that a lane finishes whole pieces of a row and
 // neighbouring lanes neighbouring pieces.  rbase / cbase: the wave's first row and column; scratch: 32 * (32 FN + 4) floats of its own.
-template <typename T, int FM, int FN> __device__ __forceinline__ void finish(const Args& g, f16v (&acc)[FM][FN], int64_t rbase, int64_t cbase, float* scratch, int lane) {
+template <typename T, int FM, int FN> __device__ __forceinline__ void finish(const Args& g, f16v (&acc)[FM][FN], int64_t rbase, int64_t cbase, float* scratch, int lane, int split) {
   constexpr int W = 32 * FN, kLd = W + 4, kPieces = W / kFinish / 2;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -294,7 +294,7 @@ template <typename T, int FM, int FN> __device__ __forceinline__ void finish(con
     __builtin_amdgcn_wave_barrier();
     if (g.partial) {
       constexpr int kPer = W / 4;
-      float* out = g.partial + (int64_t)blockIdx.y * g.m * g.n;
+      float* out = g.partial + (int64_t)split * g.m * g.n;
 #pragma unroll
       for (int p = lane; p < 32 * kPer; p += 64) {
         const int64_t row = rbase + 32 * i + p / kPer, col = cbase + (p % kPer) * 4;
@@ -325,12 +325,12 @@ template <typename T, int FM, int FN> __device__ __forceinline__ void finish(con
 }
 
 // dbias: the sums over k of operand a's rows, from products with ones (accs: 32 x 32 blocks of equal columns)
-template <int FM> __device__ __forceinline__ void put_sums(const Args& g, const f16v (&accs)[FM], int64_t rbase, int lane) {
+template <int FM> __device__ __forceinline__ void put_sums(const Args& g, const f16v (&accs)[FM], int64_t rbase, int lane, int split) {
   if (lane < 32) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int64_t row = rbase + 32 * i + lane;
-      if (row < g.m) g.colsum[blockIdx.y * g.m + row] = accs[i][0];
+      if (row < g.m) g.colsum[split * g.m + row] = accs[i][0];
     }
   }
 }
@@ -399,22 +399,21 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args g) {
     buf ^= 1;
   }
 
-  if (!AKC && sums) put_sums(g, accs, m0 + wm, lane);
+  if (!AKC && sums) put_sums(g, accs, m0 + wm, lane, blockIdx.y);
   __syncthreads();      // the k-tiles are dead: LDS is the waves' own scratch from here
-  finish<T, F, F>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(smem) + wave * 32 * (W + 4), lane);
+  finish<T, F, F>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(smem) + wave * 32 * (W + 4), lane, blockIdx.y);
 }
 
 // The same product where everything is a multiple of the pieces (rule: dense_pieces below): operands by LDS-DMA, several k-tiles ahead.
 // BM x BN outputs, WAVES_M x WAVES_N waves.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AKC, bool BKC, int STAGES>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void dma_kernel(Args g) {
+__device__ __forceinline__ void dma_tile(const Args& g, int block, int blocks, int split, char* smem) {
   using P = core::Product<T, BM, BN, WAVES_M, WAVES_N, 1, AKC, BKC, kBkBytes, STAGES>;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_n = (int)((g.n + BN - 1) / BN);
-  const int tile = core::xcd_order(blockIdx.x, gridDim.x);
+  const int tile = core::xcd_order(block, blocks);
   const int64_t m0 = (int64_t)(tile / tiles_n) * BM, n0 = (int64_t)(tile % tiles_n) * BN;
-  const int64_t k_begin = (int64_t)blockIdx.y * g.k_per_split;
+  const int64_t k_begin = (int64_t)split * g.k_per_split;
   const int64_t k_end = k_begin + g.k_per_split < g.k ? k_begin + g.k_per_split : g.k;
   const int wm = wave / WAVES_N * P::WM, wn = wave % WAVES_N * P::WN;
   const bool sums = g.colsum != nullptr && n0 == 0 && wn == 0;
@@ -437,8 +436,26 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void dma_kernel(Args g) 
 #pragma unroll
       for (int i = 0; i < P::FM; ++i) accs[i] = mma<T>(ones16<T>(), fa[0][i], accs[i]);
   });
-  if (!AKC && sums) put_sums(g, accs, m0 + wm, lane);
-  finish<T, P::FM, P::FN>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(smem) + wave * 32 * (P::WN + 4), lane);
+  if (!AKC && sums) put_sums(g, accs, m0 + wm, lane, split);
+  finish<T, P::FM, P::FN>(g, acc, m0 + wm, n0 + wn, reinterpret_cast<float*>(smem) + wave * 32 * (P::WN + 4), lane, split);
+}
+
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AKC, bool BKC, int STAGES>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void dma_kernel(Args g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  dma_tile<T, BM, BN, WAVES_M, WAVES_N, AKC, BKC, STAGES>(g, blockIdx.x, gridDim.x, blockIdx.y, smem);
+}
+
+// dx and dW in one launch, dW's workgroups (the longer contraction) first: a launch less, and neither waits for the other's last workgroups.
+constexpr int stages_of(int tile) { return tile == 64 ? 3 : 2; }
+template <typename T, int DX, int DW> __global__ __launch_bounds__(kThreads, 2) void both_kernel(Args dx, Args dw, int dw_tiles, int dw_blocks) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int id = blockIdx.x;
+  if (id < dw_blocks) dma_tile<T, DW, DW, 2, 2, false, false, stages_of(DW)>(dw, id % dw_tiles, dw_tiles, id / dw_tiles, smem);
+  else {
+    const int blocks = gridDim.x - dw_blocks;
+    dma_tile<T, DX, DX, 2, 2, true, false, stages_of(DX)>(dx, id - dw_blocks, blocks, 0, smem);
+  }
 }
 
 // ---- the splits of a long contraction joined, in a fixed order: out = finish(sum over s of partial[s]) -----------------------------------
@@ -576,8 +593,9 @@ struct Plan {
   int64_t k_per_split;
 };
 
-// The workgroups of a product of [m, k] and [k, n]: 128-wide tiles where they alone give every CU one, else 64-wide ones (a quarter of the
-// outputs each: four times the workgroups); where that is still too few the contraction is split, down to four k-tiles a split.  The CU
+// The workgroups of a product of [m, k] and [k, n]: 128-wide tiles where they alone give every CU one and the contraction is long enough to be
+// bound by LDS, or four (short contractions are bound by memory, which more and smaller workgroups keep busier: 36864 x 256 x 256 with a
+// residual 25 us against 35), else 64-wide ones; where that is still too few the contraction is split, down to four k-tiles a split.  The CU
 // count is the part's (256): a plan must not depend on the device that is current when the workspace is sized.  wide: 256-wide tiles are there
 // (not for dW, whose sums for dbias and two transposed operands do not leave the registers for them).
 inline Plan plan_of(int64_t m, int64_t n, int64_t k, int size, bool wide = true) {
@@ -585,7 +603,7 @@ inline Plan plan_of(int64_t m, int64_t n, int64_t k, int size, bool wide = true)
   const int64_t bk = kBkBytes / size, k_tiles = ceil_div(k, bk);
   const auto count = [&](int64_t t) { return ceil_div(m, t) * ceil_div(n, t); };
   Plan p;
-  p.tile = wide && size == 2 && count(256) >= kCus ? 256 : count(128) >= kCus ? 128 : 64;
+  p.tile = wide && size == 2 && count(256) >= kCus ? 256 : count(128) >= 4 * kCus || (count(128) >= kCus && k_tiles >= 16) ? 128 : 64;
   if (p.tile == 64 && count(64) < kCus && k_tiles >= 64 && m >= 128 && n >= 128) p.tile = 128;      // long contraction: wide tiles, split
   const int64_t tiles = count(p.tile);
   const int64_t want = p.tile == 128 && k_tiles >= 128 ? 2 * kCus : kCus;      // two 128-wide ones to a CU hide each other's barriers
@@ -654,10 +672,10 @@ template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, flo
   g.partial = p.splits > 1 ? partial : nullptr;
   int rc;
   if (dense_pieces(g, AKC, BKC, sizeof(T))) {
-    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, 4>(g, p, st), g, p, dbias, st);
+    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, stages_of(64)>(g, p, st), g, p, dbias, st);
     if constexpr (sizeof(T) == 2 && AKC)
       if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, dbias, st);
-    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, 2>(g, p, st), g, p, dbias, st);
+    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, stages_of(128)>(g, p, st), g, p, dbias, st);
   }
   if (p.tile >= 128) {
     if constexpr (AKC && BKC) rc = launch_tile<T, 128, AKC, BKC, false>(g, p, st);
@@ -667,6 +685,17 @@ template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, flo
     else rc = g.gate ? launch_tile<T, 64, AKC, BKC, true>(g, p, st) : launch_tile<T, 64, AKC, BKC, false>(g, p, st);
   }
   return joined<T>(rc, g, p, dbias, st);
+}
+
+template <typename T, int DX, int DW> int launch_both(const Args& dx, const Args& dw, const Plan& pw, hipStream_t st) {
+  using PX = core::Product<T, DX, DX, 2, 2, 1, true, false, kBkBytes, stages_of(DX)>;
+  using PW = core::Product<T, DW, DW, 2, 2, 1, false, false, kBkBytes, stages_of(DW)>;
+  constexpr int lds = PX::kLds > PW::kLds ? PX::kLds : PW::kLds;
+  static_assert(lds <= 65536 && lds >= 4 * 32 * (DX / 2 + 4) * 4 && lds >= 4 * 32 * (DW / 2 + 4) * 4, "");
+  const int64_t x = ceil_div(dx.m, DX) * ceil_div(dx.n, DX), w = ceil_div(dw.m, DW) * ceil_div(dw.n, DW);
+  if (x + w * pw.splits >= kMaxDim) return S2L_E_SIZE;
+  hipLaunchKernelGGL((both_kernel<T, DX, DW>), dim3((unsigned)(x + w * pw.splits)), dim3(kThreads), lds, st, dx, dw, (int)w, (int)(w * pw.splits));
+  return (int)hipGetLastError();
 }
 
 // few rows, unless sign bits are wanted: a lane there has one column, a byte of them is eight
@@ -726,30 +755,37 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
   g.gate_ld = (out + 7) >> 3;
   g.slope = act == S2L_ACT_LEAKY_RELU ? slope : 0.f;
   g.act = S2L_ACT_NONE;
+  Args d = g;      // dx = dz W
+  d.b = w;
+  d.ldb = ldw;
+  d.m = rows;
+  d.n = in;
+  d.k = out;
+  d.out = dx;
+  d.ldo = lddx;
+  Args e = g;      // dW = dz^T x
+  e.b = x;
+  e.ldb = ldx;
+  e.m = out;
+  e.n = in;
+  e.k = rows;
+  e.out = dw;
+  e.ldo = in;
+  e.colsum = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
+  if (dx && dw && b.dx.tile <= 128 && b.dx.splits == 1 && dense_pieces(d, true, false, sizeof(T)) && dense_pieces(e, false, false, sizeof(T))) {
+    d.k_per_split = b.dx.k_per_split;
+    e.k_per_split = b.dw.k_per_split;
+    e.partial = b.dw.splits > 1 ? partial : nullptr;
+    int rc;
+    if (b.dx.tile == 64) rc = b.dw.tile == 64 ? launch_both<T, 64, 64>(d, e, b.dw, st) : launch_both<T, 64, 128>(d, e, b.dw, st);
+    else rc = b.dw.tile == 64 ? launch_both<T, 128, 64>(d, e, b.dw, st) : launch_both<T, 128, 128>(d, e, b.dw, st);
+    return joined<T>(rc, e, b.dw, db, st);
+  }
   if (dx && rows) {
-    Args d = g;
-    d.b = w;
-    d.ldb = ldw;
-    d.m = rows;
-    d.n = in;
-    d.k = out;
-    d.out = dx;
-    d.ldo = lddx;
     const int rc = product<T, true, false>(d, b.dx, partial, st);
     if (rc) return rc;
   }
-  if (dw) {
-    Args d = g;
-    d.b = x;
-    d.ldb = ldx;
-    d.m = out;
-    d.n = in;
-    d.k = rows;
-    d.out = dw;
-    d.ldo = in;
-    d.colsum = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
-    return product<T, false, false>(d, b.dw, partial, st, db);
-  }
+  if (dw) return product<T, false, false>(e, b.dw, partial, st, db);
   return 0;
 }
 
