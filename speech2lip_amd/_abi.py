@@ -15,7 +15,6 @@ S2L_PAD_MAY, S2L_PAD_DEFAULT = 0, 1
 S2L_POSE_OBS2CAN, S2L_POSE_CAN2OBS, S2L_POSE_CAN2OBS_INV = 0, 1, 2
 S2L_SAMPLE_ZEROS, S2L_SAMPLE_BORDER = 0, 1
 S2L_DTYPE_F32, S2L_DTYPE_BF16, S2L_DTYPE_F16 = 0, 1, 2
-S2L_MATRIX_WORDS = 5      # int64 words of an s2l_matrix record: in, out, momentum, rows | cols << 32, step (float bits)
 S2L_ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "gelu": 3, "silu": 4}
 
 # order of the pointer table of s2l_pack_weights == enum S2L_T_* in include/s2l_hip.h

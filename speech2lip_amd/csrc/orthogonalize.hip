@@ -89,40 +89,57 @@ __device__ __forceinline__ int owner(const int* first, int id) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(mine <= id)) - 1);
 }
 
-// Matrices of one size, their inputs and outputs at equal distances (one matrix; a batch): the first and the distances are in the kernel's arguments
-// and there is no table to look through, two memory round trips less in every launch (of 3 .. 6 us where the matrices are small).
+// How a workgroup finds its matrix.  Each memory round trip of it is 0.45 us of launches of 3 .. 6 us where the matrices are small, so: matrices
+// of one size, their inputs and outputs at equal distances (one matrix; a batch), from the kernel's arguments alone; others from a record per
+// workgroup, which the first pass writes (one round trip; looking through the table took two).
+struct Record {
+  int64_t base;
+  int rows, cols, index, id, pad[2];
+};
 struct Alike {
   Mat mat;
-  int per[KINDS];      // workgroups of one matrix; 0: not alike, look into the table
+  int per[KINDS];      // workgroups of one matrix; 0: not alike, look into the records
   int stride;          // bytes from one input / output to the next (at most 56 of them: below 2^31 checked)
   int64_t bytes;       // of one matrix's arrays
+  int64_t records[2];  // byte offset of the records of SYM and RECT launches in the workspace
 };
 struct Place {
-  Mat mat;
+  Mat mat;        // (in, out, momentum, step: where alike; else look at Table::mat[index] for them)
   int index;      // of the matrix
   int id;         // workgroup within the matrix
 };
+__device__ __forceinline__ Place alike_place(const Alike& alike, int kind, int id) {
+  const int k = id / alike.per[kind];
+  Mat m = alike.mat;
+  m.in = static_cast<const char*>(m.in) + (int64_t)k * alike.stride;
+  m.out = static_cast<char*>(m.out) + (int64_t)k * alike.stride;
+  m.base += k * alike.bytes;
+  m.stat += k * alike.per[STAT];
+  return Place{m, k, id - k * alike.per[kind]};
+}
 __device__ __forceinline__ Place place_of(const char* work, const Alike& alike, int kind, int id) {
-  if (alike.per[0]) {
-    const int k = id / alike.per[kind];
-    Mat m = alike.mat;
-    m.in = static_cast<const char*>(m.in) + (int64_t)k * alike.stride;
-    m.out = static_cast<char*>(m.out) + (int64_t)k * alike.stride;
-    m.base += k * alike.bytes;
-    m.stat += k * alike.per[STAT];
-    return Place{m, k, id - k * alike.per[kind]};
-  }
+  if (alike.per[0]) return alike_place(alike, kind, id);
+  const Record* rec = reinterpret_cast<const Record*>(work + alike.records[kind - SYM]) + id;
+  Place p{};
+  p.mat.base = core::uniform64(rec->base);
+  p.mat.rows = __builtin_amdgcn_readfirstlane(rec->rows);
+  p.mat.cols = __builtin_amdgcn_readfirstlane(rec->cols);
+  p.index = __builtin_amdgcn_readfirstlane(rec->index);
+  p.id = __builtin_amdgcn_readfirstlane(rec->id);
+  return p;
+}
+// a PACK launch's, from the table (once a call); a result's destination
+__device__ __forceinline__ Place pack_place(const char* work, const Alike& alike, int id) {
+  if (alike.per[0]) return alike_place(alike, PACK, id);
   const Table* t = reinterpret_cast<const Table*>(work);
-  const int k = owner(t->first[kind], id);
-  Mat m = t->mat[k];      // (one value for the workgroup: in scalar registers)
-  m.in = core::uniform64(m.in);
-  m.out = core::uniform64(m.out);
-  m.momentum = core::uniform64(m.momentum);
-  m.base = core::uniform64(m.base);
-  m.rows = __builtin_amdgcn_readfirstlane(m.rows);
-  m.cols = __builtin_amdgcn_readfirstlane(m.cols);
-  m.stat = __builtin_amdgcn_readfirstlane(m.stat);
-  return Place{m, k, id - __builtin_amdgcn_readfirstlane(t->first[kind][k])};
+  const int k = owner(t->first[PACK], id);
+  return Place{t->mat[k], k, id - t->first[PACK][k]};
+}
+__device__ __forceinline__ void destination(const char* work, const Alike& alike, Place& p) {
+  if (alike.per[0]) return;
+  const Mat& m = reinterpret_cast<const Table*>(work)->mat[p.index];
+  p.mat.out = core::uniform64(m.out);
+  p.mat.step = m.step;
 }
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, int64_t left, float* v) {
@@ -153,12 +170,21 @@ struct Momentum {
 
 // ---- first pass: the sums of squares in 64 bits (every later product scales with the norm: a sum over millions of squares in 32 bits is off by
 // more than all other roundings together), with the momentum update.  Memory bound: reads g, reads and writes m.
-template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, char* work, Momentum mo) {
+template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, char* work, Momentum mo, int64_t sym_records, int64_t rect_records, int syms, int rects) {
   __shared__ double part[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x == 0) {      // the table for the launches that follow
     const uint32_t* src = reinterpret_cast<const uint32_t*>(&t);
     for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += kThreads) reinterpret_cast<uint32_t*>(work)[i] = src[i];
+  }
+  // ... and the records (syms == rects == 0: matrices alike, none are wanted)
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < syms + rects; i += gridDim.x * kThreads) {
+    const bool rect = i >= syms;
+    const int id = rect ? i - syms : i;
+    const int* first = rect ? t.first[RECT] : t.first[SYM];
+    int k = 0;
+    while (k + 1 < kMaxMatrices && first[k + 1] <= id) ++k;
+    reinterpret_cast<Record*>(work + (rect ? rect_records : sym_records))[id] = Record{t.mat[k].base, t.mat[k].rows, t.mat[k].cols, k, id - first[k], {0, 0}};
   }
   const Mat& mat = t.mat[owner(t.first[STAT], blockIdx.x)];
   const int64_t total = elements_of(mat), chunk = chunk_of(total);
@@ -213,7 +239,7 @@ __device__ __forceinline__ void put8(_Float16* p, int64_t row, int64_t col, int6
 template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void split_kernel(char* work, Alike alike, Momentum mo, float eps, int parts) {
   __shared__ uint32_t tile[64][65];
   __shared__ double part[4];
-  const Place at0 = place_of(work, alike, PACK, blockIdx.x);
+  const Place at0 = pack_place(work, alike, blockIdx.x);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -294,7 +320,8 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr bool kSym = KIND == GRAM || KIND == POLY;
-  const Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  if constexpr (KIND == LAST) destination(work, alike, at0);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
@@ -469,7 +496,8 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr bool kSym = KIND == GRAM || KIND == POLY;
-  const Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  if constexpr (KIND == LAST) destination(work, alike, at0);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
@@ -599,6 +627,7 @@ constexpr int kMaxSteps = 100;
 struct Layout {
   int tile_sym, tile_rect;
   int blocks[KINDS];
+  int64_t sym_records, rect_records;      // byte offsets
   int64_t bytes;
 };
 
@@ -644,10 +673,12 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
     at[SYM] += ts * (ts + 1) / 2;
     at[RECT] += tiles(r.m, l->tile_rect) * tiles(r.n, l->tile_rect);
     base += r.total * 2;
-    if (at[PACK] > 0x7ffffff0 || at[SYM] > 0x7ffffff0) return S2L_E_SIZE;
+    if (at[PACK] > 0x3ffffff0 || at[SYM] > 0x3ffffff0 || at[RECT] > 0x3ffffff0) return S2L_E_SIZE;
   }
   for (int k = 0; k < KINDS; ++k) l->blocks[k] = (int)at[k];
-  const int64_t front = kTableBytes + partial_bytes((int)at[STAT]);
+  l->sym_records = kTableBytes + partial_bytes((int)at[STAT]);
+  l->rect_records = l->sym_records + at[SYM] * (int64_t)sizeof(Record);
+  const int64_t front = (l->rect_records + at[RECT] * (int64_t)sizeof(Record) + 255) / 256 * 256;
   for (int i = 0; i < count; ++i) t->mat[i].base += front;
   l->bytes = front + base;
   return 0;
@@ -655,6 +686,8 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
 
 inline Alike alike_of(const Table& t, const Layout& l, int count, int size, bool muon) {
   Alike a{};
+  a.records[0] = l.sym_records;
+  a.records[1] = l.rect_records;
   a.mat = t.mat[0];
   const int64_t stride = count > 1 ? static_cast<const char*>(t.mat[1].in) - static_cast<const char*>(t.mat[0].in) : 0;
   if (count > 1 && (muon || stride < 0 || stride > 0x7fffffff / count)) return a;
@@ -733,7 +766,8 @@ int run(const s2l_matrix* in, int count, double a, double b, double c, float eps
     if (rc) return rc;
     const Call call{alike_of(t, l, n, sizeof(T), MUON), work, st, dev};
     const auto parts = [&](int k) { return sizeof(T) == 4 || k < steps - 2 ? 2 : 1; };
-    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo);
+    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo, l.sym_records, l.rect_records, call.alike.per[0] ? 0 : l.blocks[SYM],
+                       call.alike.per[0] ? 0 : l.blocks[RECT]);
     rc = (int)hipGetLastError();
     if (rc) return rc;
     hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(l.blocks[PACK]), dim3(kThreads), 0, st, work, call.alike, mo, eps, parts(0));

@@ -16,6 +16,7 @@ torch's is bf16), with an Adam of its own for the parameters that are no such ma
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 import struct
 
@@ -144,10 +145,7 @@ class FusedAdam(torch.optim.Optimizer):
 
 def _matrix_table(records):
     """s2l_matrix records (in, out, momentum, rows, cols, step) as one host block."""
-    words = []
-    for src, out, momentum, rows, cols, step in records:
-        words += (src, out, momentum, rows | cols << 32, struct.unpack("i", struct.pack("f", step))[0])
-    return (ctypes.c_int64 * len(words))(*words)
+    return ctypes.create_string_buffer(struct.pack("=" + "qqqiif4x" * len(records), *itertools.chain.from_iterable(records)))
 
 
 def _check_iteration(who, steps, coefficients, eps):
@@ -280,29 +278,30 @@ class FusedMuon(FusedAdam):
         if group.get("algorithm", "muon") == "adam":
             return super()._step_group(gi, group, ps)
         lib = _abi.load()
-        dev = ps[0].device
         lr, mode = float(group["lr"]), group["adjust_lr_fn"]
+        index, f32, state = ps[0].get_device(), torch.float32, self.state
         records, grads, buffers = [], [], []
         for p in ps:
             g = p.grad
-            if p.device != dev or not p.is_cuda or p.dtype != torch.float32 or g.is_sparse or not p.is_contiguous():
+            if p.get_device() != index or index < 0 or p.dtype != f32 or g.layout != torch.strided or not p.is_contiguous():
                 raise _abi.S2LError("FusedMuon takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
-            st = self.state[p]
+            st = state[p]
             m = st.get("momentum_buffer")
             if m is None:
                 m = st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            if m.shape != p.shape or m.dtype != torch.float32 or m.device != dev or not m.is_contiguous():
-                m = st["momentum_buffer"] = m.to(device=dev, dtype=torch.float32).reshape(p.shape).contiguous()
-            if g.dtype != torch.float32 or not g.is_contiguous():
-                g = g.to(torch.float32).contiguous()
-            rows = p.shape[0]
-            cols = p.numel() // rows
-            scale = 0.2 * math.sqrt(max(rows, cols)) if mode == "match_rms_adamw" else math.sqrt(max(1.0, rows / cols))
+            elif m.shape != p.shape or m.dtype != f32 or m.get_device() != index or not m.is_contiguous():
+                m = st["momentum_buffer"] = m.to(device=p.device, dtype=f32).reshape(p.shape).contiguous()
+            if g.dtype != f32 or not g.is_contiguous():
+                g = g.to(f32).contiguous()
+            rows, count = p.shape[0], p.numel()
+            cols = count // rows
+            scale = 0.2 * math.sqrt(max(rows, cols)) if mode == "match_rms_adamw" else math.sqrt(rows / cols) if rows > cols else 1.0
             records.append((g.data_ptr(), p.data_ptr(), m.data_ptr(), rows, cols, lr * scale))
             grads.append(g)
             buffers.append(m)
         table = _matrix_table(records)
         a, b, c = _iteration("FusedMuon", group["ns_steps"], group["ns_coefficients"], group["eps"])
+        dev = ps[0].device
         with torch.cuda.device(dev):
             stream = torch.cuda.current_stream()
             flags = torch.zeros(len(ps), dtype=torch.int32, device=dev)

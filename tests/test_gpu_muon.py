@@ -455,7 +455,7 @@ def test_c_entry_refusals_need_no_gpu():
     muon = lambda t, n=1, steps=5, work=4096: lib.s2l_muon_step(t, n, 0.9, 1, 1.0, *ABC, 1e-7, steps, 0, work, 0)  # noqa: E731
     assert muon(table(), n=0) == 0 and muon(table(momentum=0)) == -1 and muon(table(momentum=4098)) == -3 and muon(table(), steps=0) == -2 and muon(table(), work=0) == -1
     assert lib.s2l_orthogonalize_work_bytes(0, 3) == 0 and lib.s2l_orthogonalize_work_bytes(table(rows=0), 1) == 0
-    assert lib.s2l_orthogonalize_work_bytes(table(), 1) == 4096 + 256 + 2 * (4 * 64 * 64 + 4 * 64 * 64)
+    assert lib.s2l_orthogonalize_work_bytes(table(), 1) == 4096 + 512 + 2 * (4 * 64 * 64 + 4 * 64 * 64)
 
 
 def test_groups_of_a_model():
