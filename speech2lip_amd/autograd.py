@@ -15,7 +15,7 @@ The parameters are passed to `apply` as inputs so that the engine delivers their
     unet_train            post_fusion_unet (train mode)     SimpleUnetLight.py:99-111   backward: s2l_unet_train_backward (d input + 32 tensors)
     crop_resize           crop + transforms.Resize          training.py:541-544   backward: s2l_crop_resize_backward
     sync_contrastive_loss get_sync_contrastive_loss         training.py:581-603   backward: s2l_syncnet_face_backward (d window)
-    linear                nn.Linear + activation (any size) tf_nerf.py:105-109, :149-172  backward: s2l_linear_backward
+    linear                nn.Linear + activation (any size) tf_nerf.py:105-109, :149-172  backward: s2l_linear_backward (the node is C++: csrc/linear_autograd.cpp)
     mse                   add_photometric_loss              training.py:605-619   backward: the gradient s2l_mse returns
 Gradients flow to: the 42 hot-path parameters, everything that `linear` takes, the audio columns of `rgb_forward`'s rows, the lip image, the U-Net input, the
 generated sync window, the prediction of the MSE.  Inputs the reference treats as data (audio windows, pixel coordinates,
@@ -23,7 +23,6 @@ observed frames, warp grids) get none.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
@@ -343,77 +342,23 @@ def lpips_distance(module, in0_nhwc, in1_nhwc, from01: bool = False, precision: 
     return _LpipsDistance.apply(module, in0_nhwc, in1_nhwc, bool(from01), precision)
 
 
-_nothing = contextlib.nullcontext()
-_LINEAR_DTYPES = {torch.float32: _abi.S2L_DTYPE_F32, torch.bfloat16: _abi.S2L_DTYPE_BF16, torch.float16: _abi.S2L_DTYPE_F16}
+_LINEAR_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_linear_native = (None, None)      # the loaded library, and the C++ node bound to its entries
 
 
-def _dense_rows(t):
-    """`t` [..., n] as rows of dense columns: (tensor [rows, n], row stride).  A view wherever the strides allow it."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    rows, n = t.shape
-    if (n > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < n):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else n)
-
-
-def _linear_forward(x, weight, bias, residual, act, slope, keep):
+def _linear_ops():
+    """csrc/linear_autograd.cpp, bound to the library in use."""
+    global _linear_native
     lib = _abi.load()
-    dt = _LINEAR_DTYPES[x.dtype]
-    x2, ldx = _dense_rows(x)
-    w2, ldw = _dense_rows(weight)
-    (rows, k), n = x2.shape, w2.shape[0]
-    out = x.new_empty((*x.shape[:-1], n))
-    res, ldr = _dense_rows(residual) if residual is not None else (None, n)
-    saved = torch.empty(lib.s2l_linear_saved_bytes(dt, act, rows, n), dtype=torch.uint8, device=x.device) if keep and act else None
-    need = lib.s2l_linear_forward_work_bytes(dt, act, saved is not None, rows, k, n)
-    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    b = bias if bias is None or bias.stride(0) == 1 else bias.contiguous()
-    index = x.get_device()
-    # (the context manager and the stream object cost 4 us a call; one layer of one sample is 10)
-    with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
-        rc = lib.s2l_linear_forward(dt, x2.data_ptr(), ldx, w2.data_ptr(), ldw, 0 if b is None else b.data_ptr(), 0 if res is None else res.data_ptr(), ldr,
-                                    out.data_ptr(), n, 0 if saved is None else saved.data_ptr(), 0 if work is None else work.data_ptr(), rows, k, n, act, slope,
-                                    torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _abi.check(rc, "s2l_linear_forward")
-    return out, x2, w2, saved
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, slope):
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        out, x2, w2, saved = _linear_forward(x, weight, bias, residual, act, slope, need_x or need_w or need_b)
-        ctx.save_for_backward(x2 if need_w or need_b else None, w2 if need_x else None, saved)      # (the bias gradient is a by-product of dW)
-        ctx.meta = (act, slope, x.shape, weight.shape)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        act, slope, x_shape, w_shape = ctx.meta
-        x2, w2, saved = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            lib = _abi.load()
-            dt = _LINEAR_DTYPES[dy.dtype]
-            d2, ldd = _dense_rows(dy)
-            (rows, n), k = d2.shape, w_shape[1]
-            dx = dy.new_empty(x_shape) if need_x else None
-            dw = dy.new_empty(w_shape) if need_w or need_b else None
-            db = dy.new_empty(n) if need_b else None
-            work = torch.empty(lib.s2l_linear_backward_work_bytes(dt, act, rows, k, n), dtype=torch.uint8, device=dy.device)
-            index = dy.get_device()
-            with _nothing if torch.cuda.current_device() == index else torch.cuda.device(index):
-                rc = lib.s2l_linear_backward(dt, d2.data_ptr(), ldd, 0 if x2 is None else x2.data_ptr(), k if x2 is None or rows < 2 else x2.stride(0),
-                                             0 if w2 is None else w2.data_ptr(), k if w2 is None or n < 2 else w2.stride(0),
-                                             0 if saved is None else saved.data_ptr(), 0 if dx is None else dx.data_ptr(), k,
-                                             0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), work.data_ptr(), rows, k, n, act, slope,
-                                             torch._C._cuda_getCurrentRawStream(index))
-            if rc:
-                _abi.check(rc, "s2l_linear_backward")
-        return dx, dw if need_w else None, db, dy if need_r else None, None, None
+    if _linear_native[0] is not lib:
+        try:
+            from . import _linear_ops as ops
+        except ImportError as e:
+            raise _abi.S2LError(f"_linear_ops.so does not load ({e}): build it with `python -m speech2lip_amd.build`") from e
+        ops.bind(*(ctypes.cast(getattr(lib, "s2l_linear_" + name), ctypes.c_void_p).value
+                   for name in ("saved_bytes", "forward_work_bytes", "backward_work_bytes", "forward", "backward")))
+        _linear_native = (lib, ops)
+    return _linear_native[1]
 
 
 def _linear_refuse(x, weight, bias, residual):
@@ -446,19 +391,11 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     act = _abi.S2L_ACT.get(activation)
     if act is None:
         raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")
-    grad = False
+    slope = float(negative_slope)
     try:
-        dtype, index, xs, ws = x.dtype, x.get_device(), x.shape, weight.shape
-        fine = (dtype in _LINEAR_DTYPES and index >= 0 and len(ws) == 2 and xs[-1] == ws[1] and ws[0] > 0 and ws[1] > 0
-                and (bias is None or bias.shape == ws[:1]) and (residual is None or residual.shape == xs[:-1] + ws[:1]))
-        for t in (x, weight, bias, residual):
-            if t is not None:
-                fine = fine and t.dtype == dtype and t.get_device() == index
-                grad = grad or t.requires_grad
-    except (AttributeError, IndexError, TypeError):
-        fine = False
-    if not fine:
+        out = _linear_ops().linear(x, weight, bias, residual, act, slope)
+    except TypeError:
+        out = None
+    if out is None:
         _linear_refuse(x, weight, bias, residual)
-    if grad and torch.is_grad_enabled():
-        return _Linear.apply(x, weight, bias, residual, act, float(negative_slope))
-    return _linear_forward(x, weight, bias, residual, act, float(negative_slope), False)[0]
+    return out

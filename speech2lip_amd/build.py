@@ -12,6 +12,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libs2l_hip.so")
 REF_LIB = os.path.join(PKG, "libs2l_hip_ref.so")      # the same ABI + the non-default kernel forms (-DS2L_WITH_REFERENCE_KERNELS): tests / tools only
+TORCH_OPS = os.path.join(PKG, "_linear_ops.so")        # the autograd node of the dense layer: C++ against torch, calls LIB through its C ABI
 RESOURCES = os.path.join(PKG, "kernel_resources.json")      # per-kernel registers / spills / scratch / LDS of the last build
 SOURCES = ["pack.hip", "frontend.hip", "rows.hip", "render.hip", "ensemble.hip", "train.hip", "composite.hip", "unet.hip", "warp.hip", "syncnet.hip", "lpips.hip", "syncchain.hip", "train_bf16.hip", "quant.hip", "render16.hip", "convh.hip",
            "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "orthogonalize.hip"]
@@ -54,11 +55,24 @@ def _hipcc() -> str:
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(REF_LIB):
+    if not os.path.exists(LIB) or not os.path.exists(REF_LIB) or not os.path.exists(TORCH_OPS):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_OPS))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(PKG, "..", "include", "s2l_hip.h")]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _torch_ops_command() -> list:
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+               os.path.join(cpp_extension.ROCM_HOME or "/opt/rocm", "include")]
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *sum((["-isystem", d] for d in include), []),
+            os.path.join(CSRC, "linear_autograd.cpp"), "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-o", TORCH_OPS + ".tmp"]
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
@@ -96,6 +110,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     finally:
         sys.path.pop(0)
     procs = []
+    ops = subprocess.Popen(_torch_ops_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     for src in SOURCES:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         cmd = [hipcc, *FLAGS, *SOURCE_FLAGS.get(src, ()), "-I", objdir, "-c", os.path.join(CSRC, src), "-o", obj]
@@ -116,6 +131,10 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         if verbose and rest.strip():
             print(rest)
         (ref_objs if is_ref else objs).append(obj)
+    out, _ = ops.communicate()
+    if ops.returncode != 0:
+        raise RuntimeError(f"g++ failed on linear_autograd.cpp:\n{out}")
+    os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
     ref_names = {s.replace(".hip", ".o") for s in REF_SOURCES}
     for out_lib, parts in ((LIB, objs), (REF_LIB, [o for o in objs if os.path.basename(o) not in ref_names] + ref_objs)):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out_lib + ".tmp", *parts]

@@ -7,9 +7,9 @@
 // the smallest end in 0.7 .. 1.2: U V^T but for that band.  p amplifies small singular values by a = 3.44 a step (485 over five), and with them
 // whatever rounding put into their directions, so the products' precision goes by the STEP, not by the type alone: X, A and B are held as two
 // IEEE halves (hi = f16(x), lo = f16(x - hi): 22 significant bits) and a product is three f16 MFMAs, hi hi + hi lo + lo hi, summed in fp32 --
-// fp32's own accuracy at 2.7 times the fp32 MFMA's peak -- in every step for fp32 input, and in all but the last two steps for bf16 / f16 input,
-// whose last two run on hi alone (their roundings of 2^-12 are amplified at most 12-fold; one product in every step would leave 2-4 % of error on
-// matrices of fast falling spectrum, and bf16 products 15-30 %).
+// fp32's own accuracy at 2.7 times the fp32 MFMA's peak -- in every step for fp32 and f16 input, and in all but the last two steps for bf16 input,
+// whose last two run on hi alone (their roundings of 2^-11 are amplified at most 12-fold and stay below the result's own 2^-8; one product in
+// every step would leave 2-4 % of error on matrices of fast falling spectrum, and bf16 products 15-30 %).
 // Values are scaled by 2^11: |X| <= ||X||_2 <= 1.2 and the entries of A and B <= 3.5 use the range of the halves from 2^-24 to 7168.
 //
 // All matrices of a call go through the same 2 + 3 * steps launches: one pass for the Frobenius norms (with the momentum update), one that scales
@@ -765,7 +765,7 @@ int run(const s2l_matrix* in, int count, double a, double b, double c, float eps
     rc = lay_out(in + first, n, &t, &l);
     if (rc) return rc;
     const Call call{alike_of(t, l, n, sizeof(T), MUON), work, st, dev};
-    const auto parts = [&](int k) { return sizeof(T) == 4 || k < steps - 2 ? 2 : 1; };
+    const auto parts = [&](int k) { return !std::is_same_v<T, __bf16> || k < steps - 2 ? 2 : 1; };
     hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo, l.sym_records, l.rect_records, call.alike.per[0] ? 0 : l.blocks[SYM],
                        call.alike.per[0] ? 0 : l.blocks[RECT]);
     rc = (int)hipGetLastError();

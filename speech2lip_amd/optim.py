@@ -205,7 +205,7 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
     side.  With the default coefficients the singular values end in 0.7 .. 1.2 (but for the smallest): nearly U V^T.
 
     update [..., rows, cols], or a list of such tensors of any sizes, all float32, all bfloat16 or all float16 on one GPU -> the same shape(s) and type,
-    in one set of launches.  float32: fp32's accuracy throughout; the 16-bit types: rounded once, their last two steps on half-precision products.
+    in one set of launches.  fp32's accuracy throughout, rounded once; bfloat16: its last two steps on half-precision products (below its rounding).
     A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not)."""
     many = isinstance(update, (list, tuple))
     given = list(update) if many else [update]
