@@ -26,6 +26,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 # such instructions in their own assembly text and are compiled as they were measured
 SCALAR_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCE_FLAGS = {s: SCALAR_FP32 for s in SOURCES if s.startswith(("linear", "orthogonalize"))}
+SOURCE_FLAGS["orthogonalize.hip"] = SCALAR_FP32 + ["-mllvm", "-amdgpu-kernarg-preload-count=16"]      # its launches are short: see its place_of
 _REMARK = re.compile(r"remark:\s+(Function Name|VGPRs|AGPRs|ScratchSize \[bytes/lane\]|SGPRs Spill|VGPRs Spill|LDS Size \[bytes/block\]|"
                      r"Occupancy \[waves/SIMD\]):\s*(\S+)")
 

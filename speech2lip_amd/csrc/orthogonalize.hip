@@ -117,10 +117,21 @@ __device__ __forceinline__ Place alike_place(const Alike& alike, int kind, int i
   m.stat += k * alike.per[STAT];
   return Place{m, k, id - k * alike.per[kind]};
 }
-__device__ __forceinline__ Place place_of(const char* work, const Alike& alike, int kind, int id) {
-  if (alike.per[0]) return alike_place(alike, kind, id);
-  const Record* rec = reinterpret_cast<const Record*>(work + alike.records[kind - SYM]) + id;
+// What every workgroup of a product needs first: plain scalars at the front of the kernel's arguments, which the hardware puts into scalar registers
+// with the wave (the build asks for 16 dwords of it), so that matrices alike need no load at all before their first operand request.
+#define S2L_FRONT char *work, int per, int rows, int cols, int64_t base, int64_t bytes_or_records, int from, int parts_out, float coef_a, float coef_b, float coef_c, int blocks
+#define S2L_FRONT_PASS work, per, rows, cols, base, bytes_or_records
+__device__ __forceinline__ Place place_of(const char* work, int per, int rows, int cols, int64_t base, int64_t bytes_or_records, int id) {
   Place p{};
+  if (per) {
+    p.index = id / per;
+    p.id = id - p.index * per;
+    p.mat.rows = rows;
+    p.mat.cols = cols;
+    p.mat.base = base + p.index * bytes_or_records;
+    return p;
+  }
+  const Record* rec = reinterpret_cast<const Record*>(work + bytes_or_records) + id;
   p.mat.base = core::uniform64(rec->base);
   p.mat.rows = __builtin_amdgcn_readfirstlane(rec->rows);
   p.mat.cols = __builtin_amdgcn_readfirstlane(rec->cols);
@@ -136,7 +147,11 @@ __device__ __forceinline__ Place pack_place(const char* work, const Alike& alike
   return Place{t->mat[k], k, id - t->first[PACK][k]};
 }
 __device__ __forceinline__ void destination(const char* work, const Alike& alike, Place& p) {
-  if (alike.per[0]) return;
+  if (alike.per[0]) {
+    p.mat.out = static_cast<char*>(alike.mat.out) + (int64_t)p.index * alike.stride;
+    p.mat.step = alike.mat.step;
+    return;
+  }
   const Mat& m = reinterpret_cast<const Table*>(work)->mat[p.index];
   p.mat.out = core::uniform64(m.out);
   p.mat.step = m.step;
@@ -301,10 +316,8 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
 
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
+// from: which of the two X^T arrays holds this step's; parts_out: halves that the next reader wants; coef_*: the step's coefficients
 struct Step {
-  float a, b, c;
-  int from;             // which of the two X^T arrays holds this step's
-  int parts_out;        // halves that the next reader wants
   float shrink;         // LAST, Muon: 1 - lr wd
   int* nan_flags;       // LAST, Muon: one int per matrix, set where the parameter as read holds a NaN
 };
@@ -314,13 +327,13 @@ template <int TILE, int PARTS, int STAGES, int KIND>
 using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, KIND != GRAM, KIND != GRAM, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES>;
 
 template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T>
-__global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike alike, Step st) {
+__global__ __launch_bounds__(kThreads, 2) void product_kernel(S2L_FRONT, Alike alike, Step st) {
   using C = Core<TILE, PARTS, STAGES, KIND>;
   constexpr int W = TILE / 2, F = W / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr bool kSym = KIND == GRAM || KIND == POLY;
-  Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  Place at0 = place_of(S2L_FRONT_PASS, core::xcd_order(blockIdx.x, blocks));
   if constexpr (KIND == LAST) destination(work, alike, at0);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
@@ -343,7 +356,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
   typename C::SB sb;
   int depth;
   if constexpr (KIND == GRAM) {
-    const _Float16* xt = arrays + (st.from ? r.xt[1] : r.xt[0]);
+    const _Float16* xt = arrays + (from ? r.xt[1] : r.xt[0]);
     sa.setup(xt, r.mp, m0, r.mp, 0, wave, lane);
     sb.setup(xt, r.mp, n0, r.mp, 0, wave, lane);
     depth = r.np;
@@ -353,7 +366,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
     depth = r.mp;
   } else {
     sa.setup(arrays + r.b, r.mp, m0, r.mp, 0, wave, lane);
-    sb.setup(arrays + (st.from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, wave, lane);
+    sb.setup(arrays + (from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, wave, lane);
     depth = r.mp;
   }
   f16v acc[F][F];
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
           for (int e = 0; e < 4; ++e) {
             float x = (float)hi[e];
             if constexpr (PARTS == 2) x += (float)lo[e];
-            v[e] = fmaf(st.c, v[e] * (1.f / kScale), st.b * x) + (row == col + e ? st.a * kScale : 0.f);
+            v[e] = fmaf(coef_c, v[e] * (1.f / kScale), coef_b * x) + (row == col + e ? coef_a * kScale : 0.f);
           }
         } else {
 #pragma unroll
@@ -446,14 +459,14 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
         if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
       } else {
         // 32 rows of four pieces, two pieces a lane: the symmetric ones as they are and mirrored, X^T mirrored
-        _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : st.from ? r.xt[0] : r.xt[1]);
+        _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : from ? r.xt[0] : r.xt[1]);
 #pragma unroll
         for (int e = 0; kSym && e < 2; ++e) {
           const int row = (lane >> 2) + 16 * e, c = lane & 3;
           uint32_t w[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
-          put8(to, rb + row, cb + 8 * c, r.mp, st.parts_out, w);
+          put8(to, rb + row, cb + 8 * c, r.mp, parts_out, w);
         }
         if (!kSym || ti != tj) {
 #pragma unroll
@@ -462,7 +475,7 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(char* work, Alike 
             uint32_t w[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
-            put8(to, cb + row, rb + 8 * c, r.mp, st.parts_out, w);
+            put8(to, cb + row, rb + 8 * c, r.mp, parts_out, w);
           }
         }
       }
@@ -490,13 +503,13 @@ template <int N, int REQUESTS> __device__ __forceinline__ void wait_younger(int 
 }
 
 template <int PARTS, int KIND, bool MUON, typename T>
-__global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike alike, Step st) {
+__global__ __launch_bounds__(kThreads, 2) void small_kernel(S2L_FRONT, Alike alike, Step st) {
   using C = Small<PARTS, KIND>;
   using L = typename C::L;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr bool kSym = KIND == GRAM || KIND == POLY;
-  Place at0 = place_of(work, alike, kSym ? SYM : RECT, core::xcd_order(blockIdx.x, gridDim.x));
+  Place at0 = place_of(S2L_FRONT_PASS, core::xcd_order(blockIdx.x, blocks));
   if constexpr (KIND == LAST) destination(work, alike, at0);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
@@ -514,7 +527,7 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
   }
   const int m0 = ti * 32, n0 = tj * 32;
   typename C::S sa, sb;
-  const _Float16* xt = arrays + (st.from ? r.xt[1] : r.xt[0]);
+  const _Float16* xt = arrays + (from ? r.xt[1] : r.xt[0]);
   sa.setup(KIND == GRAM ? xt : KIND == POLY ? arrays + r.a : arrays + r.b, r.mp, m0, r.mp, 0, wave, lane);
   sb.setup(KIND == POLY ? arrays + r.a : xt, r.mp, n0, kSym ? r.mp : r.np, 0, wave, lane);
   const int stages = __builtin_amdgcn_readfirstlane((KIND == GRAM ? r.np : r.mp) / 64);
@@ -609,13 +622,13 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(char* work, Alike al
       if constexpr (KIND == POLY) {
         float x = (float)hi[e];
         if constexpr (PARTS == 2) x += (float)lo[e];
-        v = fmaf(st.c, v * (1.f / kScale), st.b * x) + (grow == gcol + e ? st.a * kScale : 0.f);
+        v = fmaf(coef_c, v * (1.f / kScale), coef_b * x) + (grow == gcol + e ? coef_a * kScale : 0.f);
       } else {
         v *= 1.f / kScale;
       }
       w[e] = halves(v);
     }
-    put8(arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : st.from ? r.xt[0] : r.xt[1]), grow, gcol, r.mp, st.parts_out, w);
+    put8(arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : from ? r.xt[0] : r.xt[1]), grow, gcol, r.mp, parts_out, w);
   }
 }
 
@@ -720,6 +733,14 @@ inline bool within_range(double a, double b, double c, int steps) {
   return true;
 }
 
+struct Front {
+  int per, rows, cols;
+  int64_t base, bytes_or_records;
+  int from, parts_out;
+  float a, b, c;
+};
+#define S2L_FRONT_OF(f) (f).per, (f).rows, (f).cols, (f).base, (f).bytes_or_records, (f).from, (f).parts_out, (f).a, (f).b, (f).c, blocks
+
 struct Call {
   Alike alike;
   char* work;
@@ -727,7 +748,7 @@ struct Call {
   int dev;
 };
 
-template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int one(int blocks, const Call& c, const Step& s) {
+template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int one(int blocks, const Call& c, const Front& f, const Step& s) {
   using C = Core<TILE, PARTS, STAGES, KIND>;
   constexpr int lds = C::kLds > 4 * 32 * 33 * 4 ? C::kLds : 4 * 32 * 33 * 4;
   const auto kernel = product_kernel<TILE, PARTS, STAGES, KIND, MUON, T>;
@@ -736,21 +757,24 @@ template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int 
     const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, opted, c.dev);
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, c.st, c.work, c.alike, s);
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, c.st, c.work, S2L_FRONT_OF(f), c.alike, s);
   return (int)hipGetLastError();
 }
 
-template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, const Call& c, const Step& s) {
+template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, const Call& c, const Front& f, const Step& s) {
   constexpr int lds = Small<PARTS, KIND>::kLds;
   static_assert(lds <= 65536, "above 64 KiB the launch needs an opt-in");
-  hipLaunchKernelGGL((small_kernel<PARTS, KIND, MUON, T>), dim3(blocks), dim3(kThreads), lds, c.st, c.work, c.alike, s);
+  hipLaunchKernelGGL((small_kernel<PARTS, KIND, MUON, T>), dim3(blocks), dim3(kThreads), lds, c.st, c.work, S2L_FRONT_OF(f), c.alike, s);
   return (int)hipGetLastError();
 }
 
-template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, const Call& c, const Step& s) {
-  if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, s) : small<1, KIND, MUON, T>(blocks, c, s);
-  if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, s);
-  return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, s);
+template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, const Call& c, Front f, const Step& s) {
+  constexpr int kind = KIND == GRAM || KIND == POLY ? SYM : RECT;
+  f.per = c.alike.per[kind];
+  f.bytes_or_records = f.per ? c.alike.bytes : c.alike.records[kind - SYM];
+  if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, f, s) : small<1, KIND, MUON, T>(blocks, c, f, s);
+  if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
+  return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, f, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, f, s);
 }
 
 template <typename T, bool MUON>
@@ -774,17 +798,18 @@ int run(const s2l_matrix* in, int count, double a, double b, double c, float eps
     rc = (int)hipGetLastError();
     if (rc) return rc;
     for (int k = 0; k < steps; ++k) {
-      Step s{(float)a, (float)b, (float)c, k & 1, parts(k), shrink, nan_flags ? nan_flags + first : nullptr};
+      const Step s{shrink, nan_flags ? nan_flags + first : nullptr};
+      Front f{0, call.alike.mat.rows, call.alike.mat.cols, call.alike.mat.base, 0, k & 1, parts(k), (float)a, (float)b, (float)c};
       // (GRAM, POLY and APPLY do not depend on the matrices' type: one instance)
-      rc = any<GRAM, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, s);
+      rc = any<GRAM, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, f, s);
       if (rc) return rc;
-      rc = any<POLY, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, s);
+      rc = any<POLY, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, f, s);
       if (rc) return rc;
       if (k + 1 < steps) {
-        s.parts_out = parts(k + 1);
-        rc = any<APPLY, false, float>(l.tile_rect, parts(k), l.blocks[RECT], call, s);
+        f.parts_out = parts(k + 1);
+        rc = any<APPLY, false, float>(l.tile_rect, parts(k), l.blocks[RECT], call, f, s);
       } else {
-        rc = any<LAST, MUON, T>(l.tile_rect, parts(k), l.blocks[RECT], call, s);
+        rc = any<LAST, MUON, T>(l.tile_rect, parts(k), l.blocks[RECT], call, f, s);
       }
       if (rc) return rc;
     }
