@@ -12,7 +12,7 @@
 // every step would leave 2-4 % of error on matrices of fast falling spectrum, and bf16 products 15-30 %).
 // Values are scaled by 2^11: |X| <= ||X||_2 <= 1.2 and the entries of A and B <= 3.5 use the range of the halves from 2^-24 to 7168.
 //
-// All matrices of a call go through the same 2 + 3 * steps launches: one pass for the Frobenius norms (with the momentum update), one that scales
+// All matrices of a call go through the same 2 + 3 * steps launches (one more a step where a long Gram product is cut along k): one pass for the Frobenius norms (with the momentum update), one that scales
 // and splits into X^T, then per step the Gram product (symmetric: tiles on and below the diagonal, written twice), the polynomial (the same, its
 // epilogue adds a I + b A), and X <- B X, which leaves X^T or, last, writes the result: the rounded output, or the parameter's update.  X is held
 // transposed only: X <- B X reads it with k contiguous, the Gram product along its rows, through the transposing LDS read (X beside it cost
@@ -44,7 +44,7 @@ struct Mat {
   int stat;             // first partial sum of squares
 };
 
-enum { STAT = 0, PACK = 1, SYM = 2, RECT = 3, KINDS = 4 };      // the kinds of launches
+enum { STAT = 0, PACK = 1, SYM = 2, RECT = 3, DEEP = 4, KINDS = 5 };      // the kinds of launches (DEEP: the Gram products where some are cut along k)
 
 struct Table {
   int first[KINDS][kMaxMatrices];      // each matrix's first workgroup; 0x7fffffff behind the last matrix
@@ -53,6 +53,7 @@ struct Table {
 static_assert(sizeof(Table) <= 3840, "the table and a few scalars share the 4 KiB of kernel arguments");
 
 __host__ __device__ inline int padded(int v) { return (v + kPad - 1) / kPad * kPad; }
+__host__ __device__ inline int64_t tiles(int v, int tile) { return (padded(v) + tile - 1) / tile; }
 __host__ __device__ inline int64_t elements_of(const Mat& t) { return (int64_t)t.rows * t.cols; }
 __host__ __device__ inline int64_t chunk_of(int64_t elements) {      // elements of one workgroup of the first pass: a multiple of its 2048
   const int64_t c = (elements + kMaxPartials - 1) / kMaxPartials;
@@ -79,6 +80,20 @@ __host__ __device__ inline Arrays arrays_of(int rows, int cols) {
   return r;
 }
 
+constexpr int kWorthCutting = 1024;      // what a cut has to take off the longest workgroup's k: 20 us, against the join's 8
+// A long Gram product (n >> m) is cut along k into pieces of about `chunk`, whose sums join_kernel adds: see chunk_for.  0: none is.
+struct Pieces {
+  int count, depth;      // depth of each but the last: a multiple of 64
+};
+__host__ __device__ inline Pieces pieces_of(int np, int chunk) {
+  if (!chunk) return Pieces{1, np};
+  int count = (np + chunk / 2) / chunk;
+  count = count < 1 ? 1 : count > 16 ? 16 : count;
+  const int depth = (np / 64 + count - 1) / count * 64;
+  return np - depth < kWorthCutting ? Pieces{1, np} : Pieces{(np + depth - 1) / depth, depth};
+}
+__host__ __device__ inline int64_t sums_bytes(int count, int tiles) { return count > 1 ? (int64_t)count * tiles * 128 * 128 * 4 : 0; }
+
 constexpr int64_t kTableBytes = 4096;
 constexpr int64_t partial_bytes(int stat_blocks) { return ((int64_t)stat_blocks * 8 + 255) / 256 * 256; }
 
@@ -94,19 +109,20 @@ __device__ __forceinline__ int owner(const int* first, int id) {
 // workgroup, which the first pass writes (one round trip; looking through the table took two).
 struct Record {
   int64_t base;
-  int rows, cols, index, id, pad[2];
+  int rows, cols, index, id, piece, pad;
 };
 struct Alike {
   Mat mat;
   int per[KINDS];      // workgroups of one matrix; 0: not alike, look into the records
   int stride;          // bytes from one input / output to the next (at most 56 of them: below 2^31 checked)
   int64_t bytes;       // of one matrix's arrays
-  int64_t records[2];  // byte offset of the records of SYM and RECT launches in the workspace
+  int64_t records[3];  // byte offset of the records of SYM, RECT and DEEP launches in the workspace
 };
 struct Place {
   Mat mat;        // (in, out, momentum, step: where alike; else look at Table::mat[index] for them)
   int index;      // of the matrix
-  int id;         // workgroup within the matrix
+  int id;         // workgroup within the matrix (DEEP: within the piece)
+  int piece;
 };
 __device__ __forceinline__ Place alike_place(const Alike& alike, int kind, int id) {
   const int k = id / alike.per[kind];
@@ -115,7 +131,7 @@ __device__ __forceinline__ Place alike_place(const Alike& alike, int kind, int i
   m.out = static_cast<char*>(m.out) + (int64_t)k * alike.stride;
   m.base += k * alike.bytes;
   m.stat += k * alike.per[STAT];
-  return Place{m, k, id - k * alike.per[kind]};
+  return Place{m, k, id - k * alike.per[kind], 0};
 }
 // What every workgroup of a product needs first: plain scalars at the front of the kernel's arguments, which the hardware puts into scalar registers
 // with the wave (the build asks for 16 dwords of it), so that matrices alike need no load at all before their first operand request.
@@ -137,6 +153,7 @@ __device__ __forceinline__ Place place_of(const char* work, int per, int rows, i
   p.mat.cols = __builtin_amdgcn_readfirstlane(rec->cols);
   p.index = __builtin_amdgcn_readfirstlane(rec->index);
   p.id = __builtin_amdgcn_readfirstlane(rec->id);
+  p.piece = __builtin_amdgcn_readfirstlane(rec->piece);
   return p;
 }
 // a PACK launch's, from the table (once a call); a result's destination
@@ -144,7 +161,7 @@ __device__ __forceinline__ Place pack_place(const char* work, const Alike& alike
   if (alike.per[0]) return alike_place(alike, PACK, id);
   const Table* t = reinterpret_cast<const Table*>(work);
   const int k = owner(t->first[PACK], id);
-  return Place{t->mat[k], k, id - t->first[PACK][k]};
+  return Place{t->mat[k], k, id - t->first[PACK][k], 0};
 }
 __device__ __forceinline__ void destination(const char* work, const Alike& alike, Place& p) {
   if (alike.per[0]) {
@@ -178,6 +195,12 @@ __device__ __forceinline__ void store8f(float* p, int64_t left, const float* v) 
   }
 }
 
+// the records' places in the workspace and their numbers: SYM, RECT, DEEP
+struct Lists {
+  int64_t at[3];
+  int count[3];
+};
+
 struct Momentum {
   float mu;
   int nesterov;
@@ -185,21 +208,27 @@ struct Momentum {
 
 // ---- first pass: the sums of squares in 64 bits (every later product scales with the norm: a sum over millions of squares in 32 bits is off by
 // more than all other roundings together), with the momentum update.  Memory bound: reads g, reads and writes m.
-template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, char* work, Momentum mo, int64_t sym_records, int64_t rect_records, int syms, int rects) {
+template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void norm_kernel(Table t, char* work, Momentum mo, Lists lists) {
   __shared__ double part[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x == 0) {      // the table for the launches that follow
     const uint32_t* src = reinterpret_cast<const uint32_t*>(&t);
     for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += kThreads) reinterpret_cast<uint32_t*>(work)[i] = src[i];
   }
-  // ... and the records (syms == rects == 0: matrices alike, none are wanted)
-  for (int i = blockIdx.x * kThreads + threadIdx.x; i < syms + rects; i += gridDim.x * kThreads) {
-    const bool rect = i >= syms;
-    const int id = rect ? i - syms : i;
-    const int* first = rect ? t.first[RECT] : t.first[SYM];
+  // ... and the records (none where matrices are alike)
+  const int syms = lists.count[0], rects = lists.count[1];
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < syms + rects + lists.count[2]; i += gridDim.x * kThreads) {
+    const int list = i < syms ? 0 : i < syms + rects ? 1 : 2, id = i - (list == 0 ? 0 : list == 1 ? syms : syms + rects);
+    const int* first = list == 0 ? t.first[SYM] : list == 1 ? t.first[RECT] : t.first[DEEP];
     int k = 0;
     while (k + 1 < kMaxMatrices && first[k + 1] <= id) ++k;
-    reinterpret_cast<Record*>(work + (rect ? rect_records : sym_records))[id] = Record{t.mat[k].base, t.mat[k].rows, t.mat[k].cols, k, id - first[k], {0, 0}};
+    Record rec{t.mat[k].base, t.mat[k].rows, t.mat[k].cols, k, id - first[k], 0, 0};
+    if (list == 2) {      // piece by piece: neighbours read the same rows
+      const int side = (int)tiles(rec.rows < rec.cols ? rec.rows : rec.cols, 128), all = side * (side + 1) / 2;
+      rec.piece = rec.id / all;
+      rec.id -= rec.piece * all;
+    }
+    reinterpret_cast<Record*>(work + (list == 0 ? lists.at[0] : list == 1 ? lists.at[1] : lists.at[2]))[id] = rec;
   }
   const Mat& mat = t.mat[owner(t.first[STAT], blockIdx.x)];
   const int64_t total = elements_of(mat), chunk = chunk_of(total);
@@ -314,37 +343,66 @@ template <typename T, bool MUON> __global__ __launch_bounds__(kThreads) void spl
   }
 }
 
-enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
+enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3, CUT = 4 };      // CUT: Gram products, some of them in pieces
 
 // from: which of the two X^T arrays holds this step's; parts_out: halves that the next reader wants; coef_*: the step's coefficients
 struct Step {
   float shrink;         // LAST, Muon: 1 - lr wd
   int* nan_flags;       // LAST, Muon: one int per matrix, set where the parameter as read holds a NaN
+  int chunk;            // CUT: as pieces_of takes it
 };
 
 // Tiles: 128 x 128 by four waves of 64 x 64 (two halves: 32 k a stage, two workgroups to a CU), or 64 x 64 by four of 32 x 32.  Else 64 k a stage.
-template <int TILE, int PARTS, int STAGES, int KIND>
-using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, KIND != GRAM, KIND != GRAM, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES>;
+// GROUPS 2: eight waves, each four of them on every other k-step, for launches of one workgroup to a CU at most: see groups_for.
+template <int TILE, int PARTS, int STAGES, int KIND, int GROUPS>
+using Core = core::Product<_Float16, TILE, TILE, 2, 2, PARTS, KIND != GRAM && KIND != CUT, KIND != GRAM && KIND != CUT, TILE == 128 && PARTS == 2 ? 64 : 128, STAGES, GROUPS>;
 
-template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T>
-__global__ __launch_bounds__(kThreads, 2) void product_kernel(S2L_FRONT, Alike alike, Step st) {
-  using C = Core<TILE, PARTS, STAGES, KIND>;
+// a 32 x 32 block in LDS (rows of 33) to its place at (rb, cb), and mirrored: 32 rows of four pieces, two pieces a lane
+template <bool PLAIN> __device__ __forceinline__ void put_block(_Float16* to, const uint32_t* scratch, int rb, int cb, int ld, int parts, bool mirrored, int lane) {
+#pragma unroll
+  for (int e = 0; PLAIN && e < 2; ++e) {
+    const int row = (lane >> 2) + 16 * e, c = lane & 3;
+    uint32_t w[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
+    put8(to, rb + row, cb + 8 * c, ld, parts, w);
+  }
+  if (mirrored) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = (lane >> 2) + 16 * e, c = lane & 3;
+      uint32_t w[8];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
+      put8(to, cb + row, rb + 8 * c, ld, parts, w);
+    }
+  }
+}
+
+// tile id of the lower triangle: id = ti (ti + 1) / 2 + tj
+__device__ __forceinline__ void triangle(int id, int& ti, int& tj) {
+  ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+  while (ti * (ti + 1) / 2 > id) --ti;
+  while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+  tj = id - ti * (ti + 1) / 2;
+}
+
+template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T, int GROUPS>
+__global__ __launch_bounds__(GROUPS * kThreads, GROUPS == 2 ? 1 : 2) void product_kernel(S2L_FRONT, Alike alike, Step st) {
+  using C = Core<TILE, PARTS, STAGES, KIND, GROUPS>;
   constexpr int W = TILE / 2, F = W / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr bool kSym = KIND == GRAM || KIND == POLY;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = GROUPS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  const int part = wave & 3;      // of the tile
+  constexpr bool kGram = KIND == GRAM || KIND == CUT, kSym = kGram || KIND == POLY;
   Place at0 = place_of(S2L_FRONT_PASS, core::xcd_order(blockIdx.x, blocks));
   if constexpr (KIND == LAST) destination(work, alike, at0);
   const Mat& mat = at0.mat;
   const Arrays r = arrays_of(mat.rows, mat.cols);
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
   int ti, tj;
-  if constexpr (kSym) {      // tile id of the lower triangle: id = ti (ti + 1) / 2 + tj
-    const int id = at0.id;
-    ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-    while (ti * (ti + 1) / 2 > id) --ti;
-    while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
-    tj = id - ti * (ti + 1) / 2;
+  if constexpr (kSym) {
+    triangle(at0.id, ti, tj);
   } else {
     const int id = at0.id, tiles_n = (r.np + TILE - 1) / TILE;
     ti = id / tiles_n;
@@ -352,23 +410,18 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(S2L_FRONT, Alike a
   }
   const int m0 = ti * TILE, n0 = tj * TILE;
 
+  int depth = kGram ? r.np : r.mp, k0 = 0;
+  [[maybe_unused]] Pieces pieces{1, 0};
+  if constexpr (KIND == CUT) {
+    pieces = pieces_of(r.np, st.chunk);
+    k0 = at0.piece * pieces.depth;
+    depth = r.np - k0 < pieces.depth ? r.np - k0 : pieces.depth;
+  }
   typename C::SA sa;
   typename C::SB sb;
-  int depth;
-  if constexpr (KIND == GRAM) {
-    const _Float16* xt = arrays + (from ? r.xt[1] : r.xt[0]);
-    sa.setup(xt, r.mp, m0, r.mp, 0, wave, lane);
-    sb.setup(xt, r.mp, n0, r.mp, 0, wave, lane);
-    depth = r.np;
-  } else if constexpr (KIND == POLY) {
-    sa.setup(arrays + r.a, r.mp, m0, r.mp, 0, wave, lane);
-    sb.setup(arrays + r.a, r.mp, n0, r.mp, 0, wave, lane);
-    depth = r.mp;
-  } else {
-    sa.setup(arrays + r.b, r.mp, m0, r.mp, 0, wave, lane);
-    sb.setup(arrays + (from ? r.xt[1] : r.xt[0]), r.mp, n0, r.np, 0, wave, lane);
-    depth = r.mp;
-  }
+  const _Float16* xt = arrays + (from ? r.xt[1] : r.xt[0]);
+  sa.setup(kGram ? xt : KIND == POLY ? arrays + r.a : arrays + r.b, r.mp, m0, r.mp, k0, wave, lane);
+  sb.setup(KIND == POLY ? arrays + r.a : xt, r.mp, n0, kSym ? r.mp : r.np, k0, wave, lane);
   f16v acc[F][F];
 #pragma unroll
   for (int i = 0; i < F; ++i)
@@ -380,23 +433,64 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(S2L_FRONT, Alike a
   constexpr bool kAhead = KIND == POLY && F == 1;
   uint64_t own[kAhead ? 4 : 1][PARTS];
   if constexpr (kAhead) {
-    const _Float16* a = arrays + r.a + core::pair_at<PARTS>(m0 + (wave >> 1) * W + (lane & 31), n0 + (wave & 1) * W, r.mp) + 4 * (lane >> 5);
+    const _Float16* a = arrays + r.a + core::pair_at<PARTS>(m0 + (part >> 1) * W + (lane & 31), n0 + (part & 1) * W, r.mp) + 4 * (lane >> 5);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) __builtin_memcpy(&own[q][p], a + 8 * q + p * core::kPairs, 8);
   }
   C::run(sa, sb, depth / C::BK, smem, acc, wave, lane, [](auto&) {});
+  constexpr int kSums = GROUPS == 2 ? 2 * 4 * F * 4 * 64 * 16 : 0;
+  if constexpr (GROUPS == 2) {      // each group hands the other's half of the rows over, in whole pieces, and goes on with its own
+    static_assert(F == 2, "a block of rows for each group");
+    f4* sums = reinterpret_cast<f4*>(smem);
+    const auto at = [&](int reader, int j, int q) { return (((reader * 4 + part) * F + j) * 4 + q) * 64 + lane; };
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      if (i == group) continue;
+#pragma unroll
+      for (int j = 0; j < F; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sums[at(i, j, q)] = f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      if (i != group) continue;
+#pragma unroll
+      for (int j = 0; j < F; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4 o = sums[at(i, j, q)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += o[e];
+        }
+    }
+  }
 
+  if constexpr (KIND == CUT) {
+    if (pieces.count > 1) {      // raw sums, 1 KiB a store, in the order in which join_kernel reads them
+      const int side = (int)tiles(r.m, TILE);
+      f4* to = reinterpret_cast<f4*>(arrays + r.total) + ((int64_t)at0.piece * (side * (side + 1) / 2) + at0.id) * (TILE * TILE / 4) + lane;
+#pragma unroll
+      for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) to[(((wave * F + i) * F + j) * 4 + q) * 64] = f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      return;
+    }
+  }
   // lane: row lane & 31 of a 32 x 32 block, register q: column 8 (q / 4) + 4 (lane / 32) + q % 4.  Through LDS, a block at a time and a wave by
   // itself, so that both orientations leave as whole 16-byte pieces.
-  const int wm = m0 + (wave >> 1) * W, wn = n0 + (wave & 1) * W;
+  const int wm = m0 + (part >> 1) * W, wn = n0 + (part & 1) * W;
   const int rows_end = r.mp, cols_end = kSym ? r.mp : r.np;
   if (wm >= rows_end || wn >= cols_end) return;      // (a 128-wide tile of an odd number of 64s)
-  uint32_t* scratch = reinterpret_cast<uint32_t*>(smem) + wave * 32 * 33;
+  uint32_t* scratch = reinterpret_cast<uint32_t*>(smem + kSums) + wave * 32 * 33;
   const int li = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int i = 0; i < F; ++i) {
+    if (GROUPS == 2 && i != group) continue;
 #pragma unroll
     for (int j = 0; j < F; ++j) {
       const int rb = wm + 32 * i, cb = wn + 32 * j;
@@ -458,31 +552,50 @@ __global__ __launch_bounds__(kThreads, 2) void product_kernel(S2L_FRONT, Alike a
         }
         if (MUON && bad && st.nan_flags) st.nan_flags[at0.index] = 1;
       } else {
-        // 32 rows of four pieces, two pieces a lane: the symmetric ones as they are and mirrored, X^T mirrored
-        _Float16* to = arrays + (KIND == GRAM ? r.a : KIND == POLY ? r.b : from ? r.xt[0] : r.xt[1]);
-#pragma unroll
-        for (int e = 0; kSym && e < 2; ++e) {
-          const int row = (lane >> 2) + 16 * e, c = lane & 3;
-          uint32_t w[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) w[x] = scratch[row * 33 + 8 * c + x];
-          put8(to, rb + row, cb + 8 * c, r.mp, parts_out, w);
-        }
-        if (!kSym || ti != tj) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = (lane >> 2) + 16 * e, c = lane & 3;
-            uint32_t w[8];
-#pragma unroll
-            for (int x = 0; x < 8; ++x) w[x] = scratch[(8 * c + x) * 33 + row];
-            put8(to, cb + row, rb + 8 * c, r.mp, parts_out, w);
-          }
-        }
+        put_block<kSym>(arrays + (kGram ? r.a : KIND == POLY ? r.b : from ? r.xt[0] : r.xt[1]), scratch, rb, cb, r.mp, parts_out, !kSym || ti != tj, lane);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
   }
+}
+
+// A = the sum of its pieces, in their order.  A wave: a 32 x 32 block; memory bound (4 bytes a piece read, 8 or 4 written an element).
+__global__ __launch_bounds__(kThreads) void join_kernel(char* work, int64_t records, int parts_out, int chunk) {
+  __shared__ uint32_t blocks[4][32 * 33];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Place at0 = place_of(work, 0, 0, 0, 0, records, blockIdx.x >> 2);
+  const Arrays r = arrays_of(at0.mat.rows, at0.mat.cols);
+  const Pieces pieces = pieces_of(r.np, chunk);
+  if (pieces.count == 1) return;
+  _Float16* arrays = reinterpret_cast<_Float16*>(work + at0.mat.base);
+  const int side = (int)tiles(r.m, 128), all = side * (side + 1) / 2;
+  int ti, tj;
+  triangle(at0.id, ti, tj);
+  const int block = (blockIdx.x & 3) * 4 + wave;      // (wave of the product, i, j)
+  const int rb = ti * 128 + (block >> 3) * 64 + (block >> 1 & 1) * 32, cb = tj * 128 + (block >> 2 & 1) * 64 + (block & 1) * 32;
+  if (rb >= r.mp || cb >= r.mp) return;
+  const f4* from = reinterpret_cast<const f4*>(arrays + r.total) + (int64_t)at0.id * 4096 + block * 256 + lane;
+  f4 sum[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sum[q] = from[q * 64];
+  for (int p = 1; p < pieces.count; ++p) {
+    f4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = from[(int64_t)p * all * 4096 + q * 64];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[q][e] += v[q][e];
+  }
+  uint32_t* scratch = blocks[wave];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) scratch[(lane & 31) * 33 + 8 * q + 4 * (lane >> 5) + e] = halves(sum[q][e] * (1.f / kScale));
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  put_block<true>(arrays + r.a, scratch, rb, cb, r.mp, parts_out, ti != tj, lane);
 }
 
 // ---- few and small matrices: 32 x 32 tiles, the k-steps of a stage dealt to the four waves ------------------------------------------------
@@ -516,11 +629,7 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(S2L_FRONT, Alike ali
   _Float16* arrays = reinterpret_cast<_Float16*>(work + mat.base);
   int ti, tj;
   if constexpr (kSym) {
-    const int id = at0.id;
-    ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-    while (ti * (ti + 1) / 2 > id) --ti;
-    while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
-    tj = id - ti * (ti + 1) / 2;
+    triangle(at0.id, ti, tj);
   } else {
     ti = at0.id / (r.np / 32);
     tj = at0.id - ti * (r.np / 32);
@@ -640,18 +749,35 @@ constexpr int kMaxSteps = 100;
 struct Layout {
   int tile_sym, tile_rect;
   int blocks[KINDS];
-  int64_t sym_records, rect_records;      // byte offsets
+  int64_t records[3];      // byte offsets: SYM, RECT, DEEP
+  int chunk;               // of Gram products in pieces; 0: none
   int64_t bytes;
 };
 
-inline int64_t tiles(int v, int tile) { return (padded(v) + tile - 1) / tile; }
-
 // Table and workspace of one set of launches.  128-wide tiles where they alone occupy half of the part's 256 CUs (they read half as much per
 // product and their waves twice as little of LDS), else 64-wide ones: four times the workgroups; 32-wide where those are too few as well.
-#ifndef EXP_T32
-#define EXP_T32 128
-#endif
-inline int tile_for(int64_t of128, int64_t of64) { return of128 >= 128 ? 128 : of64 >= EXP_T32 ? 64 : 32; }
+inline int tile_for(int64_t of128, int64_t of64) { return of128 >= 128 ? 128 : of64 >= 128 ? 64 : 32; }
+
+// Two groups of waves where 128-wide tiles give no CU a second workgroup, whose waves would work while the first one's
+// wait (a call of one 2048 x 2048 in fp32: 333 against 376 us; of four 1024 x 1024: 186 against 222).
+inline int groups_for(int blocks) { return blocks <= 256 ? 2 : 1; }
+
+// How long the pieces are: half of what a CU has to do on average (it runs two workgroups), where the longest product is so much longer that the
+// other CUs would wait for it; only in 128-wide tiles (0.02 us per k of a workgroup's).  Four 1024 x 1024 with a 1024 x 4096 and its transpose, a
+// step: 1079 us uncut, 971 cut; with pieces half as long 1040 against 943 (products that stay whole are then twice as long as the
+// pieces, and whole ones fill some XCDs, pieces others); two 2048 x 5504 in bf16: 1032 against 1020.
+inline int chunk_for(const s2l_matrix* in, int count) {
+  int64_t work = 0;
+  int longest = 0;
+  for (int i = 0; i < count; ++i) {
+    const int m = in[i].rows < in[i].cols ? in[i].rows : in[i].cols, np = padded(in[i].rows < in[i].cols ? in[i].cols : in[i].rows);
+    work += tiles(m, 128) * (tiles(m, 128) + 1) / 2 * np;
+    longest = np > longest ? np : longest;
+  }
+  int64_t chunk = work / 512;
+  if (chunk < 512) chunk = 512;
+  return pieces_of(longest, (int)(chunk < longest ? chunk : longest)).count > 1 ? (int)chunk : 0;
+}
 
 inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
   int64_t sym[2] = {}, rect[2] = {};
@@ -665,6 +791,7 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
   }
   l->tile_sym = tile_for(sym[0], sym[1]);
   l->tile_rect = tile_for(rect[0], rect[1]);
+  l->chunk = l->tile_sym == 128 ? chunk_for(in, count) : 0;
   int64_t at[KINDS] = {}, base = 0;
   for (int i = 0; i < kMaxMatrices; ++i)
     for (int k = 0; k < KINDS; ++k) t->first[k][i] = 0x7fffffff;
@@ -685,13 +812,18 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
     at[PACK] += (int64_t)(r.mp / 64) * (r.np / 64);
     at[SYM] += ts * (ts + 1) / 2;
     at[RECT] += tiles(r.m, l->tile_rect) * tiles(r.n, l->tile_rect);
-    base += r.total * 2;
-    if (at[PACK] > 0x3ffffff0 || at[SYM] > 0x3ffffff0 || at[RECT] > 0x3ffffff0) return S2L_E_SIZE;
+    const int cut = pieces_of(r.np, l->chunk).count;
+    at[DEEP] += l->chunk ? cut * (ts * (ts + 1) / 2) : 0;
+    base += r.total * 2 + sums_bytes(cut, (int)(ts * (ts + 1) / 2));
+    if (at[PACK] > 0x3ffffff0 || at[SYM] > 0x3ffffff0 || at[RECT] > 0x3ffffff0 || at[DEEP] > 0x3ffffff0) return S2L_E_SIZE;
   }
   for (int k = 0; k < KINDS; ++k) l->blocks[k] = (int)at[k];
-  l->sym_records = kTableBytes + partial_bytes((int)at[STAT]);
-  l->rect_records = l->sym_records + at[SYM] * (int64_t)sizeof(Record);
-  const int64_t front = (l->rect_records + at[RECT] * (int64_t)sizeof(Record) + 255) / 256 * 256;
+  int64_t front = kTableBytes + partial_bytes((int)at[STAT]);
+  for (int k = 0; k < 3; ++k) {
+    l->records[k] = front;
+    front += at[SYM + k] * (int64_t)sizeof(Record);
+  }
+  front = (front + 255) / 256 * 256;
   for (int i = 0; i < count; ++i) t->mat[i].base += front;
   l->bytes = front + base;
   return 0;
@@ -699,10 +831,10 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
 
 inline Alike alike_of(const Table& t, const Layout& l, int count, int size, bool muon) {
   Alike a{};
-  a.records[0] = l.sym_records;
-  a.records[1] = l.rect_records;
+  for (int k = 0; k < 3; ++k) a.records[k] = l.records[k];
   a.mat = t.mat[0];
   const int64_t stride = count > 1 ? static_cast<const char*>(t.mat[1].in) - static_cast<const char*>(t.mat[0].in) : 0;
+  if (l.chunk) return a;
   if (count > 1 && (muon || stride < 0 || stride > 0x7fffffff / count)) return a;
   for (int i = 1; i < count; ++i)
     if (t.mat[i].rows != a.mat.rows || t.mat[i].cols != a.mat.cols || static_cast<const char*>(t.mat[i].in) != static_cast<const char*>(a.mat.in) + i * stride ||
@@ -748,16 +880,17 @@ struct Call {
   int dev;
 };
 
-template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T> int one(int blocks, const Call& c, const Front& f, const Step& s) {
-  using C = Core<TILE, PARTS, STAGES, KIND>;
-  constexpr int lds = C::kLds > 4 * 32 * 33 * 4 ? C::kLds : 4 * 32 * 33 * 4;
-  const auto kernel = product_kernel<TILE, PARTS, STAGES, KIND, MUON, T>;
+template <int TILE, int PARTS, int STAGES, int KIND, bool MUON, typename T, int GROUPS = 1> int one(int blocks, const Call& c, const Front& f, const Step& s) {
+  using C = Core<TILE, PARTS, STAGES, KIND, GROUPS>;
+  constexpr int epilogue = GROUPS * 4 * 32 * 33 * 4 + (GROUPS == 2 ? 65536 : 0), lds = C::kLds > epilogue ? C::kLds : epilogue;
+  static_assert(lds <= 160 * 1024, "");
+  const auto kernel = product_kernel<TILE, PARTS, STAGES, KIND, MUON, T, GROUPS>;
   if constexpr (lds > 65536) {
     static LdsOptIn opted;
     const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, opted, c.dev);
     if (rc) return rc;
   }
-  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), lds, c.st, c.work, S2L_FRONT_OF(f), c.alike, s);
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(GROUPS * kThreads), lds, c.st, c.work, S2L_FRONT_OF(f), c.alike, s);
   return (int)hipGetLastError();
 }
 
@@ -769,12 +902,14 @@ template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, cons
 }
 
 template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, const Call& c, Front f, const Step& s) {
-  constexpr int kind = KIND == GRAM || KIND == POLY ? SYM : RECT;
+  constexpr int kind = KIND == CUT ? DEEP : KIND == GRAM || KIND == POLY ? SYM : RECT;
   f.per = c.alike.per[kind];
   f.bytes_or_records = f.per ? c.alike.bytes : c.alike.records[kind - SYM];
-  if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, f, s) : small<1, KIND, MUON, T>(blocks, c, f, s);
-  if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
-  return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, f, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, f, s);
+  if constexpr (KIND == CUT) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
+  else if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, f, s) : small<1, KIND, MUON, T>(blocks, c, f, s);
+  else if (tile == 128 && groups_for(blocks) == 2) return parts == 2 ? one<128, 2, 4, KIND, MUON, T, 2>(blocks, c, f, s) : one<128, 1, 4, KIND, MUON, T, 2>(blocks, c, f, s);
+  else if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
+  else return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, f, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, f, s);
 }
 
 template <typename T, bool MUON>
@@ -790,18 +925,29 @@ int run(const s2l_matrix* in, int count, double a, double b, double c, float eps
     if (rc) return rc;
     const Call call{alike_of(t, l, n, sizeof(T), MUON), work, st, dev};
     const auto parts = [&](int k) { return !std::is_same_v<T, __bf16> || k < steps - 2 ? 2 : 1; };
-    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo, l.sym_records, l.rect_records, call.alike.per[0] ? 0 : l.blocks[SYM],
-                       call.alike.per[0] ? 0 : l.blocks[RECT]);
+    Lists lists{};
+    for (int k = 0; k < 3 && !call.alike.per[0]; ++k) {
+      lists.at[k] = l.records[k];
+      lists.count[k] = l.blocks[SYM + k];
+    }
+    hipLaunchKernelGGL((norm_kernel<T, MUON>), dim3(l.blocks[STAT]), dim3(kThreads), 0, st, t, work, mo, lists);
     rc = (int)hipGetLastError();
     if (rc) return rc;
     hipLaunchKernelGGL((split_kernel<T, MUON>), dim3(l.blocks[PACK]), dim3(kThreads), 0, st, work, call.alike, mo, eps, parts(0));
     rc = (int)hipGetLastError();
     if (rc) return rc;
     for (int k = 0; k < steps; ++k) {
-      const Step s{shrink, nan_flags ? nan_flags + first : nullptr};
+      const Step s{shrink, nan_flags ? nan_flags + first : nullptr, l.chunk};
       Front f{0, call.alike.mat.rows, call.alike.mat.cols, call.alike.mat.base, 0, k & 1, parts(k), (float)a, (float)b, (float)c};
       // (GRAM, POLY and APPLY do not depend on the matrices' type: one instance)
-      rc = any<GRAM, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, f, s);
+      if (l.chunk) {
+        rc = any<CUT, false, float>(l.tile_sym, parts(k), l.blocks[DEEP], call, f, s);
+        if (rc) return rc;
+        hipLaunchKernelGGL(join_kernel, dim3(4 * l.blocks[SYM]), dim3(kThreads), 0, st, work, l.records[0], parts(k), l.chunk);
+        rc = (int)hipGetLastError();
+      } else {
+        rc = any<GRAM, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, f, s);
+      }
       if (rc) return rc;
       rc = any<POLY, false, float>(l.tile_sym, parts(k), l.blocks[SYM], call, f, s);
       if (rc) return rc;

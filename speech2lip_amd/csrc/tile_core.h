@@ -144,9 +144,10 @@ template <typename T, int ROWS, bool KC, int ROWB, int PARTS, int WAVES> struct 
   }
 };
 
-// BM x BN outputs per workgroup, WM x WN waves.  PARTS 2: hi + lo halves of both operands, three products per pair (lo lo is below fp32's rounding).
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool AKC, bool BKC, int ROWB, int STAGES> struct Product {
-  static constexpr int kWaves = WAVES_M * WAVES_N, kThreads = 64 * kWaves;
+// BM x BN outputs per workgroup, WM x WN waves (KGROUPS times: group g of them takes every KGROUPS-th k-step, and the caller adds the groups' sums).
+// PARTS 2: hi + lo halves of both operands, three products per pair (lo lo is below fp32's rounding).
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool AKC, bool BKC, int ROWB, int STAGES, int KGROUPS = 1, bool AHEAD = (KGROUPS > 1)> struct Product {
+  static constexpr int kWaves = WAVES_M * WAVES_N * KGROUPS, kThreads = 64 * kWaves;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, FM = WM / 32, FN = WN / 32;
   using SA = Stream<T, BM, AKC, ROWB, PARTS, kWaves>;
   using SB = Stream<T, BN, BKC, ROWB, PARTS, kWaves>;
@@ -175,7 +176,8 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool 
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem);
     const int tiles = __builtin_amdgcn_readfirstlane(count);
     const int uwave = __builtin_amdgcn_readfirstlane(wave);
-    const int wm = (wave / WAVES_N) * WM, wn = (wave % WAVES_N) * WN;
+    [[maybe_unused]] const int group = uwave / (WAVES_M * WAVES_N);
+    const int wm = (wave / WAVES_N % WAVES_M) * WM, wn = (wave % WAVES_N) * WN;
     int put = 0, get = 0;      // stage to fill, stage to use
     auto fill = [&]() {
       a.issue(lds0 + put * kStage, uwave);
@@ -183,6 +185,55 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int PARTS, bool 
       put = put + 1 == STAGES ? 0 : put + 1;
     };
     asm volatile("s_nop 4" : : : "memory");      // scalar registers that a vector instruction wrote, read by the assembly text's loads
+    if constexpr (AHEAD) {
+      // One workgroup alone on its CU: its waves run in step, so what they do one after the other the CU does one after the other.  Each k-tile's
+      // fragments are therefore read between the products of the tile before.
+      constexpr int kSteps = ROWB / 32 / KGROUPS, kReads = kSteps * PARTS * (FM + FN), kProducts = kSteps * (2 * PARTS - 1) * FM * FN;
+      static_assert(kReads <= kProducts, "");
+      u4 frag[2][kSteps][PARTS][FM + FN];      // A's, then B's
+      auto read = [&](int set, const char* lds, int u) __attribute__((always_inline)) {
+        const int f = u % (FM + FN), q = u / (FM + FN) % PARTS, s = u / (FM + FN) / PARTS;
+        frag[set][s][q][f] = f < FM ? LA::fragment(lds + q * LA::kBytes, wm + 32 * f, s * KGROUPS + group, lane)
+                                    : LB::fragment(lds + PARTS * LA::kBytes + q * LB::kBytes, wn + 32 * (f - FM), s * KGROUPS + group, lane);
+      };
+      auto next = [&]() __attribute__((always_inline)) {
+        const char* lds = smem + get * kStage;
+        get = get + 1 == STAGES ? 0 : get + 1;
+        return lds;
+      };
+      auto step = [&](int set, int kt) __attribute__((always_inline)) {      // k-tile kt, whose fragments are on their way to `set`
+        wait_younger<STAGES - 2>(tiles - 2 - kt > 0 ? tiles - 2 - kt : 0);      // k-tile kt + 1 has landed, and this wave has read k-tile kt
+        __builtin_amdgcn_s_barrier();                                          // ... everybody's, everybody has
+        asm volatile("" : : : "memory");
+        const char* lds = next();      // (behind the last k-tile: what lies there, unused)
+#pragma unroll
+        for (int t = 0; t < kProducts; ++t) {
+          const int j = t % FN, i = t / FN % FM, p = 2 * PARTS - 2 - t / (FN * FM) % (2 * PARTS - 1), s = t / (FN * FM) / (2 * PARTS - 1);
+          acc[i][j] = mma<T>(frag[set][s][p == 2][FM + j], frag[set][s][p == 1][i], acc[i][j]);      // lo hi, hi lo, hi hi: the small products first
+          __builtin_amdgcn_sched_barrier(0);
+          if (t < kReads) read(set ^ 1, lds, t);
+          if (t == kReads - 1 && kt + STAGES < tiles) fill();      // into k-tile kt's place
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      for (int s = 0; s < STAGES && s < tiles; ++s) fill();
+      wait_younger<STAGES - 1>(tiles - 1);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : : : "memory");
+      const char* first = next();
+#pragma unroll
+      for (int u = 0; u < kReads; ++u) read(0, first, u);
+      int kt = 0;
+      for (; kt + 1 < tiles; kt += 2) {
+        step(0, kt);
+        step(1, kt + 1);
+      }
+      if (kt < tiles) step(0, kt);
+      wait<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : : : "memory");
+      return;
+    }
     for (int s = 0; s < STAGES - 1 && s < tiles; ++s) fill();
     for (int kt = 0; kt < tiles; ++kt) {
       // k-tile kt has landed when at most the younger ones' requests are outstanding (loads retire in order)

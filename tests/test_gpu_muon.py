@@ -105,6 +105,42 @@ def test_large_and_wide_tiles(dev):
 
 
 @pytest.mark.gpu
+def test_long_gram_products_in_pieces(dev):
+    """Lists whose 128-wide tiles are enough for the part, with matrices so long that their Gram products are cut along k: uneven pieces, sides of
+    an odd number of 64s, more than sixteen pieces' worth of length, matrices beside them that stay whole; a workspace of NaN, guarded ends."""
+    lib = _abi.load()
+    lists = [[(1024, 1024)] * 2 + [(1000, 4100), (4096, 1024), (1100, 1090), (963, 4099)], [(640, 5000)] * 9, [(130, 30000)] + [(900, 1030)] * 5]
+    for dt, dtype in ((0, torch.float32), (1, torch.bfloat16), (2, torch.float16)):
+        for shapes in lists:
+            gs = [matrix(*s, "plain", dev, seed=i).to(dtype) for i, s in enumerate(shapes)]
+            outs = [torch.full((g.numel() + 80,), 7.0, dtype=dtype, device=dev) for g in gs]
+            size = outs[0].element_size()
+            table = optim._matrix_table([(g.data_ptr(), o.data_ptr() + 40 * size, 0, *g.shape, 0.0) for g, o in zip(gs, outs)])
+            need = lib.s2l_orthogonalize_work_bytes(table, len(gs))
+            work = torch.full((need + 256,), 255, dtype=torch.uint8, device=dev)
+            for again in range(2):
+                _abi.check(lib.s2l_orthogonalize(dt, table, len(gs), *ABC, 1e-7, 5, work.data_ptr(), torch.cuda.current_stream().cuda_stream), "orth")
+                now = [o[40:-40].reshape(g.shape).clone() for o, g in zip(outs, gs)]
+                assert again == 0 or all(torch.equal(a, b) for a, b in zip(first, now))
+                first = now
+            assert all(bool((o[:40] == 7).all()) and bool((o[-40:] == 7).all()) for o in outs) and bool((work[need:] == 255).all())
+            for i in {s: i for i, s in enumerate(shapes)}.values():
+                hold(first[i], gs[i], shapes[i])
+
+
+@pytest.mark.gpu
+def test_single_launches_of_few_workgroups(dev):
+    """128-wide tiles of at most one workgroup to a CU: two groups of waves share k."""
+    for dtype in TYPES:
+        for shape in ((4, 1024, 1024), (1, 1990, 2050), (5, 700, 1000)):
+            g = torch.stack([matrix(*shape[1:], "falling", dev, seed=s) for s in range(shape[0])]).to(dtype)
+            got = optim.orthogonalize(g)
+            assert torch.equal(got, optim.orthogonalize(g))
+            for k in (0, shape[0] - 1):
+                hold(got[k], g[k], (shape, k))
+
+
+@pytest.mark.gpu
 def test_singular_values_against_the_polynomial(dev):
     """U p(...p(s)) V^T from the singular value decomposition, in 64 bits: the result's definition without the iteration."""
     for rows, cols in ((40, 70), (130, 96)):
