@@ -5,8 +5,8 @@
 //
 // in fp32 (fp32 MFMA), bf16 or f16 (16-bit MFMA), all sums in fp32, one rounding at each store.  What is kept between the passes: for the
 // kinked activations one BIT per element, the exact sign of the fp32 z (so that the gradient's side of the kink never depends on how z would
-// round), for the smooth ones z in the call's own type (its relative rounding 2^-9 / 2^-12 moves act' by |z act''| times that, below the
-// rounding of the gradient itself).
+// round), for the smooth ones z in the call's own type (its relative rounding, 2^-8 / 2^-11 at most, moves act' by |z act''| < 0.35
+// times that: a third of the rounding of a gradient of that size).
 //
 // One tile kernel serves the three products.  An operand whose contraction index is contiguous in memory (KC: x and W of the forward, dz of
 // dx) lies in LDS as [row][128 bytes of k] with its 16-byte pieces XOR-swizzled by the row; one whose contraction index is the row (W of dx,

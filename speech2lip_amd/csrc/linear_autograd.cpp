@@ -50,8 +50,7 @@ Tensor bytes(int64_t n, const Tensor& like) { return n ? at::empty({n}, like.opt
 s2l_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
 struct LinearBackward : public Node {
-  SavedVariable x, weight;
-  Tensor saved;
+  SavedVariable x, weight, saved;
   int act = 0;
   float slope = 0.f;
   bool released = false;
@@ -62,7 +61,7 @@ struct LinearBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     x.reset_data();
     weight.reset_data();
-    saved.reset();
+    saved.reset_data();
     released = true;
   }
 
@@ -75,7 +74,7 @@ struct LinearBackward : public Node {
     if (!dy.defined()) return out;
     const bool need_x = task_should_compute_output(0), need_b = task_should_compute_output(2), need_w = task_should_compute_output(1) || need_b;
     if (need_x || need_w) {
-      const Tensor xs = need_w ? x.unpack() : Tensor(), ws = need_x ? weight.unpack() : Tensor();
+      const Tensor xs = need_w ? x.unpack() : Tensor(), ws = need_x ? weight.unpack() : Tensor(), kept = saved.unpack();
       at::AutoDispatchBelowAutograd below;
       const c10::DeviceGuard device(dy.device());
       const int dt = dtype_of(dy);
@@ -89,7 +88,7 @@ struct LinearBackward : public Node {
       if (need_w) dw = at::empty(w_sizes, dy.options());      // the bias gradient is a by-product of dW
       if (need_b) db = at::empty({n}, dy.options());
       const Tensor work = bytes(lib.backward_bytes(dt, act, d.rows, k, n), dy);
-      const int rc = lib.backward(dt, data(d.t), d.ld, data(xr.t), need_w ? xr.ld : k, data(wr.t), need_x ? wr.ld : k, data(saved), data(dx), k, data(dw),
+      const int rc = lib.backward(dt, data(d.t), d.ld, data(xr.t), need_w ? xr.ld : k, data(wr.t), need_x ? wr.ld : k, data(kept), data(dx), k, data(dw),
                                   data(db), data(work), d.rows, k, n, act, slope, stream_of(dy));
       TORCH_CHECK(rc == 0, "s2l_linear_backward: error ", rc);
       out[0] = dx;
@@ -120,6 +119,8 @@ py::object linear(const Tensor& x, const Tensor& weight, const std::optional<Ten
   if (!fine) return py::none();
   const bool need_x = x.requires_grad(), need_w = weight.requires_grad(), need_b = b.defined() && b.requires_grad(), need_r = r.defined() && r.requires_grad();
   const bool grad = at::GradMode::is_enabled() && (need_x || need_w || need_b || need_r);
+  for (const Tensor& t : {x, weight, b, r})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "linear: no forward-mode derivatives");
   Tensor out, saved;
   int rc;
   {
@@ -144,7 +145,7 @@ py::object linear(const Tensor& x, const Tensor& weight, const std::optional<Ten
     node->set_next_edges(torch::autograd::collect_next_edges(x, weight, b, r));
     if (need_w || need_b) node->x = SavedVariable(x, false);
     if (need_x) node->weight = SavedVariable(weight, false);
-    node->saved = saved;
+    if (saved.defined()) node->saved = SavedVariable(saved, false);
     node->act = act;
     node->slope = (float)slope;
     node->x_sizes = x.sizes().vec();

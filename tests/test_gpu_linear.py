@@ -291,6 +291,27 @@ def test_another_stream_and_a_captured_graph(dev):
             assert all(torch.equal(eager[a], out[a]) for a in eager), (dtype, act, seed)
 
 
+@pytest.mark.gpu
+def test_saved_tensor_hooks_checkpoints_and_forward_mode(dev):
+    """What is kept between the passes goes through the hooks (on the host, or computed again: the same bits); a forward-mode tangent is refused."""
+    from torch.utils.checkpoint import checkpoint
+    import torch.autograd.forward_ad as forward
+    for act in ("none", "leaky_relu", "gelu"):
+        t, dy = make(70, 33, 41, torch.float32, act, dev)
+        leaves = [v.detach().requires_grad_() for v in t.values()]
+        want = torch.autograd.grad(autograd.linear(*leaves, act), leaves, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = autograd.linear(*leaves, act)
+        assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, leaves, dy)))
+        twice = checkpoint(lambda *v: autograd.linear(autograd.linear(*v, act), v[1].mT, None, None, act), *leaves, use_reentrant=False)
+        plain = autograd.linear(autograd.linear(*leaves, act), leaves[1].mT, None, None, act)
+        up = torch.ones_like(plain)
+        assert torch.equal(twice, plain)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(twice, leaves, up), torch.autograd.grad(plain, leaves, up)))
+        with forward.dual_level(), pytest.raises(NotImplementedError):
+            autograd.linear(forward.make_dual(t["x"].detach(), dy @ t["weight"].detach()), t["weight"])
+
+
 def test_refusals_need_no_gpu():
     z = torch.zeros
     with pytest.raises(_abi.S2LError):
