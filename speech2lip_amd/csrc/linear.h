@@ -460,20 +460,27 @@ template <typename T, int DX, int DW> __global__ __launch_bounds__(kThreads, 2) 
 
 // ---- the splits of a long contraction joined, in a fixed order: out = finish(sum over s of partial[s]) -----------------------------------
 // 64 pieces per workgroup, the splits dealt to its four waves and joined through LDS.
-template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Args g, int splits, int blocks, T* dbias) {
+template <typename T> __global__ __launch_bounds__(kThreads) void join_kernel(Args g, int splits, int blocks, int sums, const float* colsum, T* dbias) {
   constexpr int C = kFinish;
   __shared__ float part[4][64][C + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x >= blocks) {      // behind the pieces: the bias gradient, 64 columns to a workgroup
-    const int64_t i = (int64_t)(blockIdx.x - blocks) * 64 + lane;
+  if ((int)blockIdx.x >= blocks) {      // behind the pieces: the bias gradient, sixteen columns to a workgroup
+    float* rows = &part[0][0][0];
+    const int column = threadIdx.x & 15, first = threadIdx.x >> 4;
+    const int64_t i = (int64_t)(blockIdx.x - blocks) * 16 + column;
     float v = 0.f;
     if (i < g.m) {
-#pragma unroll 4
-      for (int s = wave; s < splits; s += 4) v += g.colsum[(int64_t)s * g.m + i];
+#pragma unroll 8
+      for (int s = first; s < sums; s += 16) v += colsum[(int64_t)s * g.m + i];
     }
-    part[wave][lane][0] = v;
+    rows[first * 17 + column] = v;
     __syncthreads();
-    if (wave == 0 && i < g.m) dbias[i] = from_f<T>((part[0][lane][0] + part[1][lane][0]) + (part[2][lane][0] + part[3][lane][0]));
+    if (threadIdx.x < 16 && i < g.m) {
+      v = 0.f;
+#pragma unroll
+      for (int s = 0; s < 16; ++s) v += rows[s * 17 + column];
+      dbias[i] = from_f<T>(v);
+    }
     return;
   }
   const int64_t per = (g.n + C - 1) / C, id = (int64_t)blockIdx.x * 64 + lane;
@@ -559,27 +566,75 @@ template <typename T, int R> __global__ __launch_bounds__(kThreads) void skinny_
   }
 }
 
-// dz = dy * act'(z).  The smooth activations: rounded to the call's type (2^-8 / 2^-11 relative at most, once, before sums that average it out).
-// The kinked ones: where both products then take the LDS-DMA path (which has no place for the gate); exact but for leaky_relu's factor.
-template <typename T> __global__ __launch_bounds__(kThreads) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const void* __restrict__ saved, T* __restrict__ dz,
-                                                                                int64_t rows, int64_t n, int act, float slope) {
+// dz = dy * act'(z) of the kinked activations, where both products then take the LDS-DMA path (which has no place for the gate); exact but for
+// leaky_relu's factor.
+template <typename T> __global__ __launch_bounds__(kThreads) void gate_kernel(const T* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ bits, T* __restrict__ dz,
+                                                                               int64_t rows, int64_t n, float slope) {
   const int64_t per = (n + kFinish - 1) / kFinish, id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t row = id / per, col = id % per * kFinish;
   if (row >= rows) return;
   const bool full = col + kFinish <= n;
   const int count = full ? kFinish : (int)(n - col);
   Eight<T> a = load8(dy + row * lddy + col, full, count);
-  if (act == S2L_ACT_GELU || act == S2L_ACT_SILU) {
-    const Eight<T> z = load8(static_cast<const T*>(saved) + row * n + col, full, count);
+  const uint32_t m = bits[row * per + (col >> 3)];
 #pragma unroll
-    for (int e = 0; e < kFinish; ++e) a.e[e] = from_f<T>((float)a.e[e] * act_slope<T>((float)z.e[e], act));
-  } else {
-    const uint32_t m = static_cast<const uint8_t*>(saved)[row * per + (col >> 3)];
-#pragma unroll
-    for (int e = 0; e < kFinish; ++e)
-      if (!((m >> e) & 1)) a.e[e] = slope == 0.f ? (T)0.f : from_f<T>((float)a.e[e] * slope);
-  }
+  for (int e = 0; e < kFinish; ++e)
+    if (!((m >> e) & 1)) a.e[e] = slope == 0.f ? (T)0.f : from_f<T>((float)a.e[e] * slope);
   store8(dz + row * n + col, a, full, count);
+}
+
+// dz = dy * act'(z) of the smooth ones, rounded to the call's type: the products' matrix instructions take no other (2^-8 / 2^-11 relative at
+// most).  The bias gradient's sums are taken here, from the values before that rounding: its terms cancel as the result's do, so that their
+// roundings would show in it as large as its own (bf16 2.3e-3 of the gradient's norm against 1.7e-3, which is its own rounding).  Memory bound with
+// gelu's arithmetic beside it: 16384 x 4096 bf16 122 us, 97 without the sums.  A workgroup: `groups` pieces of eight columns (a power of two, up to
+// 32) by 256 / groups rows, `times` times; all workgroups move down the matrix together (each on rows of its own: 130 us).  colsum: [workgroup row][n].
+template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ z, T* __restrict__ dz,
+                                                                                int64_t rows, int64_t n, int groups, int times, int columns, float* __restrict__ colsum) {
+  __shared__ float part[kThreads][kFinish + 1];
+  const int lanes = kThreads / groups, lane = threadIdx.x / groups, group = threadIdx.x % groups;
+  const int by = blockIdx.x / columns, bx = blockIdx.x - by * columns;
+  const int64_t col = ((int64_t)bx * groups + group) * kFinish, row0 = (int64_t)by * lanes + lane, stride = (int64_t)(gridDim.x / columns) * lanes;
+  const bool full = col + kFinish <= n;
+  const int count = full ? kFinish : (int)(n - col);
+  float sum[kFinish];
+#pragma unroll
+  for (int e = 0; e < kFinish; ++e) sum[e] = 0.f;
+  if (count > 0) {
+    for (int t = 0; t < times; t += 4) {      // (times: a multiple of 8)
+      Eight<T> a[4], v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t row = row0 + (t + u) * stride;
+        if (row < rows) {
+          a[u] = load8(dy + row * lddy + col, full, count);
+          v[u] = load8(z + row * n + col, full, count);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t row = row0 + (t + u) * stride;
+        if (row >= rows) break;
+#pragma unroll
+        for (int e = 0; e < kFinish; ++e) {
+          const float d = (float)a[u].e[e] * act_slope<T>((float)v[u].e[e], ACT);
+          sum[e] += d;
+          a[u].e[e] = from_f<T>(d);
+        }
+        store8(dz + row * n + col, a[u], full, count);
+      }
+    }
+  }
+  if (!colsum) return;
+#pragma unroll
+  for (int e = 0; e < kFinish; ++e) part[threadIdx.x][e] = sum[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < groups * kFinish; i += kThreads) {
+    const int64_t at = (int64_t)bx * groups * kFinish + i;
+    if (at >= n) break;
+    float v = 0.f;
+    for (int k = 0; k < lanes; ++k) v += part[k * groups + i / kFinish][i % kFinish];
+    colsum[(int64_t)by * n + at] = v;
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
@@ -659,23 +714,28 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AKC, bool B
 }
 
 // after a product: its splits' partial sums joined, and the bias gradient's
-template <typename T> int joined(int rc, const Args& g, const Plan& p, void* dbias, hipStream_t st) {
-  if (rc || (p.splits == 1 && !dbias)) return rc;
-  const int64_t blocks = p.splits == 1 ? 0 : ceil_div(g.m * ceil_div(g.n, kFinish), 64), sums = dbias ? ceil_div(g.m, 64) : 0;
-  if (blocks + sums >= kMaxDim) return S2L_E_SIZE;
-  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + sums)), dim3(kThreads), 0, st, g, p.splits, (int)blocks, static_cast<T*>(dbias));
+struct Sums {
+  void* dbias;
+  int rows;           // of its partial sums
+  float* partial;
+};
+template <typename T> int joined(int rc, const Args& g, const Plan& p, Sums sums, hipStream_t st) {
+  if (rc || (p.splits == 1 && !sums.dbias)) return rc;
+  const int64_t blocks = p.splits == 1 ? 0 : ceil_div(g.m * ceil_div(g.n, kFinish), 64), more = sums.dbias ? ceil_div(g.m, 16) : 0;
+  if (blocks + more >= kMaxDim) return S2L_E_SIZE;
+  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + more)), dim3(kThreads), 0, st, g, p.splits, (int)blocks, sums.rows, sums.partial, static_cast<T*>(sums.dbias));
   return (int)hipGetLastError();
 }
 
-template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st, void* dbias = nullptr) {
+template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st, Sums sums = {}) {
   g.k_per_split = p.k_per_split;
   g.partial = p.splits > 1 ? partial : nullptr;
   int rc;
   if (dense_pieces(g, AKC, BKC, sizeof(T))) {
-    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, stages_of(64)>(g, p, st), g, p, dbias, st);
+    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, stages_of(64)>(g, p, st), g, p, sums, st);
     if constexpr (sizeof(T) == 2 && AKC)
-      if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, dbias, st);
-    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, stages_of(128)>(g, p, st), g, p, dbias, st);
+      if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, sums, st);
+    return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, stages_of(128)>(g, p, st), g, p, sums, st);
   }
   if (p.tile >= 128) {
     if constexpr (AKC && BKC) rc = launch_tile<T, 128, AKC, BKC, false>(g, p, st);
@@ -684,7 +744,7 @@ template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, flo
     if constexpr (AKC && BKC) rc = launch_tile<T, 64, AKC, BKC, false>(g, p, st);
     else rc = g.gate ? launch_tile<T, 64, AKC, BKC, true>(g, p, st) : launch_tile<T, 64, AKC, BKC, false>(g, p, st);
   }
-  return joined<T>(rc, g, p, dbias, st);
+  return joined<T>(rc, g, p, sums, st);
 }
 
 template <typename T, int DX, int DW> int launch_both(const Args& dx, const Args& dw, const Plan& pw, hipStream_t st) {
@@ -712,8 +772,22 @@ template <typename T> int forward(Args g, float* work, hipStream_t st) {
   return product<T, true, true>(g, plan_of(g.m, g.n, g.k, sizeof(T)), work, st);
 }
 
+// slope_kernel's grid: eight rows a thread, more of them (up to 32) while a thousand workgroups remain
+struct Slope {
+  int groups, times, sums;      // sums: workgroup rows
+};
+inline Slope slope_plan(int64_t rows, int64_t n) {
+  Slope s{1, 8, 0};
+  while (s.groups < 32 && s.groups * kFinish < n) s.groups *= 2;
+  const int64_t columns = ceil_div(n, (int64_t)s.groups * kFinish), lanes = kThreads / s.groups;
+  while (s.times < 32 && ceil_div(rows, 2 * s.times * lanes) * columns >= 1024) s.times *= 2;
+  s.sums = rows ? (int)ceil_div(rows, s.times * lanes) : 1;
+  return s;
+}
+
 struct Back {      // the workspace of the backward pass
   Plan dx, dw;
+  Slope slope;
   int64_t dz, partial, colsum, total;      // bytes; the partials of dx and of dW take turns
 };
 
@@ -723,10 +797,12 @@ inline Back back_plan(int64_t rows, int64_t in, int64_t out, int size, int act) 
   b.dw = plan_of(out, in, rows, size, false);
   const int64_t bk = kBkBytes / size;
   const bool gated = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU;      // (the rule goes by the sizes alone: the workspace's size does)
-  b.dz = act == S2L_ACT_GELU || act == S2L_ACT_SILU || (gated && rows % bk == 0 && out % bk == 0 && in % (16 / size) == 0) ? align256(rows * out * size) : 0;
+  const bool smooth = act == S2L_ACT_GELU || act == S2L_ACT_SILU;
+  b.slope = slope_plan(rows, out);
+  b.dz = smooth || (gated && rows % bk == 0 && out % bk == 0 && in % (16 / size) == 0) ? align256(rows * out * size) : 0;
   const int64_t p1 = partial_bytes(b.dx, rows, in), p2 = partial_bytes(b.dw, out, in);
   b.partial = p1 > p2 ? p1 : p2;
-  b.colsum = align256((int64_t)b.dw.splits * out * 4);
+  b.colsum = align256((int64_t)(smooth ? b.slope.sums : b.dw.splits) * out * 4);
   b.total = b.dz + b.partial + b.colsum;
   return b;
 }
@@ -736,11 +812,21 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
   const Back b = back_plan(rows, in, out, sizeof(T), act);
   const void* dz = dy;
   int64_t lddz = lddy;
+  float* sums = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
+  const bool summed = (act == S2L_ACT_GELU || act == S2L_ACT_SILU) && rows;      // by slope_kernel; else dW's product does it
   if (b.dz && rows) {
-    const int64_t blocks = ceil_div(rows * ceil_div(out, kFinish), kThreads);
-    if (blocks >= kMaxDim) return S2L_E_SIZE;
-    hipLaunchKernelGGL((slope_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, saved, reinterpret_cast<T*>(work),
-                       rows, out, act, act == S2L_ACT_LEAKY_RELU ? slope : 0.f);
+    if (act == S2L_ACT_GELU || act == S2L_ACT_SILU) {
+      const int64_t columns = ceil_div(out, (int64_t)b.slope.groups * kFinish);
+      if (columns * b.slope.sums >= kMaxDim) return S2L_E_SIZE;
+      const auto kernel = act == S2L_ACT_GELU ? slope_kernel<T, S2L_ACT_GELU> : slope_kernel<T, S2L_ACT_SILU>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(columns * b.slope.sums)), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const T*>(saved),
+                         reinterpret_cast<T*>(work), rows, out, b.slope.groups, b.slope.times, (int)columns, sums);
+    } else {
+      const int64_t blocks = ceil_div(rows * ceil_div(out, kFinish), kThreads);
+      if (blocks >= kMaxDim) return S2L_E_SIZE;
+      hipLaunchKernelGGL((gate_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const uint8_t*>(saved),
+                         reinterpret_cast<T*>(work), rows, out, act == S2L_ACT_LEAKY_RELU ? slope : 0.f);
+    }
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
     dz = work;
@@ -771,7 +857,7 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
   e.k = rows;
   e.out = dw;
   e.ldo = in;
-  e.colsum = db ? reinterpret_cast<float*>(work + b.dz + b.partial) : nullptr;
+  e.colsum = summed ? nullptr : sums;
   if (dx && dw && b.dx.tile <= 128 && b.dx.splits == 1 && dense_pieces(d, true, false, sizeof(T)) && dense_pieces(e, false, false, sizeof(T))) {
     d.k_per_split = b.dx.k_per_split;
     e.k_per_split = b.dw.k_per_split;
@@ -779,13 +865,13 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
     int rc;
     if (b.dx.tile == 64) rc = b.dw.tile == 64 ? launch_both<T, 64, 64>(d, e, b.dw, st) : launch_both<T, 64, 128>(d, e, b.dw, st);
     else rc = b.dw.tile == 64 ? launch_both<T, 128, 64>(d, e, b.dw, st) : launch_both<T, 128, 128>(d, e, b.dw, st);
-    return joined<T>(rc, e, b.dw, db, st);
+    return joined<T>(rc, e, b.dw, Sums{db, summed ? b.slope.sums : b.dw.splits, sums}, st);
   }
   if (dx && rows) {
     const int rc = product<T, true, false>(d, b.dx, partial, st);
     if (rc) return rc;
   }
-  if (dw) return product<T, false, false>(e, b.dw, partial, st, db);
+  if (dw) return product<T, false, false>(e, b.dw, partial, st, Sums{db, summed ? b.slope.sums : b.dw.splits, sums});
   return 0;
 }
 
