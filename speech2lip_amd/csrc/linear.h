@@ -8,7 +8,8 @@
 // round), for the smooth ones z in the call's own type (its relative rounding, 2^-8 / 2^-11 at most, moves act' by |z act''| < 0.35
 // times that: a third of the rounding of a gradient of that size).
 //
-// One tile kernel serves the three products.  An operand whose contraction index is contiguous in memory (KC: x and W of the forward, dz of
+// Operands whose rows are whole 16-byte pieces come to LDS by the DMA path (dma_kernel; dx and dW in one launch, both_kernel); all others through
+// registers (tile_kernel), which the following describes.  An operand whose contraction index is contiguous in memory (KC: x and W of the forward, dz of
 // dx) lies in LDS as [row][128 bytes of k] with its 16-byte pieces XOR-swizzled by the row; one whose contraction index is the row (W of dx,
 // both operands of dW) lies as it comes, [k][columns], and is transposed on the way out of LDS (the 16-bit types by the transposing LDS
 // read, fp32 by 4-byte reads).  Global memory is read as 16-byte pieces at element alignment into registers one k-tile ahead, so odd widths
