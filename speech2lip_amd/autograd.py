@@ -387,7 +387,8 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     x [..., in], weight [out, in] (nn.Linear's layout), bias [out], residual [..., out] -> [..., out]; all fp32, all bf16 or all fp16, on one GPU.
     activation: "none", "relu", "leaky_relu" (`negative_slope`; 0.02 is the audio encoder's), "gelu" (erf form) or "silu".  Sums, activation and
     residual are evaluated in fp32 and rounded once.  The backward pass keeps one bit per output for the kinked activations and the pre-activation
-    for the smooth ones; it can run once (no double backward, no forward mode).
+    for the smooth ones; it can run once (no double backward, no forward mode).  Tracers (torch.jit.trace, make_fx) and dispatch modes are refused;
+    torch.compile breaks its graph here.
     To capture it into a graph take torch.autograd.grad of leaves that no eager graph holds: torch ends the process where one does.  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
     act = _abi.S2L_ACT.get(activation)
     if act is None:

@@ -2,10 +2,12 @@
 // is host time: with the node in Python it took 125 us, of which the three kernels of a 64 x 64 layer are 15 and the engine's change of thread 40;
 // the rest was the interpreter, in two threads that take turns holding it.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/s2l_hip.h"
@@ -32,6 +34,16 @@ int dtype_of(const Tensor& t) {
     case at::kHalf: return S2L_DTYPE_F16;
     default: return -1;
   }
+}
+
+// What records or replaces a call's operators (torch.jit.trace, make_fx, fake tensors, any dispatch mode or subclass) sees the allocations here and
+// not the launches: the recorded program would return memory that nothing wrote.
+void refuse_recording(std::initializer_list<Tensor> tensors) {
+  bool subclass = false;
+  for (const Tensor& t : tensors) subclass |= t.defined() && t.key_set().has(c10::DispatchKey::Python);
+  TORCH_CHECK_NOT_IMPLEMENTED(!subclass && !torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::any_modes_set(),
+                              "linear: not under a tracer or a dispatch mode, nor on tensor subclasses that dispatch for themselves (its launches are no "
+                              "operators that these see)");
 }
 
 struct Rows {      // a tensor [..., n] as rows of dense columns; a view wherever the strides allow it
@@ -74,6 +86,7 @@ struct LinearBackward : public Node {
     if (!dy.defined()) return out;
     const bool need_x = task_should_compute_output(0), need_b = task_should_compute_output(2), need_w = task_should_compute_output(1) || need_b;
     if (need_x || need_w) {
+      refuse_recording({dy});
       const Tensor xs = need_w ? x.unpack() : Tensor(), ws = need_x ? weight.unpack() : Tensor(), kept = saved.unpack();
       at::AutoDispatchBelowAutograd below;
       const c10::DeviceGuard device(dy.device());
@@ -110,6 +123,7 @@ struct LinearBackward : public Node {
 py::object linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, int act, double slope) {
   const int dt = dtype_of(x);
   const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  refuse_recording({x, weight, b, r});
   const auto like = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device() && t.layout() == at::kStrided; };
   bool fine = dt >= 0 && x.is_cuda() && x.dim() >= 1 && weight.dim() == 2 && like(x) && like(weight) && x.size(-1) == weight.size(1) && weight.size(0) > 0 &&
               weight.size(1) > 0;

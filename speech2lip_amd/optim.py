@@ -143,6 +143,15 @@ class FusedAdam(torch.optim.Optimizer):
         return {id(p) for g in self.param_groups for p in g["params"] if p.grad is not None}
 
 
+def _refuse_recording(who, tensors):
+    """NotImplementedError where something records or replaces this call's operators (torch.jit.trace, make_fx, fake tensors, a dispatch mode or
+    subclass): it would see the allocations and not the launches, and the recorded program would return memory that nothing wrote."""
+    if torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() or any(
+            torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python) for t in tensors):
+        raise NotImplementedError(f"{who}: not under a tracer or a dispatch mode, nor on tensor subclasses that dispatch for themselves (its launches "
+                                  "are no operators that these see)")
+
+
 def _matrix_table(records):
     """s2l_matrix records (in, out, momentum, rows, cols, step) as one host block."""
     return ctypes.create_string_buffer(struct.pack("=" + "qqqiif4x" * len(records), *itertools.chain.from_iterable(records)))
@@ -206,7 +215,8 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
 
     update [..., rows, cols], or a list of such tensors of any sizes, all float32, all bfloat16 or all float16 on one GPU -> the same shape(s) and type,
     in one set of launches.  fp32's accuracy throughout, rounded once; bfloat16: its last two steps on half-precision products (below its rounding).
-    A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not)."""
+    A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not); not
+    under a tracer or a dispatch mode."""
     many = isinstance(update, (list, tuple))
     given = list(update) if many else [update]
     for t in given:
@@ -218,6 +228,7 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
             raise ValueError(f"orthogonalize: all float32, all bfloat16 or all float16: got {t.dtype}")
         if max(t.shape[-2:]) > 131072:
             raise ValueError(f"orthogonalize: at most 131072 rows and columns: got {tuple(t.shape)}")
+    _refuse_recording("orthogonalize", given)
     coefficients = _iteration("orthogonalize", steps, coefficients, eps)
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
@@ -277,6 +288,7 @@ class FusedMuon(FusedAdam):
     def _step_group(self, gi, group, ps):
         if group.get("algorithm", "muon") == "adam":
             return super()._step_group(gi, group, ps)
+        _refuse_recording("FusedMuon", ps)
         lib = _abi.load()
         lr, mode = float(group["lr"]), group["adjust_lr_fn"]
         index, f32, state = ps[0].get_device(), torch.float32, self.state

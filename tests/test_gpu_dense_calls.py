@@ -1,0 +1,79 @@
+"""The calls around autograd.linear, optim.orthogonalize and FusedMuon: who may record them, which views, graphs, hooks and arguments they take, and
+what they refuse."""
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
+
+import speech2lip_amd as s2l
+from speech2lip_amd import autograd, optim
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+class Watching(TorchDispatchMode):
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+class Wrapped(torch.Tensor):
+    """A subclass that dispatches for itself."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError("never reached: the call is refused before its first operator")
+
+
+def _refused_recordings(x, w, p):
+    """A recorded program would hold the allocation of the result and not the launch that writes it."""
+    for f in (lambda t: autograd.linear(t, w), lambda t: optim.orthogonalize(t), lambda t: optim.orthogonalize([t, t])[0]):
+        with pytest.raises(NotImplementedError):
+            torch.jit.trace(f, x, check_trace=False)
+        with pytest.raises(NotImplementedError):
+            make_fx(f)(x)
+        with Watching(), pytest.raises(NotImplementedError):
+            f(x)
+        with pytest.raises(NotImplementedError):
+            f(Wrapped(x))
+    with pytest.raises(NotImplementedError):
+        autograd.linear(x, w, bias=Wrapped(w[:, 0].contiguous()))
+    p.grad = torch.zeros_like(p)
+    opt = s2l.FusedMuon([p])
+    with Watching(), pytest.raises(NotImplementedError):
+        opt.step()
+
+
+def test_recording_is_refused_without_a_gpu():
+    _refused_recordings(torch.zeros(2, 3), torch.zeros(4, 3), torch.nn.Parameter(torch.zeros(4, 3)))
+
+
+@pytest.mark.gpu
+def test_recording_is_refused(dev):
+    x, w = torch.randn(2, 3, device=dev), torch.randn(4, 3, device=dev, requires_grad=True)
+    _refused_recordings(x, w.detach(), torch.nn.Parameter(torch.zeros(4, 3, device=dev)))
+    y = autograd.linear(x, w, activation="gelu")      # an eager forward pass, its backward pass under a mode
+    with Watching(), pytest.raises(NotImplementedError):
+        torch.autograd.grad(y, w, torch.ones_like(y), retain_graph=True)
+    (gw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert bool(torch.isfinite(gw).all())
+
+
+@pytest.mark.gpu
+def test_compiled_callers_break_their_graph_and_stay_right(dev):
+    def f(x, w, b):
+        return autograd.linear(x * 2, w, b, activation="silu").square().sum()
+    leaves = [torch.randn(s, device=dev, requires_grad=True) for s in ((70, 33), (41, 33), (41,))]
+    want = f(*leaves)
+    grads = torch.autograd.grad(want, leaves)
+    got = torch.compile(f, backend="eager")(*leaves)
+    assert torch.equal(want, got) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(got, leaves)))
+    g = torch.randn(30, 50, device=dev)
+    assert torch.equal(torch.compile(lambda t: optim.orthogonalize(t + 0), backend="eager")(g), optim.orthogonalize(g))
