@@ -46,13 +46,14 @@ void refuse_recording(std::initializer_list<Tensor> tensors) {
                               "operators that these see)");
 }
 
-struct Rows {      // a tensor [..., n] as rows of dense columns; a view wherever the strides allow it
+struct Rows {      // a tensor [..., n] as rows of dense columns; a view wherever the strides allow it (a lazily negated one is copied)
   Tensor t;
   int64_t rows, ld;
 };
 Rows rows_of(const Tensor& t) {
   const int64_t n = t.size(-1);
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, n});
+  if (r.is_neg()) r = r.resolve_neg();
   if ((n > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < n)) r = r.contiguous();
   return {r, r.size(0), r.size(0) > 1 ? r.stride(0) : n};
 }
@@ -144,7 +145,7 @@ py::object linear(const Tensor& x, const Tensor& weight, const std::optional<Ten
     const int64_t n = weight.size(0), k = weight.size(1);
     Rows rr{Tensor(), 0, n};
     if (r.defined()) rr = rows_of(r);
-    const Tensor bc = b.defined() ? b.contiguous() : b;
+    const Tensor bc = b.defined() ? b.resolve_neg().contiguous() : b;
     std::vector<int64_t> sizes = x.sizes().vec();
     sizes.back() = n;
     out = at::empty(sizes, x.options());

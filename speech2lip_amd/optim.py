@@ -75,7 +75,7 @@ class FusedAdam(torch.optim.Optimizer):
         lib = _abi.load()
         dev = ps[0].device
         for p in ps:
-            if p.device != dev or dev.type != "cuda" or p.dtype != torch.float32 or p.grad.is_sparse or not p.is_contiguous():
+            if p.device != dev or dev.type != "cuda" or p.dtype != torch.float32 or p.grad.is_sparse or not p.is_contiguous() or p.is_neg():
                 raise _abi.S2LError("FusedAdam takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
             st = self.state[p]
             if not st:
@@ -87,7 +87,8 @@ class FusedAdam(torch.optim.Optimizer):
             raise _abi.S2LError("FusedAdam: the parameters of one group must share their step count (one launch has one bias correction)")
         step_no = int(steps.pop()) + 1
         plan = self._plan(gi, ps)
-        grads = [p.grad if (p.grad.dtype == torch.float32 and p.grad.is_contiguous()) else p.grad.to(torch.float32).contiguous() for p in ps]
+        grads = [p.grad if (p.grad.dtype == torch.float32 and p.grad.is_contiguous() and not p.grad.is_neg())
+                 else p.grad.to(torch.float32).resolve_neg().contiguous() for p in ps]
         ptrs = []
         for p, g in zip(ps, grads):
             st = self.state[p]
@@ -233,7 +234,7 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
             raise _abi.S2LError("orthogonalize: every tensor must be on one GPU (no CPU fallback)")
-    sources = [t.contiguous() for t in given]
+    sources = [t.resolve_neg().contiguous() for t in given]
     outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in sources]
     if sources:
         _orthogonalize_into(sources, outs, steps, coefficients, eps)
@@ -295,16 +296,16 @@ class FusedMuon(FusedAdam):
         records, grads, buffers = [], [], []
         for p in ps:
             g = p.grad
-            if p.get_device() != index or index < 0 or p.dtype != f32 or g.layout != torch.strided or not p.is_contiguous():
+            if p.get_device() != index or index < 0 or p.dtype != f32 or g.layout != torch.strided or not p.is_contiguous() or p.is_neg():
                 raise _abi.S2LError("FusedMuon takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
             st = state[p]
             m = st.get("momentum_buffer")
             if m is None:
                 m = st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            elif m.shape != p.shape or m.dtype != f32 or m.get_device() != index or not m.is_contiguous():
-                m = st["momentum_buffer"] = m.to(device=p.device, dtype=f32).reshape(p.shape).contiguous()
-            if g.dtype != f32 or not g.is_contiguous():
-                g = g.to(f32).contiguous()
+            elif m.shape != p.shape or m.dtype != f32 or m.get_device() != index or not m.is_contiguous() or m.is_neg():
+                m = st["momentum_buffer"] = m.to(device=p.device, dtype=f32).reshape(p.shape).resolve_neg().contiguous()
+            if g.dtype != f32 or not g.is_contiguous() or g.is_neg():
+                g = g.to(f32).resolve_neg().contiguous()
             rows, count = p.shape[0], p.numel()
             cols = count // rows
             scale = 0.2 * math.sqrt(max(rows, cols)) if mode == "match_rms_adamw" else math.sqrt(rows / cols) if rows > cols else 1.0

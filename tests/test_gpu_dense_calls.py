@@ -77,3 +77,35 @@ def test_compiled_callers_break_their_graph_and_stay_right(dev):
     assert torch.equal(want, got) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(got, leaves)))
     g = torch.randn(30, 50, device=dev)
     assert torch.equal(torch.compile(lambda t: optim.orthogonalize(t + 0), backend="eager")(g), optim.orthogonalize(g))
+
+
+@pytest.mark.gpu
+def test_lazily_negated_tensors(dev):
+    """A view whose memory holds the negated values (what `.conj().imag` of a complex tensor is) counts as the values that it shows."""
+    torch.manual_seed(3)
+    neg = lambda *s: torch._neg_view(torch.randn(*s, device=dev))  # noqa: E731
+    held = {"x": neg(20, 30), "weight": neg(12, 30), "bias": neg(12), "residual": neg(20, 12)}
+    assert all(t.is_neg() for t in held.values())
+    dy = neg(20, 12)
+    for act in ("none", "leaky_relu", "silu"):
+        results = []
+        for make in (lambda t: t.detach(), lambda t: t.detach().resolve_neg()):
+            leaves = [make(t).requires_grad_() for t in held.values()]
+            y = autograd.linear(*leaves, activation=act)
+            results.append([y, *torch.autograd.grad(y, leaves, make(dy))])
+        assert all(torch.equal(a, b) for a, b in zip(*results)), act
+    column = torch.randn(20, 1, dtype=torch.complex64, device=dev).conj().imag      # one column: its stride says nothing
+    assert column.is_neg() and torch.equal(autograd.linear(column, held["weight"][:, :1]), autograd.linear(column.clone().resolve_neg(), held["weight"][:, :1].resolve_neg()))
+    assert torch.equal(optim.orthogonalize(held["x"]), optim.orthogonalize(held["x"].resolve_neg()))
+    for opt in (s2l.FusedMuon, s2l.FusedAdam):
+        ends = []
+        for grad in (held["weight"], held["weight"].resolve_neg()):
+            p = torch.nn.Parameter(torch.ones(12, 30, device=dev))
+            p.grad = grad
+            opt([p], lr=0.1).step()
+            ends.append(p.detach())
+        assert torch.equal(*ends)
+        p = torch.nn.Parameter(neg(4, 5))
+        p.grad = torch.ones(4, 5, device=dev)
+        with pytest.raises(RuntimeError):
+            opt([p]).step()
