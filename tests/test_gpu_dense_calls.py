@@ -109,3 +109,26 @@ def test_lazily_negated_tensors(dev):
         p.grad = torch.ones(4, 5, device=dev)
         with pytest.raises(RuntimeError):
             opt([p]).step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", (6, 10241))
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16), ids=str)
+def test_the_tail_of_gelu(dtype, rows, dev):
+    """gelu and its derivative on z in -10 .. 0 against 64 bits, relative to their own terms: one rounding at the store beside the evaluation's error.
+
+    z = x * 1 is exact.  fp32: erfc's argument is off by two roundings, which its value amplifies (1 + z^2)-fold; exp's by one, z^2 / 2-fold; the functions
+    and the remaining products take 10 units of 2^-24.  16-bit types: the formula's 4.8e-5, and 2^-24 (4 z^2 + 16) of its own arithmetic."""
+    x = torch.linspace(-10, 0, rows, device=dev).to(dtype)[:, None].requires_grad_()
+    w = torch.ones(1, 1, dtype=dtype, device=dev)
+    y = autograd.linear(x, w, activation="gelu")
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    phi, density = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5), torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+    e = 2.0 ** -24 * (4 * z * z + 16) + (0 if dtype == torch.float32 else 4.8e-5)
+    info = torch.finfo(dtype)
+    u, grid = info.eps / 2, info.tiny * info.eps / 2      # below the normal range: half a step of the grid
+    for got, want, size in ((y, z * phi, (z * phi).abs()), (gx, phi + z * density, phi + (z * density).abs())):
+        bound = u * want.abs() + (1 + u) * e * size + grid
+        far = (got.detach().double() - want).abs() / bound.clamp_min(1e-300)
+        assert float(far.max()) <= 1, (float(far.max()), float(z[far.argmax()]))
