@@ -389,7 +389,8 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     residual are evaluated in fp32 and rounded once.  The backward pass keeps one bit per output for the kinked activations and the pre-activation
     for the smooth ones; it can run once (no double backward, no forward mode).  Tracers (torch.jit.trace, make_fx) and dispatch modes are refused;
     torch.compile breaks its graph here.
-    To capture it into a graph take torch.autograd.grad of leaves that no eager graph holds: torch ends the process where one does.  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
+    To capture its backward pass into a graph, take leaves that no graph made outside the capture holds (the layer refuses to deliver a
+    gradient there).  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
     act = _abi.S2L_ACT.get(activation)
     if act is None:
         raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")

@@ -1,6 +1,7 @@
 // The host side of autograd.linear: checks, allocation and the autograd node of the dense layer (linear.hip) in C++.  A small layer's training step
 // is host time: with the node in Python it took 125 us, of which the three kernels of a 64 x 64 layer are 15 and the engine's change of thread 40;
 // the rest was the interpreter, in two threads that take turns holding it.
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -62,6 +63,11 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes(int64_t n, const Tensor& like) { return n ? at::empty({n}, like.options().dtype(at::kByte)) : Tensor(); }
 s2l_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
+bool capturing(hipStream_t stream) {      // (the null stream takes part in no capture, and asking for it would end one)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+
 struct LinearBackward : public Node {
   SavedVariable x, weight, saved;
   int act = 0;
@@ -78,6 +84,19 @@ struct LinearBackward : public Node {
     released = true;
   }
 
+  // The engine delivers a gradient on the stream on which its receiver was made: it lets that stream wait for this one.  A leaf's receiver lives as long
+  // as any graph that holds the leaf, so that an eager graph's makes a captured backward pass reach outside its capture, which torch answers by
+  // ending the process.
+  void refuse_foreign_edges() {
+    for (uint32_t i = 0; i < num_outputs(); ++i) {
+      if (!task_should_compute_output(i)) continue;
+      const auto stream = next_edge(i).function->stream();
+      TORCH_CHECK(!stream || capturing(c10::hip::HIPStreamMasqueradingAsCUDA(*stream).stream()),
+                  "linear: this backward pass is being captured, and an input of it is held by a graph made outside the capture (its gradient would be "
+                  "delivered on that graph's stream): drop that graph before the capture, or capture with detached leaves");
+    }
+  }
+
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     TORCH_CHECK(!released, "Trying to backward through the graph a second time (the dense layer's saved values have been freed; "
@@ -85,6 +104,7 @@ struct LinearBackward : public Node {
     variable_list out(4);
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
+    if (capturing(static_cast<hipStream_t>(stream_of(dy)))) refuse_foreign_edges();
     const bool need_x = task_should_compute_output(0), need_b = task_should_compute_output(2), need_w = task_should_compute_output(1) || need_b;
     if (need_x || need_w) {
       refuse_recording({dy});

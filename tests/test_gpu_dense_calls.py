@@ -132,3 +132,66 @@ def test_the_tail_of_gelu(dtype, rows, dev):
         bound = u * want.abs() + (1 + u) * e * size + grid
         far = (got.detach().double() - want).abs() / bound.clamp_min(1e-300)
         assert float(far.max()) <= 1, (float(far.max()), float(z[far.argmax()]))
+
+
+def _layer(dev, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [torch.randn(s, generator=g, device=dev) for s in ((70, 33), (41, 33), (41,), (70, 41))], torch.randn(70, 41, generator=g, device=dev)
+
+
+@pytest.mark.gpu
+def test_a_captured_backward_pass_of_leaves_that_an_eager_graph_holds_is_refused(dev):
+    import gc
+    values, dy = _layer(dev, 0)
+    leaves = [v.requires_grad_() for v in values]
+    alive = autograd.linear(*leaves, "gelu")      # say, a loss that is kept for a log
+    for backward in (lambda y: torch.autograd.grad(y, leaves, dy), lambda y: y.backward(dy)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="held by a graph made outside"):
+            with torch.cuda.graph(graph):
+                backward(autograd.linear(*leaves, "gelu"))
+        torch.cuda.synchronize()
+    want = torch.autograd.grad(alive, leaves, dy)      # the process, the eager graph and the device go on
+    again = torch.autograd.grad(autograd.linear(*leaves, "gelu"), leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
+    del alive
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(autograd.linear(*leaves, "gelu"), leaves, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.gpu
+def test_a_captured_backward_call_fills_the_gradients(dev):
+    """loss.backward() under capture: two layers, one weight in both; replayed on new values."""
+    def step(leaves, up):
+        x, w, b, r = leaves
+        y = autograd.linear(autograd.linear(x, w, b, residual=r, activation="silu"), w.mT, activation="relu")
+        y.backward(up)
+    values, _ = _layer(dev, 0)
+    static = [v.clone().requires_grad_() for v in values]
+    up = torch.zeros(70, 33, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, up)
+    torch.cuda.current_stream().wait_stream(side)
+    for v in static:
+        v.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(static, up)
+    for seed in (1, 2, 3):
+        values, _ = _layer(dev, seed)
+        with torch.no_grad():
+            for s, v in zip(static, values):
+                s.copy_(v)
+            up.copy_(values[0] * 0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = [v.clone().requires_grad_() for v in values]
+        step(fresh, up)
+        assert all(torch.equal(s.grad, f.grad) for s, f in zip(static, fresh)), seed
