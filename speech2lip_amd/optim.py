@@ -8,7 +8,7 @@ the pass reads every parameter anyway -- the NaN scan of `check_weights` (src/co
 
 Same constructor arguments, same `state_dict()` layout (`step`, `exp_avg`, `exp_avg_sq` per parameter) as `torch.optim.Adam`: a checkpoint
 written by either loads into the other (the reference's checkpoints carry `optimizer.state_dict()`, checkpoints.py:38-41).  fp32 CUDA
-parameters with dense gradients; no amsgrad / maximize / capturable (the reference uses none of them).  There is no CPU path.
+parameters with dense gradients; no amsgrad / maximize / capturable (the reference uses none of them; a step under capture is refused).  There is no CPU path.
 
 `FusedMuon` is the same for `torch.optim.Muon` (the update of a weight matrix orthogonalised before it is applied; its arithmetic in 32 bits where
 torch's is bf16), with an Adam of its own for the parameters that are no such matrix; `orthogonalize` is its Newton-Schulz iteration alone
@@ -23,6 +23,12 @@ import struct
 import torch
 
 from . import _abi
+
+
+def _refuse_capture(who, dev):
+    """A captured step would go on writing its report to host memory that the next step gives back (and Adam's would repeat one bias correction)."""
+    if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise _abi.S2LError(f"{who}: a step is not for capture into a graph")
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -74,6 +80,7 @@ class FusedAdam(torch.optim.Optimizer):
         """One launch of s2l_adam_step for the parameters `ps` of group `gi`."""
         lib = _abi.load()
         dev = ps[0].device
+        _refuse_capture("FusedAdam", dev)
         for p in ps:
             if p.device != dev or dev.type != "cuda" or p.dtype != torch.float32 or p.grad.is_sparse or not p.is_contiguous() or p.is_neg():
                 raise _abi.S2LError("FusedAdam takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
@@ -290,6 +297,7 @@ class FusedMuon(FusedAdam):
         if group.get("algorithm", "muon") == "adam":
             return super()._step_group(gi, group, ps)
         _refuse_recording("FusedMuon", ps)
+        _refuse_capture("FusedMuon", ps[0].device)
         lib = _abi.load()
         lr, mode = float(group["lr"]), group["adjust_lr_fn"]
         index, f32, state = ps[0].get_device(), torch.float32, self.state

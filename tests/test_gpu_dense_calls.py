@@ -195,3 +195,30 @@ def test_a_captured_backward_call_fills_the_gradients(dev):
         fresh = [v.clone().requires_grad_() for v in values]
         step(fresh, up)
         assert all(torch.equal(s.grad, f.grad) for s, f in zip(static, fresh)), seed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("opt", (s2l.FusedMuon, s2l.FusedAdam))
+def test_a_captured_optimizer_step_is_refused(opt, dev):
+    """Its report goes to pinned memory that the next step gives back to torch's host allocator: a replay would write into somebody else's."""
+    p, q = (torch.nn.Parameter(torch.ones(12, 30, device=dev)) for _ in range(2))
+    p.grad, q.grad = torch.full_like(p, 0.5), torch.full_like(p, 0.5)
+    one, other = opt([p], lr=0.1), opt([q], lr=0.1)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(graph):
+            p.grad.add_(0)
+            one.step()
+    torch.cuda.synchronize()
+    assert bool((p == 1).all()) and not one.state[p]
+    one.step()
+    other.step()
+    assert torch.equal(p, q) and not bool((p == 1).any())
+    assert not any(bad for _, bad in one.nan_report())
+
+
+def test_a_captured_optimizer_step_is_refused_on_the_host(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        optim._refuse_capture("FusedMuon", torch.device("cuda:0"))
+    optim._refuse_capture("FusedMuon", torch.device("cpu"))
