@@ -364,8 +364,6 @@ def _linear_ops():
 def _linear_refuse(x, weight, bias, residual):
     """What is wrong with the arguments of `linear`, as an exception."""
     given = [t for t in (x, weight, bias, residual) if t is not None]
-    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor) or not all(isinstance(t, torch.Tensor) for t in given):
-        raise TypeError("linear: x, weight, bias and residual are tensors")
     xs, ws = x.shape, weight.shape
     if x.dtype not in _LINEAR_DTYPES:
         raise ValueError(f"linear: float32, bfloat16 or float16: got {x.dtype}")
@@ -394,11 +392,12 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     act = _abi.S2L_ACT.get(activation)
     if act is None:
         raise ValueError(f"linear: activation must be one of {', '.join(_abi.S2L_ACT)}: got {activation!r}")
-    slope = float(negative_slope)
     try:
-        out = _linear_ops().linear(x, weight, bias, residual, act, slope)
+        out = _linear_ops().linear(x, weight, bias, residual, act, float(negative_slope))
     except TypeError:
-        out = None
+        if isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and all(t is None or isinstance(t, torch.Tensor) for t in (bias, residual)):
+            raise      # not about the arguments: what a saved-tensor hook raised
+        raise TypeError("linear: x, weight, bias and residual are tensors") from None
     if out is None:
         _linear_refuse(x, weight, bias, residual)
     return out

@@ -222,3 +222,23 @@ def test_a_captured_optimizer_step_is_refused_on_the_host(monkeypatch):
     with pytest.raises(RuntimeError, match="capture"):
         optim._refuse_capture("FusedMuon", torch.device("cuda:0"))
     optim._refuse_capture("FusedMuon", torch.device("cpu"))
+
+
+def test_arguments_that_are_no_tensors():
+    w = torch.zeros(4, 3)
+    for bad in (([1.0], w), (None, w), (w, None), (w, w, 1.0), (w, w, None, "r"), (w.numpy(), w)):
+        with pytest.raises(TypeError, match="are tensors"):
+            autograd.linear(*bad)
+    with pytest.raises(ValueError):
+        autograd.linear(w, w, negative_slope="steep")
+
+
+@pytest.mark.gpu
+def test_an_error_of_a_saved_tensor_hook_is_the_callers(dev):
+    x, w = torch.randn(5, 3, device=dev), torch.randn(4, 3, device=dev, requires_grad=True)
+
+    def pack(t):
+        raise TypeError("my own")
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), pytest.raises(TypeError, match="my own"):
+        autograd.linear(x, w)
+    assert torch.equal(autograd.linear(x, w.detach()), autograd.linear(x, w))
