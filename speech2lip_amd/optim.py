@@ -16,6 +16,7 @@ torch's is bf16), with an Adam of its own for the parameters that are no such ma
 from __future__ import annotations
 
 import ctypes
+import functools
 import itertools
 import math
 import struct
@@ -165,14 +166,15 @@ def _matrix_table(records):
     return ctypes.create_string_buffer(struct.pack("=" + "qqqiif4x" * len(records), *itertools.chain.from_iterable(records)))
 
 
+@functools.lru_cache(maxsize=64, typed=True)      # (of what passed; 2048 samples a step are 0.5 ms)
 def _check_iteration(who, steps, coefficients, eps):
-    if not (isinstance(steps, int) and 1 <= steps <= 100):
+    if not (isinstance(steps, int) and not isinstance(steps, bool) and 1 <= steps <= 100):
         raise ValueError(f"{who}: steps must be a whole number from 1 to 100: got {steps!r}")
-    if len(coefficients) != 3 or not all(math.isfinite(float(c)) for c in coefficients):
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
         raise ValueError(f"{who}: three finite coefficients (a, b, c): got {coefficients!r}")
     if not eps > 0:
         raise ValueError(f"{who}: eps must be above 0: got {eps!r}")
-    a, b, c = (float(v) for v in coefficients)
+    a, b, c = coefficients
     top = 1.0      # the largest singular value so far (the Frobenius norm starts at 1): the same bound as the library's, checked there again
     for k in range(steps):
         s = [top * i / 2048 for i in range(2049)]
@@ -181,19 +183,15 @@ def _check_iteration(who, steps, coefficients, eps):
         if max(q) > 16 or (k + 1 < steps and top > 4):
             raise ValueError(f"{who}: with the coefficients {coefficients!r} a singular value can grow past 4 (or its factor past 16) in step {k + 1}: "
                              "beyond the range of the iteration's halves")
-    return a, b, c
 
 
 _ORTH_DTYPES = {torch.float32: _abi.S2L_DTYPE_F32, torch.bfloat16: _abi.S2L_DTYPE_BF16, torch.float16: _abi.S2L_DTYPE_F16}
-_CHECKED = set()      # iterations that passed _check_iteration: (steps, coefficients, eps)
 
 
 def _iteration(who, steps, coefficients, eps):
-    key = (steps, tuple(coefficients), eps)
-    if key not in _CHECKED:
-        _check_iteration(who, steps, coefficients, eps)
-        _CHECKED.add(key)
-    return key[1]
+    coefficients = tuple(float(c) for c in coefficients)
+    _check_iteration(who, steps, coefficients, float(eps))
+    return coefficients
 
 
 def _orthogonalize_into(sources, outs, steps, coefficients, eps):
@@ -212,7 +210,7 @@ def _orthogonalize_into(sources, outs, steps, coefficients, eps):
     with torch.cuda.device(dev):
         work = torch.empty(lib.s2l_orthogonalize_work_bytes(table, len(records)), dtype=torch.uint8, device=dev)
         a, b, c = coefficients
-        _abi.check(lib.s2l_orthogonalize(_ORTH_DTYPES[sources[0].dtype], table, len(records), a, b, c, eps, steps, work.data_ptr(),
+        _abi.check(lib.s2l_orthogonalize(_ORTH_DTYPES[sources[0].dtype], table, len(records), a, b, c, float(eps), steps, work.data_ptr(),
                                          torch.cuda.current_stream().cuda_stream), "s2l_orthogonalize")
 
 

@@ -242,3 +242,23 @@ def test_an_error_of_a_saved_tensor_hook_is_the_callers(dev):
     with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), pytest.raises(TypeError, match="my own"):
         autograd.linear(x, w)
     assert torch.equal(autograd.linear(x, w.detach()), autograd.linear(x, w))
+
+
+def test_an_iteration_that_passed_vouches_for_no_other():
+    """steps = 2.0 equals 2 and hashes as it does."""
+    g = torch.zeros(3, 4)
+    for steps in (2, 1):
+        with pytest.raises(RuntimeError, match="GPU"):
+            optim.orthogonalize(g, steps=steps)
+    for bad in (2.0, True):
+        with pytest.raises(ValueError, match="steps"):
+            optim.orthogonalize(g, steps=bad)
+    for k in range(200):
+        with pytest.raises(RuntimeError, match="GPU"):
+            optim.orthogonalize(g, steps=1, eps=1e-7 + k * 1e-9)
+    assert optim._check_iteration.cache_info().currsize <= 64
+    for bad in ((1.0, 2.0), (float("inf"), 0.0, 0.0), "abc"):
+        with pytest.raises(ValueError):
+            optim.orthogonalize(g, coefficients=bad)
+    with pytest.raises(RuntimeError, match="GPU"):
+        optim.orthogonalize(g, coefficients=torch.tensor([1.5, -0.5, 0.0]))
