@@ -99,14 +99,14 @@ struct LinearBackward : public Node {
 
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
-    TORCH_CHECK(!released, "Trying to backward through the graph a second time (the dense layer's saved values have been freed; "
-                           "specify retain_graph=True to go through it again)");
     variable_list out(4);
     const Tensor& dy = grads[0];
     if (!dy.defined()) return out;
     if (capturing(static_cast<hipStream_t>(stream_of(dy)))) refuse_foreign_edges();
     const bool need_x = task_should_compute_output(0), need_b = task_should_compute_output(2), need_w = task_should_compute_output(1) || need_b;
     if (need_x || need_w) {
+      TORCH_CHECK(!released, "Trying to backward through the graph a second time (the dense layer's saved values have been freed; "
+                             "specify retain_graph=True to go through it again)");
       refuse_recording({dy});
       const Tensor xs = need_w ? x.unpack() : Tensor(), ws = need_x ? weight.unpack() : Tensor(), kept = saved.unpack();
       at::AutoDispatchBelowAutograd below;

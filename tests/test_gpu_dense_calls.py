@@ -262,3 +262,27 @@ def test_an_iteration_that_passed_vouches_for_no_other():
             optim.orthogonalize(g, coefficients=bad)
     with pytest.raises(RuntimeError, match="GPU"):
         optim.orthogonalize(g, coefficients=torch.tensor([1.5, -0.5, 0.0]))
+
+
+@pytest.mark.gpu
+def test_the_backward_pass_again(dev):
+    """Under retain_graph the same bits as often as asked; without it an error, unless nothing was kept (the residual's gradient is dy)."""
+    values, dy = _layer(dev, 5)
+    for act in ("none", "relu", "gelu"):
+        leaves = [v.clone().requires_grad_() for v in values]
+        y = autograd.linear(*leaves, act)
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        for keep in (True, False):
+            assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, leaves, dy, retain_graph=keep)))
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, leaves, dy)
+        residual = values[3].clone().requires_grad_()
+        y = autograd.linear(*values[:3], residual, act)
+        for _ in range(2):
+            assert torch.equal(torch.autograd.grad(y, residual, dy)[0], dy)
+        leaves = [v.clone().requires_grad_() for v in values]
+        y = autograd.linear(*leaves, act)
+        with torch.no_grad():      # an operand changed in between: refused, as torch's own layers do
+            leaves[1].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaves, dy)
