@@ -355,6 +355,8 @@ def _linear_ops():
             from . import _linear_ops as ops
         except ImportError as e:
             raise _abi.S2LError(f"_linear_ops.so does not load ({e}): build it with `python -m speech2lip_amd.build`") from e
+        if ops.built_for != f"built for torch {torch.__version__};":
+            raise _abi.S2LError(f"_linear_ops.so was {ops.built_for} this is {torch.__version__}: build it with `python -m speech2lip_amd.build`")
         ops.bind(*(ctypes.cast(getattr(lib, "s2l_linear_" + name), ctypes.c_void_p).value
                    for name in ("saved_bytes", "forward_work_bytes", "backward_work_bytes", "forward", "backward")))
         _linear_native = (lib, ops)

@@ -7,11 +7,14 @@ import re
 import shutil
 import subprocess
 import sys
+import warnings
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
+HEADER = os.path.join(PKG, "..", "include", "s2l_hip.h")
 LIB = os.path.join(PKG, "libs2l_hip.so")
 REF_LIB = os.path.join(PKG, "libs2l_hip_ref.so")      # the same ABI + the non-default kernel forms (-DS2L_WITH_REFERENCE_KERNELS): tests / tools only
+TORCH_OPS_SOURCE = "linear_autograd.cpp"
 TORCH_OPS = os.path.join(PKG, "_linear_ops.so")        # the autograd node of the dense layer: C++ against torch, calls LIB through its C ABI
 RESOURCES = os.path.join(PKG, "kernel_resources.json")      # per-kernel registers / spills / scratch / LDS of the last build
 SOURCES = ["pack.hip", "frontend.hip", "rows.hip", "render.hip", "ensemble.hip", "train.hip", "composite.hip", "unet.hip", "warp.hip", "syncnet.hip", "lpips.hip", "syncchain.hip", "train_bf16.hip", "quant.hip", "render16.hip", "convh.hip",
@@ -55,12 +58,28 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found: libs2l_hip.so cannot be built (set HIPCC=...)")
 
 
-def needs_build() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(REF_LIB) or not os.path.exists(TORCH_OPS):
+def _older(outputs, sources) -> bool:
+    if not all(os.path.exists(o) for o in outputs):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_OPS))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(PKG, "..", "include", "s2l_hip.h")]
-    return any(os.path.getmtime(d) > t for d in deps)
+    t = min(os.path.getmtime(o) for o in outputs)
+    return any(os.path.getmtime(d) > t for d in sources)
+
+
+def _library_needs_build() -> bool:
+    return _older([LIB, REF_LIB, RESOURCES], [HEADER] + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != TORCH_OPS_SOURCE])
+
+
+def _torch_ops_need_build() -> bool:
+    """_linear_ops.so is missing, older than its sources, or built against another torch."""
+    import torch
+    if _older([TORCH_OPS], [HEADER, os.path.join(CSRC, TORCH_OPS_SOURCE)]):
+        return True
+    with open(TORCH_OPS, "rb") as f:
+        return f"built for torch {torch.__version__};".encode() not in f.read()
+
+
+def needs_build() -> bool:
+    return _library_needs_build() or _torch_ops_need_build()
 
 
 def _torch_ops_command() -> list:
@@ -71,15 +90,42 @@ def _torch_ops_command() -> list:
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
                os.path.join(cpp_extension.ROCM_HOME or "/opt/rocm", "include")]
     return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *sum((["-isystem", d] for d in include), []),
-            os.path.join(CSRC, "linear_autograd.cpp"), "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f'-DS2L_TORCH_VERSION="{torch.__version__}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *sum((["-isystem", d] for d in include), []),
+            os.path.join(CSRC, TORCH_OPS_SOURCE), "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
             "-o", TORCH_OPS + ".tmp"]
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .hip translation unit and link the shared library next to this file."""
-    if not force and not needs_build() and os.path.exists(RESOURCES):
-        return LIB
+    """Compile every .hip translation unit and link the shared library next to this file; beside it the dense layer's autograd node, without which
+    (no g++, no headers of Python or torch) all but autograd.linear works: its failure is a warning."""
+    ops = _start_torch_ops() if force or _torch_ops_need_build() else None
+    try:
+        if force or _library_needs_build():
+            _build_hip(verbose)
+    finally:
+        if ops is not None:
+            _finish_torch_ops(ops)
+    return LIB
+
+
+def _start_torch_ops():
+    try:
+        return subprocess.Popen(_torch_ops_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    except Exception as e:      # no compiler, no torch to compile against
+        return e
+
+
+def _finish_torch_ops(ops) -> None:
+    out = str(ops) if isinstance(ops, Exception) else ops.communicate()[0]
+    if not isinstance(ops, Exception) and ops.returncode == 0:
+        os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
+        return
+    if os.path.exists(TORCH_OPS):      # not an old one in its place
+        os.remove(TORCH_OPS)
+    warnings.warn(f"{TORCH_OPS_SOURCE} was not built, autograd.linear will raise:\n{out}")
+
+
+def _build_hip(verbose: bool) -> None:
     hipcc = _hipcc()
     objdir = os.path.join(PKG, "build")
     os.makedirs(objdir, exist_ok=True)
@@ -111,7 +157,6 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     finally:
         sys.path.pop(0)
     procs = []
-    ops = subprocess.Popen(_torch_ops_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     for src in SOURCES:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
         cmd = [hipcc, *FLAGS, *SOURCE_FLAGS.get(src, ()), "-I", objdir, "-c", os.path.join(CSRC, src), "-o", obj]
@@ -132,10 +177,6 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         if verbose and rest.strip():
             print(rest)
         (ref_objs if is_ref else objs).append(obj)
-    out, _ = ops.communicate()
-    if ops.returncode != 0:
-        raise RuntimeError(f"g++ failed on linear_autograd.cpp:\n{out}")
-    os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
     ref_names = {s.replace(".hip", ".o") for s in REF_SOURCES}
     for out_lib, parts in ((LIB, objs), (REF_LIB, [o for o in objs if os.path.basename(o) not in ref_names] + ref_objs)):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out_lib + ".tmp", *parts]
@@ -147,7 +188,6 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     resources["reference_only"] = {k: v for k, v in ref_resources.items() if k not in resources}
     with open(RESOURCES, "w") as f:
         json.dump(resources, f, indent=0, sort_keys=True)
-    return LIB
 
 
 if __name__ == "__main__":

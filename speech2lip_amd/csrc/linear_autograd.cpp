@@ -201,6 +201,7 @@ void bind(uint64_t saved_bytes, uint64_t forward_bytes, uint64_t backward_bytes,
 }  // namespace
 
 PYBIND11_MODULE(_linear_ops, m) {
+  m.attr("built_for") = "built for torch " S2L_TORCH_VERSION ";";
   m.def("linear", &linear);
   m.def("bind", &bind);
 }
