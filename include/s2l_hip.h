@@ -262,7 +262,8 @@ int s2l_muon_step(const s2l_matrix* matrices_host, int64_t count, float momentum
 /* ---- a dense layer of any size (csrc/linear.hip) ----------------------------------------------------------------------------------
  * z = x W^T + bias,  out = act(z) + residual:  x [rows, in], weight [out, in] (nn.Linear's layout), bias [out] or NULL, residual [rows, out]
  * or NULL, all of one type (S2L_DTYPE_*).  ld*: row strides in elements; columns are dense; pointers need only their element's alignment.
- * rows >= 0 (0: nothing to do), in_features, out_features >= 1.  Sums, activation and residual in fp32, one rounding at the store.
+ * rows >= 0 (0: nothing to do), in_features, out_features >= 1, each below 2^31; what a launch cannot count (2^32 threads: 2^26 outputs of up to eight
+ * rows, 2^24 tiles of 128 x 128) is refused (S2L_E_SIZE).  Sums, activation and residual in fp32, one rounding at the store.
  * `slope`: leaky_relu's factor below zero.  The layers of the reference's networks are this with act = ReLU / LeakyReLU
  * (tf_nerf.py:105-109, :149-172, :265-283).
  * saved: NULL, or s2l_linear_saved_bytes(...) bytes that the backward pass reads (relu / leaky_relu: one bit per element, the sign of the fp32

@@ -645,6 +645,7 @@ template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void slope
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
 
 constexpr int64_t kMaxDim = (int64_t)1 << 31;
+inline bool too_many(int64_t blocks, int threads = kThreads) { return blocks * threads >= (int64_t)1 << 32; }      // a launch counts its threads in 32 bits
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
@@ -694,7 +695,7 @@ template <typename T, int TILE, bool AKC, bool BKC, bool GATE> int launch_tile(c
   constexpr int kLds = 2 * kStage > kScratch ? 2 * kStage : kScratch;
   static_assert(kLds <= 65536, "above 64 KiB the launch needs an opt-in");
   const int64_t tiles = ceil_div(g.m, TILE) * ceil_div(g.n, TILE);
-  if (tiles >= kMaxDim) return S2L_E_SIZE;
+  if (too_many(tiles)) return S2L_E_SIZE;
   hipLaunchKernelGGL((tile_kernel<T, TILE, AKC, BKC, GATE>), dim3((unsigned)tiles, (unsigned)p.splits), dim3(kThreads), kLds, st, g);
   return (int)hipGetLastError();
 }
@@ -713,7 +714,7 @@ template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, bool AKC, bool B
     if (rc) return rc;
   }
   const int64_t tiles = ceil_div(g.m, BM) * ceil_div(g.n, BN);
-  if (tiles >= kMaxDim) return S2L_E_SIZE;
+  if (too_many(tiles, P::kThreads)) return S2L_E_SIZE;
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)p.splits), dim3(P::kThreads), lds, st, g);
   return (int)hipGetLastError();
 }
@@ -727,7 +728,7 @@ struct Sums {
 template <typename T> int joined(int rc, const Args& g, const Plan& p, Sums sums, hipStream_t st) {
   if (rc || (p.splits == 1 && !sums.dbias)) return rc;
   const int64_t blocks = p.splits == 1 ? 0 : ceil_div(g.m * ceil_div(g.n, kFinish), 64), more = sums.dbias ? ceil_div(g.m, 16) : 0;
-  if (blocks + more >= kMaxDim) return S2L_E_SIZE;
+  if (too_many(blocks + more)) return S2L_E_SIZE;
   hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(blocks + more)), dim3(kThreads), 0, st, g, p.splits, (int)blocks, sums.rows, sums.partial, static_cast<T*>(sums.dbias));
   return (int)hipGetLastError();
 }
@@ -758,7 +759,7 @@ template <typename T, int DX, int DW> int launch_both(const Args& dx, const Args
   constexpr int lds = PX::kLds > PW::kLds ? PX::kLds : PW::kLds;
   static_assert(lds <= 65536 && lds >= 4 * 32 * (DX / 2 + 4) * 4 && lds >= 4 * 32 * (DW / 2 + 4) * 4, "");
   const int64_t x = ceil_div(dx.m, DX) * ceil_div(dx.n, DX), w = ceil_div(dw.m, DW) * ceil_div(dw.n, DW);
-  if (x + w * pw.splits >= kMaxDim) return S2L_E_SIZE;
+  if (too_many(x + w * pw.splits)) return S2L_E_SIZE;
   hipLaunchKernelGGL((both_kernel<T, DX, DW>), dim3((unsigned)(x + w * pw.splits)), dim3(kThreads), lds, st, dx, dw, (int)w, (int)(w * pw.splits));
   return (int)hipGetLastError();
 }
@@ -768,6 +769,7 @@ inline bool skinny(int64_t rows, bool bits) { return rows <= kSkinnyRows && !bit
 
 template <typename T> int forward(Args g, float* work, hipStream_t st) {
   if (skinny(g.m, g.bits != nullptr)) {
+    if (too_many(ceil_div(g.n, 4))) return S2L_E_SIZE;
     const dim3 grid((unsigned)ceil_div(g.n, 4));
     if (g.m == 1) hipLaunchKernelGGL((skinny_kernel<T, 1>), grid, dim3(kThreads), 0, st, g);
     else if (g.m <= 4) hipLaunchKernelGGL((skinny_kernel<T, 4>), grid, dim3(kThreads), 0, st, g);
@@ -823,13 +825,13 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
   if (b.dz && rows) {
     if (act == S2L_ACT_GELU || act == S2L_ACT_SILU) {
       const int64_t columns = ceil_div(out, (int64_t)b.slope.groups * kFinish);
-      if (columns * b.slope.sums >= kMaxDim) return S2L_E_SIZE;
+      if (too_many(columns * b.slope.sums)) return S2L_E_SIZE;
       const auto kernel = act == S2L_ACT_GELU ? slope_kernel<T, S2L_ACT_GELU> : slope_kernel<T, S2L_ACT_SILU>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)(columns * b.slope.sums)), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const T*>(saved),
                          reinterpret_cast<T*>(work), rows, out, b.slope.groups, b.slope.times, (int)columns, sums);
     } else {
       const int64_t blocks = ceil_div(rows * ceil_div(out, kFinish), kThreads);
-      if (blocks >= kMaxDim) return S2L_E_SIZE;
+      if (too_many(blocks)) return S2L_E_SIZE;
       hipLaunchKernelGGL((gate_kernel<T>), dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<const T*>(dy), lddy, static_cast<const uint8_t*>(saved),
                          reinterpret_cast<T*>(work), rows, out, act == S2L_ACT_LEAKY_RELU ? slope : 0.f);
     }

@@ -745,6 +745,7 @@ __global__ __launch_bounds__(kThreads, 2) void small_kernel(S2L_FRONT, Alike ali
 
 constexpr int kMaxSide = 1 << 17;
 constexpr int kMaxSteps = 100;
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 32) / kThreads - 1;      // a launch counts its threads in 32 bits
 
 struct Layout {
   int tile_sym, tile_rect;
@@ -815,7 +816,7 @@ inline int lay_out(const s2l_matrix* in, int count, Table* t, Layout* l) {
     const int cut = pieces_of(r.np, l->chunk).count;
     at[DEEP] += l->chunk ? cut * (ts * (ts + 1) / 2) : 0;
     base += r.total * 2 + sums_bytes(cut, (int)(ts * (ts + 1) / 2));
-    if (at[PACK] > 0x3ffffff0 || at[SYM] > 0x3ffffff0 || at[RECT] > 0x3ffffff0 || at[DEEP] > 0x3ffffff0) return S2L_E_SIZE;
+    if (at[PACK] > kMaxBlocks || 4 * at[SYM] > kMaxBlocks || at[RECT] > kMaxBlocks || at[DEEP] > kMaxBlocks) return S2L_E_SIZE;      // (4: join_kernel's)
   }
   for (int k = 0; k < KINDS; ++k) l->blocks[k] = (int)at[k];
   int64_t front = kTableBytes + partial_bytes((int)at[STAT]);

@@ -6,7 +6,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import speech2lip_amd as s2l
-from speech2lip_amd import autograd, optim
+from speech2lip_amd import _abi, autograd, optim
 
 
 @pytest.fixture(scope="module")
@@ -286,3 +286,13 @@ def test_the_backward_pass_again(dev):
             leaves[1].mul_(2)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(y, leaves, dy)
+
+
+def test_calls_beyond_a_launch_are_refused_on_the_host():
+    """2^32 threads or more: 2^26 outputs of a few rows, four to a workgroup of 256; 2^24 tiles of 128 x 128."""
+    lib, p, most = _abi.load(), 4096, (1 << 31) - 1
+    fwd = lambda rows, k, n, act=0, saved=0: lib.s2l_linear_forward(0, p, k, p, k, 0, 0, n, p, n, saved, p, rows, k, n, act, 0.0, 0)  # noqa: E731
+    assert fwd(1, 1, 1 << 26) == -2 and fwd(8, 1, most) == -2
+    assert fwd(most, 33, 1) == -2 and fwd(1 << 30, 32, 129) == -2 and fwd(8, 32, most, act=1, saved=p) == -2
+    bwd = lambda rows, k, n: lib.s2l_linear_backward(0, p, n, p, k, p, k, p, p, k, 0, 0, p, rows, k, n, 0, 0.0, 0)  # noqa: E731
+    assert bwd(most, 5, 4) == -2 and bwd(8, most, 4) == -2 and bwd(1 << 30, 129, 32) == -2
