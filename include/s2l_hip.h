@@ -282,6 +282,10 @@ int s2l_linear_forward(int dtype, const void* x, int64_t ldx, const void* weight
 int s2l_linear_backward(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int64_t ldw,
                         const void* saved, void* dx, int64_t lddx, void* dweight, void* dbias, void* work, int64_t rows,
                         int64_t in_features, int64_t out_features, int act, float slope, s2l_stream_t stream);
+/* Which kernels such a call launches, its operands dense and on 16 bytes (for tests; launches nothing).  grads: 1 dx, 2 dweight.  routes: ten ints,
+ * {path, tile, pieces of the contraction} of the forward, dx and dweight -- path 1: a wave per output, 2: tiles through registers, 3: by LDS-DMA, 4: so,
+ * dx and dweight in one launch -- then what forms dz: 0 the products' own loads, 1 a pass over dy, more: that many rows a thread. */
+int s2l_debug_linear_routes(int dtype, int act, int keep, int grads, int64_t rows, int64_t in_features, int64_t out_features, int* routes);
 
 /* optimizer.step() of the reference's training loop (train.py:173-199 builds torch.optim.Adam; training.py:559-574 steps it after
  * check_weights) for EVERY tensor of a parameter group in ONE launch: torch's _single_tensor_adam arithmetic, operation for operation in

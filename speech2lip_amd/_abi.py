@@ -204,6 +204,7 @@ EXPORTS = {
                                    c_int64, c_int64, c_int64, c_int, c_float, c_void_p]),
     "s2l_linear_backward": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                                     c_void_p, c_int64, c_int64, c_int64, c_int, c_float, c_void_p]),
+    "s2l_debug_linear_routes": (c_int, [c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_void_p]),
     "s2l_to8b": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "s2l_from8b": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }

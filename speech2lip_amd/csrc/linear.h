@@ -733,17 +733,28 @@ template <typename T> int joined(int rc, const Args& g, const Plan& p, Sums sums
   return (int)hipGetLastError();
 }
 
+// the kernel of a product alone
+struct Route {
+  bool dma;
+  int tile;
+};
+inline Route route_of(const Args& g, const Plan& p, bool akc, bool bkc, int size) {
+  const bool dma = dense_pieces(g, akc, bkc, size);
+  return Route{dma, p.tile == 256 && !dma ? 128 : p.tile};
+}
+
 template <typename T, bool AKC, bool BKC> int product(Args g, const Plan& p, float* partial, hipStream_t st, Sums sums = {}) {
   g.k_per_split = p.k_per_split;
   g.partial = p.splits > 1 ? partial : nullptr;
   int rc;
-  if (dense_pieces(g, AKC, BKC, sizeof(T))) {
-    if (p.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, stages_of(64)>(g, p, st), g, p, sums, st);
+  const Route r = route_of(g, p, AKC, BKC, sizeof(T));
+  if (r.dma) {
+    if (r.tile == 64) return joined<T>(launch_dma<T, 64, 64, 2, 2, AKC, BKC, stages_of(64)>(g, p, st), g, p, sums, st);
     if constexpr (sizeof(T) == 2 && AKC)
-      if (p.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, sums, st);
+      if (r.tile == 256) return joined<T>(launch_dma<T, 256, 256, 2, 4, AKC, BKC, 2>(g, p, st), g, p, sums, st);
     return joined<T>(launch_dma<T, 128, 128, 2, 2, AKC, BKC, stages_of(128)>(g, p, st), g, p, sums, st);
   }
-  if (p.tile >= 128) {
+  if (r.tile == 128) {
     if constexpr (AKC && BKC) rc = launch_tile<T, 128, AKC, BKC, false>(g, p, st);
     else rc = g.gate ? launch_tile<T, 128, AKC, BKC, true>(g, p, st) : launch_tile<T, 128, AKC, BKC, false>(g, p, st);
   } else {
@@ -815,6 +826,41 @@ inline Back back_plan(int64_t rows, int64_t in, int64_t out, int size, int act) 
   return b;
 }
 
+// what the two products of the backward pass read and write, dz given
+struct Products {
+  Args dx, dw;
+  bool together;      // one launch for both
+};
+inline Products products_of(const Back& b, const void* dz, int64_t lddz, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* saved, void* dx, int64_t lddx, void* dw,
+                            float* colsum, int64_t rows, int64_t in, int64_t out, int size, int act, float slope) {
+  const bool gated = (act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU) && !b.dz;
+  Args g{};
+  g.a = dz;
+  g.lda = lddz;
+  g.gate = gated ? static_cast<const uint8_t*>(saved) : nullptr;
+  g.gate_ld = (out + 7) >> 3;
+  g.slope = act == S2L_ACT_LEAKY_RELU ? slope : 0.f;
+  g.act = S2L_ACT_NONE;
+  Args d = g;      // dx = dz W
+  d.b = w;
+  d.ldb = ldw;
+  d.m = rows;
+  d.n = in;
+  d.k = out;
+  d.out = dx;
+  d.ldo = lddx;
+  Args e = g;      // dW = dz^T x
+  e.b = x;
+  e.ldb = ldx;
+  e.m = out;
+  e.n = in;
+  e.k = rows;
+  e.out = dw;
+  e.ldo = in;
+  e.colsum = colsum;
+  return Products{d, e, dx && dw && b.dx.tile <= 128 && b.dx.splits == 1 && dense_pieces(d, true, false, size) && dense_pieces(e, false, false, size)};
+}
+
 template <typename T> int backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* saved, void* dx, int64_t lddx,
                                    void* dw, void* db, char* work, int64_t rows, int64_t in, int64_t out, int act, float slope, hipStream_t st) {
   const Back b = back_plan(rows, in, out, sizeof(T), act);
@@ -840,33 +886,10 @@ template <typename T> int backward(const void* dy, int64_t lddy, const void* x, 
     dz = work;
     lddz = out;
   }
-  const bool gated = (act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU) && !b.dz;
   float* partial = reinterpret_cast<float*>(work + b.dz);
-  Args g{};
-  g.a = dz;
-  g.lda = lddz;
-  g.gate = gated ? static_cast<const uint8_t*>(saved) : nullptr;
-  g.gate_ld = (out + 7) >> 3;
-  g.slope = act == S2L_ACT_LEAKY_RELU ? slope : 0.f;
-  g.act = S2L_ACT_NONE;
-  Args d = g;      // dx = dz W
-  d.b = w;
-  d.ldb = ldw;
-  d.m = rows;
-  d.n = in;
-  d.k = out;
-  d.out = dx;
-  d.ldo = lddx;
-  Args e = g;      // dW = dz^T x
-  e.b = x;
-  e.ldb = ldx;
-  e.m = out;
-  e.n = in;
-  e.k = rows;
-  e.out = dw;
-  e.ldo = in;
-  e.colsum = summed ? nullptr : sums;
-  if (dx && dw && b.dx.tile <= 128 && b.dx.splits == 1 && dense_pieces(d, true, false, sizeof(T)) && dense_pieces(e, false, false, sizeof(T))) {
+  Products both = products_of(b, dz, lddz, x, ldx, w, ldw, saved, dx, lddx, dw, summed ? nullptr : sums, rows, in, out, sizeof(T), act, slope);
+  Args &d = both.dx, &e = both.dw;
+  if (both.together) {
     d.k_per_split = b.dx.k_per_split;
     e.k_per_split = b.dw.k_per_split;
     e.partial = b.dw.splits > 1 ? partial : nullptr;

@@ -104,3 +104,39 @@ extern "C" int s2l_linear_backward(int dtype, const void* dy, int64_t lddy, cons
     return backward<__bf16>(dy, lddy, x, ldx, weight, ldw, saved, dx, lddx, dweight, dbias, ws, rows, in_features, out_features, act, slope, st);
   return backward<_Float16>(dy, lddy, x, ldx, weight, ldw, saved, dx, lddx, dweight, dbias, ws, rows, in_features, out_features, act, slope, st);
 }
+
+extern "C" int s2l_debug_linear_routes(int dtype, int act, int keep, int grads, int64_t rows, int64_t in_features, int64_t out_features, int* routes) {
+  using namespace s2l::lin;
+  const int size = size_of(dtype);
+  if (!size || act < S2L_ACT_NONE || act > S2L_ACT_SILU) return S2L_E_UNSUPPORTED;
+  if (bad_dims(rows, in_features, out_features) || rows < 1) return S2L_E_SIZE;
+  if (!routes) return S2L_E_NULL;
+  const auto put = [&](int at, int path, int tile, int splits) {
+    routes[at] = path;
+    routes[at + 1] = tile;
+    routes[at + 2] = splits;
+  };
+  const bool kinked = act == S2L_ACT_RELU || act == S2L_ACT_LEAKY_RELU;
+  for (int i = 0; i < 10; ++i) routes[i] = 0;
+  char* p = reinterpret_cast<char*>(uintptr_t{4096});      // (never read: an address of whole 16-byte pieces)
+  if (skinny(rows, keep && kinked)) {
+    put(0, 1, 0, 1);
+  } else {
+    Args g{};
+    g.a = g.b = p;
+    g.lda = g.ldb = g.k = in_features;
+    g.m = rows;
+    g.n = out_features;
+    const Plan plan = plan_of(rows, out_features, in_features, size);
+    const Route r = route_of(g, plan, true, true, size);
+    put(0, r.dma ? 3 : 2, r.tile, plan.splits);
+  }
+  const Back b = back_plan(rows, in_features, out_features, size, act);
+  const Products both = products_of(b, p, out_features, p, in_features, p, in_features, p, grads & 1 ? p : nullptr, in_features, grads & 2 ? p : nullptr, nullptr, rows,
+                                    in_features, out_features, size, act, 0.5f);
+  const Route dx = route_of(both.dx, b.dx, true, false, size), dw = route_of(both.dw, b.dw, false, false, size);
+  if (grads & 1) put(3, both.together ? 4 : dx.dma ? 3 : 2, dx.tile, b.dx.splits);
+  if (grads & 2) put(6, both.together ? 4 : dw.dma ? 3 : 2, dw.tile, b.dw.splits);
+  routes[9] = !b.dz ? 0 : kinked ? 1 : b.slope.times;
+  return S2L_OK;
+}
