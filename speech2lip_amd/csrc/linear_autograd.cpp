@@ -39,9 +39,9 @@ int dtype_of(const Tensor& t) {
 
 // What records or replaces a call's operators (torch.jit.trace, make_fx, fake tensors, any dispatch mode or subclass) sees the allocations here and
 // not the launches: the recorded program would return memory that nothing wrote.
-void refuse_recording(std::initializer_list<Tensor> tensors) {
+void refuse_recording(std::initializer_list<const Tensor*> tensors) {
   bool subclass = false;
-  for (const Tensor& t : tensors) subclass |= t.defined() && t.key_set().has(c10::DispatchKey::Python);
+  for (const Tensor* t : tensors) subclass |= t->defined() && t->key_set().has(c10::DispatchKey::Python);
   TORCH_CHECK_NOT_IMPLEMENTED(!subclass && !torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::any_modes_set(),
                               "linear: not under a tracer or a dispatch mode, nor on tensor subclasses that dispatch for themselves (its launches are no "
                               "operators that these see)");
@@ -107,7 +107,7 @@ struct LinearBackward : public Node {
     if (need_x || need_w) {
       TORCH_CHECK(!released, "Trying to backward through the graph a second time (the dense layer's saved values have been freed; "
                              "specify retain_graph=True to go through it again)");
-      refuse_recording({dy});
+      refuse_recording({&dy});
       const Tensor xs = need_w ? x.unpack() : Tensor(), ws = need_x ? weight.unpack() : Tensor(), kept = saved.unpack();
       at::AutoDispatchBelowAutograd below;
       const c10::DeviceGuard device(dy.device());
@@ -144,7 +144,7 @@ struct LinearBackward : public Node {
 py::object linear(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, int act, double slope) {
   const int dt = dtype_of(x);
   const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
-  refuse_recording({x, weight, b, r});
+  refuse_recording({&x, &weight, &b, &r});
   const auto like = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device() && t.layout() == at::kStrided; };
   bool fine = dt >= 0 && x.is_cuda() && x.dim() >= 1 && weight.dim() == 2 && like(x) && like(weight) && x.size(-1) == weight.size(1) && weight.size(0) > 0 &&
               weight.size(1) > 0;

@@ -152,11 +152,15 @@ class FusedAdam(torch.optim.Optimizer):
         return {id(p) for g in self.param_groups for p in g["params"] if p.grad is not None}
 
 
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
+
+
 def _refuse_recording(who, tensors):
     """NotImplementedError where something records or replaces this call's operators (torch.jit.trace, make_fx, fake tensors, a dispatch mode or
     subclass): it would see the allocations and not the launches, and the recorded program would return memory that nothing wrote."""
+    others = [t for t in tensors if type(t) not in _PLAIN]
     if torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() or any(
-            torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python) for t in tensors):
+            torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python) for t in others):
         raise NotImplementedError(f"{who}: not under a tracer or a dispatch mode, nor on tensor subclasses that dispatch for themselves (its launches "
                                   "are no operators that these see)")
 
@@ -282,7 +286,7 @@ class FusedMuon(FusedAdam):
                 raise ValueError("FusedMuon: invalid hyper-parameter (lr, weight_decay >= 0, momentum in 0 .. 1)")
             if full["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
                 raise ValueError(f"FusedMuon: adjust_lr_fn must be None, \"original\" or \"match_rms_adamw\": got {full['adjust_lr_fn']!r}")
-            _iteration("FusedMuon", full["ns_steps"], full["ns_coefficients"], full["eps"])
+            g["ns_coefficients"] = _iteration("FusedMuon", full["ns_steps"], full["ns_coefficients"], full["eps"])
             g["params"] = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
             for p in g["params"]:
                 t = p[1] if isinstance(p, tuple) else p
@@ -294,7 +298,7 @@ class FusedMuon(FusedAdam):
     def _step_group(self, gi, group, ps):
         if group.get("algorithm", "muon") == "adam":
             return super()._step_group(gi, group, ps)
-        _refuse_recording("FusedMuon", ps)
+        _refuse_recording("FusedMuon", ())
         _refuse_capture("FusedMuon", ps[0].device)
         lib = _abi.load()
         lr, mode = float(group["lr"]), group["adjust_lr_fn"]
@@ -302,14 +306,16 @@ class FusedMuon(FusedAdam):
         records, grads, buffers = [], [], []
         for p in ps:
             g = p.grad
-            if p.get_device() != index or index < 0 or p.dtype != f32 or g.layout != torch.strided or not p.is_contiguous() or p.is_neg():
+            if p.get_device() != index or index < 0 or p.dtype != f32 or g.layout != torch.strided or not p.is_contiguous():
                 raise _abi.S2LError("FusedMuon takes contiguous fp32 CUDA parameters of one device with dense gradients (no CPU path)")
             st = state[p]
             m = st.get("momentum_buffer")
             if m is None:
+                if p.is_neg():
+                    raise _abi.S2LError("FusedMuon: a parameter that is a lazily negated view")
                 m = st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            elif m.shape != p.shape or m.dtype != f32 or m.get_device() != index or not m.is_contiguous() or m.is_neg():
-                m = st["momentum_buffer"] = m.to(device=p.device, dtype=f32).reshape(p.shape).resolve_neg().contiguous()
+            elif m.shape != p.shape or m.dtype != f32 or m.get_device() != index or not m.is_contiguous():
+                m = st["momentum_buffer"] = m.to(device=p.device, dtype=f32).reshape(p.shape).contiguous()
             if g.dtype != f32 or not g.is_contiguous() or g.is_neg():
                 g = g.to(f32).resolve_neg().contiguous()
             rows, count = p.shape[0], p.numel()
@@ -319,7 +325,8 @@ class FusedMuon(FusedAdam):
             grads.append(g)
             buffers.append(m)
         table = _matrix_table(records)
-        a, b, c = _iteration("FusedMuon", group["ns_steps"], group["ns_coefficients"], group["eps"])
+        a, b, c = coefficients = tuple(group["ns_coefficients"])
+        _check_iteration("FusedMuon", group["ns_steps"], coefficients, group["eps"])
         dev = ps[0].device
         with torch.cuda.device(dev):
             stream = torch.cuda.current_stream()
