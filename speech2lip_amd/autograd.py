@@ -386,8 +386,9 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
 
     x [..., in], weight [out, in] (nn.Linear's layout), bias [out], residual [..., out] -> [..., out]; all fp32, all bf16 or all fp16, on one GPU.
     activation: "none", "relu", "leaky_relu" (`negative_slope`; 0.02 is the audio encoder's), "gelu" (erf form) or "silu".  Sums, activation and
-    residual are evaluated in fp32 and rounded once.  The backward pass keeps one bit per output for the kinked activations and the pre-activation
-    for the smooth ones; it runs once, or as often as retain_graph=True lets it, and is not differentiable itself (nor is there a forward mode).
+    residual are evaluated in fp32 and rounded once; so is dy act'(z), in the call's type, which dx and dW are products of (float16: scale the loss).
+    The backward pass keeps one bit per output for the kinked activations and the pre-activation for the smooth ones; it runs once, or as often as
+    retain_graph=True lets it, and is not differentiable itself (nor is there a forward mode).
     Tracers (torch.jit.trace, make_fx) and dispatch modes are refused; torch.compile breaks its graph here.
     To capture its backward pass into a graph, take leaves that no graph made outside the capture holds (the layer refuses to deliver a
     gradient there).  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
