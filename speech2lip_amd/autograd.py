@@ -389,7 +389,8 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none", negati
     residual are evaluated in fp32 and rounded once; so is dy act'(z), in the call's type, which dx and dW are products of (float16: scale the loss).
     The backward pass keeps one bit per output for the kinked activations and the pre-activation for the smooth ones; it runs once, or as often as
     retain_graph=True lets it, and is not differentiable itself (nor is there a forward mode).
-    Tracers (torch.jit.trace, make_fx) and dispatch modes are refused; torch.compile breaks its graph here.
+    make_fx and dispatch modes see two operators (torch.ops.speech2lip_amd.linear_forward, linear_backward); torch.compile breaks its graph here,
+    torch.jit.trace is refused.
     To capture its backward pass into a graph, take leaves that no graph made outside the capture holds (the layer refuses to deliver a
     gradient there).  Row strides are taken as they are; a tensor whose columns are not dense is copied."""
     act = _abi.S2L_ACT.get(activation)

@@ -71,9 +71,9 @@ def _library_needs_build() -> bool:
 
 def _torch_ops_need_build() -> bool:
     """_linear_ops.so is missing, older than its sources, or built against another torch."""
-    import torch
     if _older([TORCH_OPS], [HEADER, os.path.join(CSRC, TORCH_OPS_SOURCE)]):
         return True
+    import torch
     with open(TORCH_OPS, "rb") as f:
         return f"built for torch {torch.__version__};".encode() not in f.read()
 

@@ -152,17 +152,11 @@ class FusedAdam(torch.optim.Optimizer):
         return {id(p) for g in self.param_groups for p in g["params"] if p.grad is not None}
 
 
-_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
-
-
-def _refuse_recording(who, tensors):
-    """NotImplementedError where something records or replaces this call's operators (torch.jit.trace, make_fx, fake tensors, a dispatch mode or
-    subclass): it would see the allocations and not the launches, and the recorded program would return memory that nothing wrote."""
-    others = [t for t in tensors if type(t) not in _PLAIN]
-    if torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() or any(
-            torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python) for t in others):
-        raise NotImplementedError(f"{who}: not under a tracer or a dispatch mode, nor on tensor subclasses that dispatch for themselves (its launches "
-                                  "are no operators that these see)")
+def _refuse_tracing(who):
+    """NotImplementedError under what records a program (torch.jit.trace, make_fx, fake tensors): it would not see the launches."""
+    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and any(
+            torch._C._get_dispatch_mode(key) is not None for key in torch._C._TorchDispatchModeKey.__members__.values())):
+        raise NotImplementedError(f"{who}: not under a tracer, which would not see its launches")
 
 
 def _matrix_table(records):
@@ -198,8 +192,22 @@ def _iteration(who, steps, coefficients, eps):
     return coefficients
 
 
-def _orthogonalize_into(sources, outs, steps, coefficients, eps):
-    """The matrices of `sources` (dense [..., rows, cols], one type, one GPU) to `outs`, in one set of launches."""
+def _check_matrices(given):
+    for t in given:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("orthogonalize: a tensor [..., rows, cols] or a list of them")
+        if t.dim() < 2:
+            raise ValueError(f"orthogonalize: matrices [..., rows, cols]: got {tuple(t.shape)}")
+        if t.dtype not in _ORTH_DTYPES or t.dtype != given[0].dtype:
+            raise ValueError(f"orthogonalize: all float32, all bfloat16 or all float16: got {t.dtype}")
+        if max(t.shape[-2:]) > 131072:
+            raise ValueError(f"orthogonalize: at most 131072 rows and columns: got {tuple(t.shape)}")
+
+
+def _orthogonalize_all(given, steps, a, b, c, eps):
+    """The matrices of `given` (one type, one GPU) in one set of launches."""
+    sources = [t.resolve_neg().contiguous() for t in given]
+    outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in sources]
     lib = _abi.load()
     records = []
     for src, out in zip(sources, outs):
@@ -208,14 +216,31 @@ def _orthogonalize_into(sources, outs, steps, coefficients, eps):
         if stride:
             records += [(src.data_ptr() + i * stride, out.data_ptr() + i * stride, 0, rows, cols, 0.0) for i in range(src.numel() // (rows * cols))]
     if not records:
-        return
+        return outs
     dev = sources[0].device
     table = _matrix_table(records)
     with torch.cuda.device(dev):
         work = torch.empty(lib.s2l_orthogonalize_work_bytes(table, len(records)), dtype=torch.uint8, device=dev)
-        a, b, c = coefficients
-        _abi.check(lib.s2l_orthogonalize(_ORTH_DTYPES[sources[0].dtype], table, len(records), a, b, c, float(eps), steps, work.data_ptr(),
+        _abi.check(lib.s2l_orthogonalize(_ORTH_DTYPES[sources[0].dtype], table, len(records), a, b, c, eps, steps, work.data_ptr(),
                                          torch.cuda.current_stream().cuda_stream), "s2l_orthogonalize")
+    return outs
+
+
+def _orthogonalize_operator(updates, steps, a, b, c, eps):
+    _check_matrices(updates)
+    _check_iteration("orthogonalize", steps, (a, b, c), eps)
+    if any(t.device != updates[0].device for t in updates):
+        raise _abi.S2LError("orthogonalize: every tensor must be on one GPU (no CPU fallback)")
+    return _orthogonalize_all(updates, steps, a, b, c, eps)
+
+
+# The same as an operator that torch knows, for what watches, records or replaces a call's operators (dispatch modes: make_fx, fake tensors, selective
+# checkpoints, counters; subclasses that dispatch for themselves): it would see the allocation of the results and not the launches that write them.
+_operators = torch.library.Library("speech2lip_amd", "FRAGMENT")
+_operators.define("orthogonalize(Tensor[] updates, int steps, float a, float b, float c, float eps) -> Tensor[]")
+_operators.impl("orthogonalize", _orthogonalize_operator, "CUDA")
+_operators.impl("orthogonalize", lambda updates, *_: [torch.empty_like(t, memory_format=torch.contiguous_format) for t in updates], "Meta")
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
 
 
 @torch.no_grad()
@@ -226,28 +251,21 @@ def orthogonalize(update, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)
     update [..., rows, cols], or a list of such tensors of any sizes, all float32, all bfloat16 or all float16 on one GPU -> the same shape(s) and type,
     in one set of launches.  Operands of 22 bits, sums in fp32, rounded once: an fp32 iteration's accuracy; bfloat16: its last two steps on
     half-precision products (relative error 1.8e-3 to 2.2e-3, of which its rounding is 1.7e-3).
-    A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not); not
-    under a tracer or a dispatch mode."""
+    A matrix that holds a NaN or an infinity comes out all NaN, a zero matrix zero.  Not differentiable (an optimiser's step is not), not
+    under torch.jit.trace."""
     many = isinstance(update, (list, tuple))
     given = list(update) if many else [update]
-    for t in given:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError("orthogonalize: a tensor [..., rows, cols] or a list of them")
-        if t.dim() < 2:
-            raise ValueError(f"orthogonalize: matrices [..., rows, cols]: got {tuple(t.shape)}")
-        if t.dtype not in _ORTH_DTYPES or t.dtype != given[0].dtype:
-            raise ValueError(f"orthogonalize: all float32, all bfloat16 or all float16: got {t.dtype}")
-        if max(t.shape[-2:]) > 131072:
-            raise ValueError(f"orthogonalize: at most 131072 rows and columns: got {tuple(t.shape)}")
-    _refuse_recording("orthogonalize", given)
-    coefficients = _iteration("orthogonalize", steps, coefficients, eps)
+    _check_matrices(given)
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError("orthogonalize: not under torch.jit.trace, which would record the allocation of the result and not the launches that write it")
+    a, b, c = _iteration("orthogonalize", steps, coefficients, eps)
     for t in given:
         if not t.is_cuda or t.device != given[0].device:
             raise _abi.S2LError("orthogonalize: every tensor must be on one GPU (no CPU fallback)")
-    sources = [t.resolve_neg().contiguous() for t in given]
-    outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in sources]
-    if sources:
-        _orthogonalize_into(sources, outs, steps, coefficients, eps)
+    if torch._C._len_torch_dispatch_stack() or not _PLAIN.issuperset(map(type, given)):
+        outs = torch.ops.speech2lip_amd.orthogonalize(given, steps, a, b, c, float(eps)) if given else []
+    else:
+        outs = _orthogonalize_all(given, steps, a, b, c, float(eps))
     return outs if many else outs[0]
 
 
@@ -299,7 +317,7 @@ class FusedMuon(FusedAdam):
     def _step_group(self, gi, group, ps):
         if group.get("algorithm", "muon") == "adam":
             return super()._step_group(gi, group, ps)
-        _refuse_recording("FusedMuon", ())
+        _refuse_tracing("FusedMuon")
         _refuse_capture("FusedMuon", ps[0].device)
         lib = _abi.load()
         lr, mode = float(group["lr"]), group["adjust_lr_fn"]

@@ -1,9 +1,11 @@
-"""The calls around autograd.linear, optim.orthogonalize and FusedMuon: who may record them, which views, graphs, hooks and arguments they take, and
+"""The calls around autograd.linear, optim.orthogonalize and FusedMuon: what records or watches them, which views, graphs, hooks and arguments they take, and
 what they refuse."""
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
+from torch.utils._pytree import tree_map
 
 import speech2lip_amd as s2l
 from speech2lip_amd import _abi, autograd, optim
@@ -16,54 +18,142 @@ def dev():
 
 
 class Watching(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
     def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
         return func(*args, **(kwargs or {}))
 
 
 class Wrapped(torch.Tensor):
-    """A subclass that dispatches for itself."""
+    """A subclass that dispatches for itself: it holds a tensor and unwraps it for every operator."""
 
     @staticmethod
     def __new__(cls, t):
-        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, strides=t.stride(), dtype=t.dtype, device=t.device)
+
+    def __init__(self, t):
+        self.inner = t
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
-        raise AssertionError("never reached: the call is refused before its first operator")
+        inner = lambda t: t.inner if isinstance(t, Wrapped) else t  # noqa: E731
+        wrap = lambda t: Wrapped(t) if isinstance(t, torch.Tensor) else t  # noqa: E731
+        return tree_map(wrap, func(*tree_map(inner, args), **tree_map(inner, kwargs or {})))
 
 
-def _refused_recordings(x, w, p):
-    """A recorded program would hold the allocation of the result and not the launch that writes it."""
+def _refused_under_jit_trace(x, w, p):
+    """The recorded program would hold the allocation of the result and not the launch that writes it."""
     for f in (lambda t: autograd.linear(t, w), lambda t: optim.orthogonalize(t), lambda t: optim.orthogonalize([t, t])[0]):
         with pytest.raises(NotImplementedError):
             torch.jit.trace(f, x, check_trace=False)
-        with pytest.raises(NotImplementedError):
-            make_fx(f)(x)
-        with Watching(), pytest.raises(NotImplementedError):
-            f(x)
-        with pytest.raises(NotImplementedError):
-            f(Wrapped(x))
-    with pytest.raises(NotImplementedError):
-        autograd.linear(x, w, bias=Wrapped(w[:, 0].contiguous()))
     p.grad = torch.zeros_like(p)
     opt = s2l.FusedMuon([p])
-    with Watching(), pytest.raises(NotImplementedError):
+    with FakeTensorMode(), pytest.raises(NotImplementedError):
         opt.step()
 
 
-def test_recording_is_refused_without_a_gpu():
-    _refused_recordings(torch.zeros(2, 3), torch.zeros(4, 3), torch.nn.Parameter(torch.zeros(4, 3)))
+def test_recording_without_a_gpu():
+    x, w = torch.zeros(2, 3), torch.zeros(4, 3)
+    _refused_under_jit_trace(x, w, torch.nn.Parameter(torch.zeros(4, 3)))
+    for f in (lambda t: autograd.linear(t, w), lambda t: optim.orthogonalize(t)):      # other recorders: as any call without a GPU
+        for call in (lambda: make_fx(f)(x), lambda: f(Wrapped(x))):
+            with pytest.raises(RuntimeError, match="GPU"):
+                call()
+        with Watching(), pytest.raises(RuntimeError, match="GPU"):
+            f(x)
 
 
 @pytest.mark.gpu
-def test_recording_is_refused(dev):
-    x, w = torch.randn(2, 3, device=dev), torch.randn(4, 3, device=dev, requires_grad=True)
-    _refused_recordings(x, w.detach(), torch.nn.Parameter(torch.zeros(4, 3, device=dev)))
-    y = autograd.linear(x, w, activation="gelu")      # an eager forward pass, its backward pass under a mode
-    with Watching(), pytest.raises(NotImplementedError):
-        torch.autograd.grad(y, w, torch.ones_like(y), retain_graph=True)
-    (gw,) = torch.autograd.grad(y, w, torch.ones_like(y))
-    assert bool(torch.isfinite(gw).all())
+def test_jit_trace_is_refused(dev):
+    _refused_under_jit_trace(torch.randn(2, 3, device=dev), torch.randn(4, 3, device=dev), torch.nn.Parameter(torch.zeros(4, 3, device=dev)))
+
+
+def _both_passes(act):
+    def f(x, w, b, r, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = autograd.linear(*leaves, act)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    return f
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ("real", "fake"))
+def test_make_fx_records_the_operators(mode, dev):
+    """The recorded program, run on other values, gives the eager call's bits."""
+    values, dy = _layer(dev, 1)
+    fresh, fdy = _layer(dev, 2)
+    for act in ("none", "relu", "gelu"):
+        f = _both_passes(act)
+        program = make_fx(f, tracing_mode=mode)(*values, dy)
+        assert {"speech2lip_amd.linear_forward.default", "speech2lip_amd.linear_backward.default"} <= {str(n.target) for n in program.graph.nodes}
+        assert all(torch.equal(a, b) for a, b in zip(f(*fresh, fdy), program(*fresh, fdy)))
+    g = lambda t: optim.orthogonalize([t[0], t[1, :9]])  # noqa: E731
+    one, other = torch.randn(2, 20, 30, device=dev), torch.randn(2, 20, 30, device=dev)
+    program = make_fx(g, tracing_mode=mode)(one)
+    assert all(torch.equal(a, b) for a, b in zip(g(other), program(other)))
+
+
+@pytest.mark.gpu
+def test_modes_subclasses_counters_and_selective_checkpoints(dev):
+    from functools import partial
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    from torch.utils.flop_counter import FlopCounterMode
+    values, dy = _layer(dev, 3)
+    g = torch.randn(20, 30, device=dev)
+    for act in ("none", "leaky_relu", "silu"):
+        f = _both_passes(act)
+        want = f(*values, dy)
+        for mode in (Watching(), FlopCounterMode(display=False)):
+            with mode:
+                got, orth = f(*values, dy), optim.orthogonalize(g)
+            assert all(torch.equal(a, b) for a, b in zip(want, got)) and torch.equal(orth, optim.orthogonalize(g))
+            if isinstance(mode, Watching):
+                assert sum("linear_forward" in n for n in mode.seen) == 1 and sum("linear_backward" in n for n in mode.seen) == 1
+                assert sum("orthogonalize" in n for n in mode.seen) == 1
+        leaves = [v.clone().requires_grad_() for v in values]
+        y = autograd.linear(*leaves, act)      # an eager forward pass, its backward pass under a mode
+        with Watching():
+            assert all(torch.equal(a, b) for a, b in zip(want[1:], torch.autograd.grad(y, leaves, dy)))
+        wrapped = autograd.linear(*(Wrapped(v) for v in values), act)
+        assert isinstance(wrapped, Wrapped) and torch.equal(wrapped.inner, want[0])
+        for saving in (True, False):
+            policy = lambda ctx, op, *a, **k: CheckpointPolicy.MUST_SAVE if saving else CheckpointPolicy.PREFER_RECOMPUTE  # noqa: E731
+            y = checkpoint(lambda *t: autograd.linear(*t, act).square(), *leaves, use_reentrant=False, context_fn=partial(create_selective_checkpoint_contexts, policy))
+            plain = autograd.linear(*leaves, act).square()
+            assert torch.equal(y, plain)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), torch.autograd.grad(plain, leaves, dy)))
+    wrapped = optim.orthogonalize(Wrapped(g))
+    assert isinstance(wrapped, Wrapped) and torch.equal(wrapped.inner, optim.orthogonalize(g))
+
+
+@pytest.mark.gpu
+def test_the_operators_check_what_they_are_given(dev):
+    ops = torch.ops.speech2lip_amd
+    autograd._linear_ops()
+    (x, w, b, r), dy = _layer(dev, 4)
+    y, kept = ops.linear_forward(x, w, b, r, 3, 0.0, True)
+    assert torch.equal(y, autograd.linear(x, w, b, r, "gelu")) and kept.numel() == y.numel() * 4
+    back = lambda **k: ops.linear_backward(*{**dict(dy=dy, x=x, w=w, kept=kept, xs=x.shape, ws=w.shape, act=3, slope=0.0, nx=True, nw=True, nb=True), **k}.values())  # noqa: E731
+    assert [t.shape for t in back()] == [x.shape, w.shape, b.shape] and [t.numel() for t in back(nw=False, nb=False)] == [x.numel(), 0, 0]
+    for bad in ((x, w.mT, b, r, 0), (x, w, x, r, 0), (x, w, b, b, 0), (x, w.half(), b, r, 0), (x, w, b, r, 5), (x, w, b, r, -1), (x.cpu(), w, b, r, 0)):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.linear_forward(*bad, 0.0, True)
+    for bad in (dict(dy=dy[1:]), dict(x=x[1:]), dict(x=None), dict(w=w.mT), dict(w=None), dict(kept=None), dict(kept=kept[1:]), dict(kept=kept.view(torch.float32)), dict(xs=w.shape),
+                dict(ws=x.shape), dict(ws=(41,)), dict(xs=()), dict(act=7), dict(nx=False, nw=False), dict(nw=False), dict(dy=dy.half())):
+        with pytest.raises((ValueError, RuntimeError)):
+            back(**bad)
+    for bad in ([x[0]], [x, w.half()], [x.long()]):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.orthogonalize(bad, 5, 3.4445, -4.7750, 2.0315, 1e-7)
+    with pytest.raises(ValueError):
+        ops.orthogonalize([x], 0, 3.4445, -4.7750, 2.0315, 1e-7)
+    torch.library.opcheck(ops.linear_forward.default, (x, w, b, r, 3, 0.0, True), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(ops.linear_forward.default, (x, w, None, None, 0, 0.0, False), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(ops.linear_backward.default, (dy, x, w, kept, x.shape, w.shape, 3, 0.0, True, True, False), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(ops.orthogonalize.default, ([x, w], 5, 3.4445, -4.7750, 2.0315, 1e-7), test_utils=("test_schema", "test_faketensor"))
 
 
 @pytest.mark.gpu
@@ -296,3 +386,11 @@ def test_calls_beyond_a_launch_are_refused_on_the_host():
     assert fwd(most, 33, 1) == -2 and fwd(1 << 30, 32, 129) == -2 and fwd(8, 32, most, act=1, saved=p) == -2
     bwd = lambda rows, k, n: lib.s2l_linear_backward(0, p, n, p, k, p, k, p, p, k, 0, 0, p, rows, k, n, 0, 0.0, 0)  # noqa: E731
     assert bwd(most, 5, 4) == -2 and bwd(8, most, 4) == -2 and bwd(1 << 30, 129, 32) == -2
+
+
+@pytest.mark.gpu
+def test_the_librarys_refusals_are_the_packages_errors(dev):
+    with pytest.raises(_abi.S2LError, match="bad size"):
+        autograd.linear(torch.zeros(1, 1, device=dev), torch.zeros(1 << 26, 1, device=dev))
+    with Watching(), pytest.raises(RuntimeError, match="bad size"):
+        autograd.linear(torch.zeros(1, 1, device=dev), torch.zeros(1 << 26, 1, device=dev))
