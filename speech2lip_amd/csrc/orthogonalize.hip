@@ -904,15 +904,23 @@ template <int PARTS, int KIND, bool MUON, typename T> int small(int blocks, cons
   return (int)hipGetLastError();
 }
 
+template <int PARTS, int KIND, bool MUON, typename T> int sized(int tile, int blocks, const Call& c, const Front& f, const Step& s) {
+  if constexpr (KIND == CUT) return one<128, PARTS, 2, KIND, MUON, T>(blocks, c, f, s);
+  else if (tile == 32) return small<PARTS, KIND, MUON, T>(blocks, c, f, s);
+  else if (tile == 128 && groups_for(blocks) == 2) return one<128, PARTS, 4, KIND, MUON, T, 2>(blocks, c, f, s);
+  else if (tile == 128) return one<128, PARTS, 2, KIND, MUON, T>(blocks, c, f, s);
+  else return one<64, PARTS, 3, KIND, MUON, T>(blocks, c, f, s);
+}
+
+// how many halves step k works on
+template <typename T> int parts_of(int k, int steps) { return !std::is_same_v<T, __bf16> || k < steps - 2 ? 2 : 1; }
+
 template <int KIND, bool MUON, typename T> int any(int tile, int parts, int blocks, const Call& c, Front f, const Step& s) {
   constexpr int kind = KIND == CUT ? DEEP : KIND == GRAM || KIND == POLY ? SYM : RECT;
   f.per = c.alike.per[kind];
   f.bytes_or_records = f.per ? c.alike.bytes : c.alike.records[kind - SYM];
-  if constexpr (KIND == CUT) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
-  else if (tile == 32) return parts == 2 ? small<2, KIND, MUON, T>(blocks, c, f, s) : small<1, KIND, MUON, T>(blocks, c, f, s);
-  else if (tile == 128 && groups_for(blocks) == 2) return parts == 2 ? one<128, 2, 4, KIND, MUON, T, 2>(blocks, c, f, s) : one<128, 1, 4, KIND, MUON, T, 2>(blocks, c, f, s);
-  else if (tile == 128) return parts == 2 ? one<128, 2, 2, KIND, MUON, T>(blocks, c, f, s) : one<128, 1, 2, KIND, MUON, T>(blocks, c, f, s);
-  else return parts == 2 ? one<64, 2, 3, KIND, MUON, T>(blocks, c, f, s) : one<64, 1, 3, KIND, MUON, T>(blocks, c, f, s);
+  if constexpr (KIND == LAST) return sized<std::is_same_v<T, __bf16> ? 1 : 2, KIND, MUON, T>(tile, blocks, c, f, s);      // (parts_of the last step)
+  else return parts == 2 ? sized<2, KIND, MUON, T>(tile, blocks, c, f, s) : sized<1, KIND, MUON, T>(tile, blocks, c, f, s);
 }
 
 template <typename T, bool MUON>
@@ -927,7 +935,7 @@ int run(const s2l_matrix* in, int count, double a, double b, double c, float eps
     rc = lay_out(in + first, n, &t, &l);
     if (rc) return rc;
     const Call call{alike_of(t, l, n, sizeof(T), MUON), work, st, dev};
-    const auto parts = [&](int k) { return !std::is_same_v<T, __bf16> || k < steps - 2 ? 2 : 1; };
+    const auto parts = [&](int k) { return parts_of<T>(k, steps); };
     Lists lists{};
     for (int k = 0; k < 3 && !call.alike.per[0]; ++k) {
       lists.at[k] = l.records[k];

@@ -394,3 +394,41 @@ def test_the_librarys_refusals_are_the_packages_errors(dev):
         autograd.linear(torch.zeros(1, 1, device=dev), torch.zeros(1 << 26, 1, device=dev))
     with Watching(), pytest.raises(RuntimeError, match="bad size"):
         autograd.linear(torch.zeros(1, 1, device=dev), torch.zeros(1 << 26, 1, device=dev))
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads(dev):
+    """Each thread on a stream of its own, forward, backward and orthogonalisation at once: the bits of the calls alone."""
+    import threading
+    sizes = ((70, 33, 41, "gelu"), (4160, 192, 4120, "relu"), (9, 256, 64, "none"), (4128, 520, 288, "silu"))
+    jobs = []
+    for i, (rows, k, n, act) in enumerate(sizes):
+        g = torch.Generator(device=dev).manual_seed(i)
+        dtype = torch.bfloat16 if i % 2 else torch.float32
+        values = [torch.randn(s, generator=g, device=dev).to(dtype) for s in ((rows, k), (n, k), (n,), (rows, n))]
+        dy, update = torch.randn(rows, n, generator=g, device=dev).to(dtype), torch.randn(3, 40 + i, 600, generator=g, device=dev)
+        jobs.append((values, dy, act, update))
+
+    def run(values, dy, act, update):
+        return (*_both_passes(act)(*values, dy), optim.orthogonalize(update))
+    want = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = run(*jobs[i])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(want[i], got)):
+                        wrong.append(i)
+        except Exception as e:      # noqa: BLE001 (reported below)
+            wrong.append((i, e))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not wrong and not any(t.is_alive() for t in threads), wrong
