@@ -59,7 +59,6 @@ template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v
 
 // 16 bytes at element alignment: the target's unaligned global access makes this one load
 template <typename T> __device__ __forceinline__ u4 load16(const T* p) { u4 v; __builtin_memcpy(&v, p, 16); return v; }
-template <typename T> __device__ __forceinline__ void store16(T* p, u4 v) { __builtin_memcpy(p, &v, 16); }
 
 // the first `count` (< a piece) elements, the rest zero
 template <typename T> __device__ __forceinline__ u4 load_some(const T* p, int count) {
